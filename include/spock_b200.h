@@ -46,7 +46,8 @@ int spock_destroy(spock_ctx* ctx);
  * when ctx is NULL). Valid until the next call on the same context. */
 const char* spock_last_error(const spock_ctx* ctx);
 /* Blocks until the stream's work is done; returns SPOCK_ERR_TIMEOUT when a
- * kernel reported a bounded wait that gave up. */
+ * kernel reported a bounded wait that gave up, SPOCK_ERR_INVALID when a ragged
+ * step met an index out of range in its device data. */
 int spock_sync(spock_ctx* ctx, void* stream);
 /* Number of kernels this library has launched since load (diagnostics). */
 uint64_t spock_kernel_launch_count(void);
@@ -275,6 +276,146 @@ int spock_attention_decode(spock_ctx* ctx, int32_t exact, const void* proj, cons
 int spock_attention_prefill(spock_ctx* ctx, int32_t exact, const void* proj, const void* q_norm, const void* k_norm,
                             float eps, float rope_theta, const int32_t* pos, void* kv_cache, int32_t max_seq,
                             int64_t batch, int32_t len, void* out, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Ragged steps: several new tokens per sequence over a paged cache.         */
+/* ------------------------------------------------------------------------ */
+/* What a server needs to verify drafted tokens (or to mix prompt chunks and
+ * decode tokens in one batch): the prep + store and the attention of the
+ * gated full-attention layers over a KV cache held in pages, the DeltaNet step
+ * over a span of tokens, and the acceptance of the drafts. No counterpart in
+ * the reference, which serves one sequence token by token.
+ *
+ * All four take packed token rows: `start` (device int32 [batch + 1],
+ * ascending) gives sequence b the rows start[b] .. start[b+1]-1 (possibly
+ * none) of every row-shaped tensor of `total` rows; rows behind
+ * start[batch] are neither read nor written. Lengths, starts, page-table
+ * entries and token ids live on the device, so the kernels check them: one
+ * that is out of range is never used as an address, the outputs of that
+ * sequence are unspecified, and the next spock_sync (spock_model_sync for a
+ * model on the same context) returns SPOCK_ERR_INVALID.
+ * The calls keep no scratch in the context: workspaces are the caller's, so
+ * calls on several streams, or captured in several CUDA graphs, need only
+ * workspaces of their own. A workspace's contents need no initialisation and
+ * mean nothing after the call's work is done. */
+
+/* A KV cache in pages, and each sequence's pages and length. k and v point at
+ * (page 0, position 0, head 0, dim 0) and share the strides, which are in
+ * elements; a head's head_dim elements are contiguous. */
+typedef struct {
+  void* k;
+  void* v;                   /* 16-byte aligned                                      */
+  int64_t page_stride;       /* strides: multiples of 8, head_stride of 64           */
+  int64_t pos_stride;
+  int64_t head_stride;
+  const int32_t* page_table; /* device [batch][table_stride]: page of positions
+                                [i*page_size, (i+1)*page_size); entries behind a
+                                sequence's length are not read                       */
+  int64_t table_stride;
+  const int32_t* kv_len;     /* device [batch]: positions held, this call's new
+                                tokens included                                      */
+  int32_t table_width;       /* entries per row (<= table_stride)                    */
+  int32_t num_pages;
+  int32_t page_size;         /* a multiple of 8                                      */
+  int32_t kv_heads;
+  int32_t head_dim;          /* 64, 128 or 256                                       */
+  int32_t dtype;             /* SPOCK_F16 or SPOCK_BF16: cache, rows and outputs     */
+} spock_paged_kv;
+
+/* Projected rows -> rotated queries and the cache rows of the new tokens:
+ * split, per-head RMSNorm in the (1+w) form over head_dim, partial rotary,
+ * store. The paged form of the first half of spock_attention_prefill; it
+ * rounds once, at the end.
+ *   proj    [total] rows, proj_ld elements apart (a multiple of 8):
+ *           q_heads x [q | gate] (gated = 1) or q_heads x [q], then kv_heads x
+ *           k, kv_heads x v, head_dim each. The gates are left where they are
+ *           (spock_paged_attention reads them there)
+ *   q_norm, k_norm [head_dim] in the cache's dtype; both NULL: no norm
+ *   rope    fp32 [rope_len][rotary/2][cos, sin], pairs (d, d + rotary/2);
+ *           rotary a multiple of head_dim/16, 0 (rope NULL) for none
+ *   q_out   [total][q_heads][head_dim]
+ * Token t of a sequence with n new tokens sits at position kv_len - n + t,
+ * which must be >= 0 (and < rope_len); tokens with a negative position are
+ * skipped, nothing is written for them. Pages shared by two sequences must
+ * not be written by both. */
+int spock_paged_attention_prep(spock_ctx* ctx, const spock_paged_kv* kv, int32_t batch, const int32_t* start,
+                               int64_t total, const void* proj, int64_t proj_ld, int32_t q_heads, int32_t gated,
+                               const void* q_norm, const void* k_norm, float eps, const float* rope,
+                               int64_t rope_len, int32_t rotary, void* q_out, void* stream);
+
+/* Attention of each sequence's new tokens over its pages: token t of n sees
+ * positions 0 .. kv_len - n + t (causal; none if that is negative: the row is
+ * then zero), q_heads a multiple of kv_heads, at most 128 query heads per kv
+ * head. One entry for decode tokens, drafts, prompt chunks and any mix.
+ *   out[r][h] = sum_p softmax_p(scale * q[r][h] . k_p) v_p, times
+ *   sigmoid(gate[r][h]) when gate is not NULL; rounded once
+ *   q, gate rows and heads at their own strides (elements, multiples of 8)
+ *   out     [total][q_heads][head_dim], contiguous
+ * Slots behind kv_len are not used, whatever they hold; the positions below
+ * it hold finite keys and values.
+ * workspace: at least spock_paged_attention_workspace() bytes, 16-byte aligned. */
+int spock_paged_attention(spock_ctx* ctx, const spock_paged_kv* kv, int32_t batch, const int32_t* start, int64_t total,
+                          int32_t q_heads, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                          const void* gate, int64_t gate_row_stride, int64_t gate_head_stride, float scale, void* out,
+                          void* workspace, size_t workspace_bytes, void* stream);
+/* Bytes of workspace for any call with this head_dim (and kv head count) on the context's GPU. */
+int spock_paged_attention_workspace(spock_ctx* ctx, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                    size_t* bytes);
+
+/* One or more tokens per sequence through a DeltaNet layer's mixer core:
+ * spock_deltanet_decode_step over a span of tokens, with the state written
+ * only where asked, so drafted tokens can be verified (outputs, no state) and
+ * the accepted ones committed afterwards (state, no outputs). Per token: the
+ * conv window, SiLU, L2 of q and k, g and beta, S <- e^g S + k d^T with
+ * d = beta (v - (e^g S)^T k), o = S^T q / sqrt(key_dim), gated RMSNorm. All of
+ * it in fp32, rounded to fp16 once (the single-token step also rounds the conv
+ * output, q, k and w*norm, as the shaders store them). key_dim = value_dim =
+ * 128, conv width 4.
+ *   qkv     [total] rows of conv_dim fp16, qkv_ld elements apart; not changed
+ *   a, b    [total] rows of num_heads fp16, ab_ld apart; z [total] rows of
+ *           num_heads*128 fp16, z_ld apart (NULL when out is NULL)
+ *   counts  device int32 [batch] or NULL: sequence b takes its first
+ *           min(counts[b], start[b+1]-start[b]) rows; NULL = all
+ *   state, conv_state  as in spock_deltanet_decode_step; read
+ *   state_out, conv_state_out  the same shapes, both or neither: state after
+ *           the taken rows (unchanged values when none); may be state and
+ *           conv_state themselves
+ *   out     [total][num_heads*128] fp16 or NULL; rows not taken keep their values
+ * At least one of out and state_out is given. */
+int spock_deltanet_decode_span(spock_ctx* ctx, const spock_dn_layer* layer, int32_t batch, const int32_t* start,
+                               const int32_t* counts, int64_t total, const void* qkv, int64_t qkv_ld, const void* a,
+                               const void* b, int64_t ab_ld, const void* z, int64_t z_ld, const void* conv_state,
+                               const float* state, void* conv_state_out, float* state_out, void* out, void* stream);
+
+/* Acceptance of drafted tokens from given random numbers (speculative
+ * sampling). Sequence b's rows are the model's inputs of the step: its last
+ * accepted token, then its drafts; row i's logits are tested against the token
+ * of row i+1. With p = softmax(logits[i] / temperature[b]) and q =
+ * draft_probs[i] (one-hot at the draft when draft_probs is NULL), draft x of
+ * row i+1 is accepted iff u_accept[i] * q(x) < p(x), up to the first that is
+ * not. The next token is then drawn at that row from max(p - q, 0) (from p if
+ * that is zero everywhere), or from p at the last row when all were accepted:
+ * the lowest j with weight > 0 whose inclusive running sum exceeds
+ * u_sample[b] * (sum of the weights), the last j with weight > 0 if none does.
+ * temperature[b] <= 0: greedy, a draft is accepted iff it is the arg max
+ * (lowest index among equals), which is also the next token. Decided in 64
+ * bits. NaN logits count as -inf.
+ *   logits [total] rows of vocab, logits_ld apart (fp32, fp16, bf16)
+ *   tokens int32 [total]; draft_probs fp32 [total] rows, probs_ld apart (a
+ *   sequence's last row is not read) or NULL
+ *   temperature fp32 [batch] or NULL (1.0); u_accept fp32 [total]; u_sample fp32 [batch]
+ *   emitted    int32 [batch]: accepted drafts + 1, the number of valid
+ *              entries of the sequence's rows in out_tokens and of input rows
+ *              to commit (spock_deltanet_decode_span's counts); 0 for no rows
+ *   out_tokens int32 [total]: accepted drafts, the next token, then -1 to the
+ *              sequence's end
+ * workspace: at least spock_draft_verify_workspace() bytes, 16-byte aligned. */
+int spock_draft_verify(spock_ctx* ctx, int32_t dtype, const void* logits, int64_t logits_ld, int64_t total,
+                       int64_t vocab, int32_t batch, const int32_t* start, const int32_t* tokens,
+                       const float* draft_probs, int64_t probs_ld, const float* temperature, const float* u_accept,
+                       const float* u_sample, int32_t* emitted, int32_t* out_tokens, void* workspace,
+                       size_t workspace_bytes, void* stream);
+int spock_draft_verify_workspace(spock_ctx* ctx, int64_t total, int64_t vocab, int32_t batch, size_t* bytes);
 
 /* ------------------------------------------------------------------------ */
 /* Full-model decode (Qwen3.5-0.8B layout): the decode glue around the mixer. */

@@ -39,7 +39,9 @@ EXPORTED = ["spock_create", "spock_destroy", "spock_last_error", "spock_sync",
             "spock_model_create", "spock_model_destroy", "spock_model_last_error", "spock_model_set_weight",
             "spock_model_reset", "spock_model_step", "spock_model_generate", "spock_model_load_artifact",
             "spock_model_prefill", "spock_noalloc_sync", "spock_model_sync",
-            "spock_rms_norm", "spock_matvec", "spock_argmax", "spock_attention_decode", "spock_attention_prefill"]
+            "spock_rms_norm", "spock_matvec", "spock_argmax", "spock_attention_decode", "spock_attention_prefill",
+            "spock_paged_attention_prep", "spock_paged_attention", "spock_paged_attention_workspace",
+            "spock_deltanet_decode_span", "spock_draft_verify", "spock_draft_verify_workspace"]
 
 
 class SpockError(RuntimeError):
@@ -60,6 +62,14 @@ class DnLayer(ctypes.Structure):
                 ("conv_kernel", ctypes.c_int32), ("conv_weight", ctypes.c_void_p),
                 ("a_log_bias", ctypes.c_void_p), ("norm_weight", ctypes.c_void_p),
                 ("eps", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+class PagedKv(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("pos_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("page_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("kv_len", ctypes.c_void_p), ("table_width", ctypes.c_int32),
+                ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32)]
 
 
 _LIB = None
@@ -100,6 +110,16 @@ def lib():
         L.spock_chunk_last_to_fp16.argtypes = [vp, i64, i64, i64, i64, vp, vp, vp]
         L.spock_deltanet_decode_step.argtypes = [vp, ctypes.POINTER(DnLayer), i64] + [vp] * 9
         L.spock_deltanet_recurrent.argtypes = [vp, i64, i32, i32, i32] + [vp] * 8
+        f32, szp = ctypes.c_float, ctypes.POINTER(ctypes.c_size_t)
+        L.spock_paged_attention_prep.argtypes = [vp, vp, i32, vp, i64, vp, i64, i32, i32, vp, vp, f32, vp, i64, i32,
+                                                 vp, vp]
+        L.spock_paged_attention.argtypes = [vp, vp, i32, vp, i64, i32, vp, i64, i64, vp, i64, i64, f32, vp, vp,
+                                            ctypes.c_size_t, vp]
+        L.spock_paged_attention_workspace.argtypes = [vp, i32, i32, i32, szp]
+        L.spock_deltanet_decode_span.argtypes = [vp, vp, i32, vp, vp, i64, vp, i64, vp, vp, i64, vp, i64] + [vp] * 6
+        L.spock_draft_verify.argtypes = [vp, i32, vp, i64, i64, i64, i32, vp, vp, vp, i64] + [vp] * 6 + [
+            ctypes.c_size_t, vp]
+        L.spock_draft_verify_workspace.argtypes = [vp, i64, i64, i32, szp]
         _LIB = L
     return _LIB
 
@@ -133,6 +153,7 @@ class Context:
             raise SpockError(rc, L.spock_last_error(None).decode())
         self.h = h
         self.device = device
+        self.ws_bytes = {}  # workspace sizes by shape
 
     @classmethod
     def get(cls, device=0):
@@ -306,6 +327,252 @@ def deltanet_recurrent(q, k, v, g, beta, state, num_heads=16, key_dim=128, value
                                              _ptr(v), _ptr(g), _ptr(beta), _ptr(state), _ptr(out),
                                              _stream(stream)))
     return out
+
+
+# ---- ragged steps: several new tokens per sequence, packed rows ----------------
+# `start` int32 [batch + 1]: sequence b owns rows start[b] .. start[b + 1] - 1 of
+# every row-shaped tensor. All tensors of a call are on one device; the work goes
+# to that device's current stream unless `stream` is given. Starts, lengths, page
+# tables and token ids are checked on the device: Context.sync() raises for one
+# that was out of range.
+
+def _bad(msg):
+    raise SpockError(SPOCK_ERR_INVALID, msg)
+
+
+def _ragged(first, tensors):
+    """Checks (name, tensor, dtype, ndim, contiguous) entries against `first`'s device; the device's context."""
+    dev = first.device
+    for name, t, dtype, ndim, contiguous in tensors:
+        if t is None:
+            continue
+        if t.device != dev:
+            _bad(f"{name}: expected a tensor on {dev}")
+        if t.dtype != dtype:
+            _bad(f"{name}: expected {dtype}, got {t.dtype}")
+        if t.dim() != ndim:
+            _bad(f"{name}: expected {ndim} dimensions, got {t.dim()}")
+        if contiguous:
+            if not t.is_contiguous():
+                _bad(f"{name}: expected a contiguous tensor")
+        elif ndim and t.shape[-1] > 1 and t.stride(-1) != 1:
+            _bad(f"{name}: expected a contiguous last dimension")
+    if dev.type != "cuda":
+        _bad("expected CUDA tensors")
+    return Context.get(dev.index or 0)
+
+
+def _stream_of(t, stream):
+    import torch
+    return stream.cuda_stream if stream is not None else torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _new(shape, dtype, like, stream):
+    """An uninitialised tensor for work on `stream` (None: the current one)."""
+    import torch
+    t = torch.empty(shape, dtype=dtype, device=like.device)
+    if stream is not None:  # allocated on the current stream: not to be reused before `stream` is done with it
+        t.record_stream(stream)
+    return t
+
+
+def _row_stride(t):
+    """Elements from one row to the next (any value does for a single row)."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[-1] + 7) // 8 * 8 if t.dim() == 2 else t.shape[1] * t.shape[2]
+
+
+def _paged_kv(k_pages, v_pages, page_table, kv_len, start):
+    """spock_paged_kv over pages [num_pages, page_size, kv_heads, head_dim] (any strides, head_dim contiguous)."""
+    import torch
+    batch = start.shape[0] - 1
+    if k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+        _bad("k_pages and v_pages must have the same shape and strides")
+    if batch < 1 or page_table.shape[0] != batch or kv_len.shape[0] != batch:
+        _bad("start, page_table and kv_len disagree on the batch")
+    pages, page, heads, dim = k_pages.shape
+    if k_pages.dtype not in (torch.float16, torch.bfloat16):
+        raise SpockError(SPOCK_ERR_UNSUPPORTED, "the cache is fp16 or bf16")
+    st = k_pages.stride()
+    # strides of dimensions of one element say nothing
+    return PagedKv(k_pages.data_ptr(), v_pages.data_ptr(), st[0] if pages > 1 else page * heads * dim,
+                   st[1] if page > 1 else heads * dim, st[2] if heads > 1 else dim, page_table.data_ptr(),
+                   max(page_table.stride(0), page_table.shape[1]) if batch == 1 else page_table.stride(0),
+                   kv_len.data_ptr(), page_table.shape[1], pages, page, heads, dim,
+                   F16 if k_pages.dtype == torch.float16 else BF16)
+
+
+def paged_attention_prep(proj, start, k_pages, v_pages, page_table, kv_len, rope=None, q_norm=None, k_norm=None,
+                         gated=True, eps=1e-6, q_out=None, stream=None):
+    """Projected rows -> rotated queries, K and V stored into the pages (spock_paged_attention_prep).
+
+    proj [total, (q_heads * (2 if gated else 1) + 2 * kv_heads) * head_dim] fp16/bf16 (q | gate per head, then k, v);
+    k_pages, v_pages [num_pages, page_size, kv_heads, head_dim], written in place; page_table int32 [batch, width];
+    kv_len int32 [batch], the new tokens included; rope fp32 [positions, rotary / 2, 2] (cos, sin) or None;
+    q_norm, k_norm [head_dim] ((1 + w) RMSNorm) or None. Returns q [total, q_heads, head_dim]."""
+    import torch
+    i32, f32, dt = torch.int32, torch.float32, k_pages.dtype
+    ctx = _ragged(proj, (("proj", proj, dt, 2, False), ("start", start, i32, 1, True),
+                         ("k_pages", k_pages, dt, 4, False), ("v_pages", v_pages, dt, 4, False),
+                         ("page_table", page_table, i32, 2, False), ("kv_len", kv_len, i32, 1, True),
+                         ("rope", rope, f32, 3, True), ("q_norm", q_norm, dt, 1, True),
+                         ("k_norm", k_norm, dt, 1, True), ("q_out", q_out, dt, 3, True)))
+    kv = _paged_kv(k_pages, v_pages, page_table, kv_len, start)
+    dim, total, per = kv.head_dim, proj.shape[0], 2 if gated else 1
+    heads = proj.shape[1] // dim - 2 * kv.kv_heads
+    q_heads = heads // per
+    if proj.shape[1] % dim or heads <= 0 or heads % per:
+        _bad("proj: the row is not q heads (with gates), k heads and v heads")
+    if any(w is not None and w.shape[0] != dim for w in (q_norm, k_norm)):
+        _bad("q_norm and k_norm have head_dim elements")
+    if rope is not None and rope.shape[2] != 2:
+        _bad("rope: expected [positions, rotary / 2, 2]")
+    if q_out is None:
+        q_out = _new((total, q_heads, dim), dt, proj, stream)
+    elif q_out.shape != (total, q_heads, dim):
+        _bad("q_out: expected [total, q_heads, head_dim]")
+    ctx.check(lib().spock_paged_attention_prep(
+        ctx.h, ctypes.byref(kv), start.shape[0] - 1, start.data_ptr(), total, proj.data_ptr(), _row_stride(proj),
+        q_heads, int(bool(gated)), None if q_norm is None else q_norm.data_ptr(),
+        None if k_norm is None else k_norm.data_ptr(), eps, None if rope is None else rope.data_ptr(),
+        0 if rope is None else rope.shape[0], 0 if rope is None else 2 * rope.shape[1], q_out.data_ptr(),
+        _stream_of(proj, stream)))
+    return q_out
+
+
+def _workspace(ctx, query, key, like, stream):
+    """A workspace tensor from the caching allocator (so a captured graph keeps its own)."""
+    import torch
+    n = ctx.ws_bytes.get(key)
+    if n is None:
+        size = ctypes.c_size_t()
+        ctx.check(query(ctx.h, *key[1:], ctypes.byref(size)))
+        n = size.value
+        if len(ctx.ws_bytes) < 1024:  # sizes only, by shape
+            ctx.ws_bytes[key] = n
+    return _new(n, torch.uint8, like, stream), n
+
+
+def paged_attention(q, start, k_pages, v_pages, page_table, kv_len, scale, gate=None, out=None, workspace=None,
+                    stream=None):
+    """Causal attention of each sequence's new tokens over its pages (spock_paged_attention).
+
+    q [total, q_heads, head_dim] and gate (or None), any row and head strides; the cache as in paged_attention_prep.
+    Token t of n sees positions 0 .. kv_len - n + t. Returns out [total, q_heads, head_dim]: softmax(scale q k) v,
+    times sigmoid(gate); rows behind start[batch] are left as they are. `workspace`: a uint8 tensor of
+    the caller's instead of one from the caching allocator."""
+    import torch
+    i32, dt = torch.int32, k_pages.dtype
+    ctx = _ragged(q, (("q", q, dt, 3, False), ("start", start, i32, 1, True), ("k_pages", k_pages, dt, 4, False),
+                      ("v_pages", v_pages, dt, 4, False), ("page_table", page_table, i32, 2, False),
+                      ("kv_len", kv_len, i32, 1, True), ("gate", gate, dt, 3, False), ("out", out, dt, 3, True)))
+    kv = _paged_kv(k_pages, v_pages, page_table, kv_len, start)
+    total, q_heads, dim = q.shape
+    if dim != kv.head_dim:
+        _bad("q: expected head_dim elements per head")
+    if gate is not None and gate.shape != q.shape:
+        _bad("gate: expected the shape of q")
+    if out is None:
+        out = _new((total, q_heads, dim), dt, q, stream)
+    elif out.shape != q.shape:
+        _bad("out: expected the shape of q")
+    if workspace is None:
+        workspace, n = _workspace(ctx, lib().spock_paged_attention_workspace, ("attn", q_heads, kv.kv_heads, dim), q,
+                                  stream)
+    else:
+        _ragged(q, (("workspace", workspace, torch.uint8, 1, True),))
+        n = workspace.shape[0]
+    ctx.check(lib().spock_paged_attention(
+        ctx.h, ctypes.byref(kv), start.shape[0] - 1, start.data_ptr(), total, q_heads, q.data_ptr(), _row_stride(q),
+        q.stride(1) if q_heads > 1 else dim, None if gate is None else gate.data_ptr(),
+        0 if gate is None else _row_stride(gate), 0 if gate is None else gate.stride(1) if q_heads > 1 else dim, scale,
+        out.data_ptr(), workspace.data_ptr(), n, _stream_of(q, stream)))
+    return out
+
+
+def deltanet_decode_span(layer, qkv, conv_state, state, a, b, z, start, counts=None, state_out=None, conv_out=None,
+                         out=None, stream=None):
+    """One or more tokens per sequence through a DeltaNet mixer core (spock_deltanet_decode_span).
+
+    qkv [total, 3 * heads * 128], a and b [total, heads], z [total, heads * 128] fp16 (any row stride); conv_state
+    [batch, 3 * heads * 128, 4] fp16, state [batch, heads, 128, 128] fp32, both only read. With `out` (or when nothing
+    else is asked for) the gated outputs [total, heads * 128] are written and returned; with state_out and conv_out
+    (which may be state and conv_state) the state after each sequence's first counts[b] rows (None: all)."""
+    import torch
+    f16, f32, i32 = torch.float16, torch.float32, torch.int32
+    ctx = _ragged(qkv, (("qkv", qkv, f16, 2, False), ("a", a, f16, 2, False), ("b", b, f16, 2, False),
+                        ("z", z, f16, 2, False), ("conv_state", conv_state, f16, 3, True),
+                        ("state", state, f32, 4, True), ("start", start, i32, 1, True),
+                        ("counts", counts, i32, 1, True), ("state_out", state_out, f32, 4, True),
+                        ("conv_out", conv_out, f16, 3, True), ("out", out, f16, 2, True),
+                        ("conv_weight", layer.conv_weight, layer.conv_weight.dtype, layer.conv_weight.dim(), True),
+                        ("a_log_bias", layer.a_log_bias, f32, 2, True), ("norm_weight", layer.norm_weight, f32, 1, True)))
+    h, total, batch = layer.num_heads, qkv.shape[0], start.shape[0] - 1
+    inner = h * layer.value_dim
+    if out is None and state_out is None:
+        out = _new((total, inner), f16, qkv, stream)
+    shapes = ((qkv, (total, 3 * inner)), (a, (total, h)), (b, (total, h)), (z, (total, inner)),
+              (conv_state, (batch, 3 * inner, 4)), (conv_out, (batch, 3 * inner, 4)),
+              (state, (batch, h, 128, 128)), (state_out, (batch, h, 128, 128)), (out, (total, inner)),
+              (counts, (batch,)), (layer.a_log_bias, (h, 2)), (layer.norm_weight, (layer.value_dim,)))
+    for t, shape in shapes:
+        if t is not None and t.shape != shape:
+            _bad(f"expected a tensor of shape {shape}, got {tuple(t.shape)}")
+    if layer.conv_weight.numel() != 3 * inner * layer.conv_kernel or layer.conv_weight.element_size() != 2:
+        _bad("conv_weight: expected fp16 [conv_dim, conv_kernel]")
+    if total > 1 and a.stride(0) != b.stride(0):
+        _bad("a and b must have the same row stride")
+    st = layer.c_struct()
+    p = lambda t: None if t is None else t.data_ptr()
+    ctx.check(lib().spock_deltanet_decode_span(
+        ctx.h, ctypes.byref(st), batch, start.data_ptr(), p(counts), total, qkv.data_ptr(), _row_stride(qkv),
+        a.data_ptr(), b.data_ptr(), _row_stride(a), p(z), 0 if z is None else _row_stride(z), conv_state.data_ptr(),
+        state.data_ptr(), p(conv_out), p(state_out), p(out), _stream_of(qkv, stream)))
+    return out if out is not None else (state_out, conv_out)
+
+
+def draft_verify(logits, tokens, start, u_accept, u_sample, temperature=None, draft_probs=None, emitted=None,
+                 out_tokens=None, workspace=None, stream=None):
+    """Acceptance of drafted tokens from given random numbers (spock_draft_verify).
+
+    logits [total, vocab] fp32/fp16/bf16: a sequence's rows are its last accepted token and its drafts; tokens int32
+    [total], the input token of each row; u_accept fp32 [total], u_sample fp32 [batch]; temperature fp32 [batch] (0:
+    greedy) or None (1.0); draft_probs fp32 [total, vocab], row i the distribution that row i + 1's token was drawn
+    from, or None for drafts without one. Returns (emitted int32 [batch], out_tokens int32 [total]): the accepted
+    drafts, the next token, then -1."""
+    import torch
+    f32, i32 = torch.float32, torch.int32
+    if logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise SpockError(SPOCK_ERR_UNSUPPORTED, "logits are fp32, fp16 or bf16")
+    ctx = _ragged(logits, (("logits", logits, logits.dtype, 2, False), ("tokens", tokens, i32, 1, True),
+                           ("start", start, i32, 1, True), ("u_accept", u_accept, f32, 1, True),
+                           ("u_sample", u_sample, f32, 1, True), ("temperature", temperature, f32, 1, True),
+                           ("draft_probs", draft_probs, f32, 2, False), ("emitted", emitted, i32, 1, True),
+                           ("out_tokens", out_tokens, i32, 1, True)))
+    (total, vocab), batch = logits.shape, start.shape[0] - 1
+    if (tokens.shape[0] != total or u_accept.shape[0] != total or u_sample.shape[0] != batch or
+            (temperature is not None and temperature.shape[0] != batch) or
+            (draft_probs is not None and draft_probs.shape != logits.shape) or
+            (emitted is not None and emitted.shape[0] != batch) or
+            (out_tokens is not None and out_tokens.shape[0] != total)):
+        _bad("tokens, u_accept and out_tokens have a value per row, u_sample, temperature and emitted one per sequence")
+    if emitted is None:
+        emitted = _new(batch, i32, logits, stream)
+    if out_tokens is None:
+        out_tokens = _new(total, i32, logits, stream)
+    if workspace is None:
+        workspace, n = _workspace(ctx, lib().spock_draft_verify_workspace, ("verify", total, vocab, batch), logits,
+                                  stream)
+    else:
+        _ragged(logits, (("workspace", workspace, torch.uint8, 1, True),))
+        n = workspace.shape[0]
+    p = lambda t: None if t is None else t.data_ptr()
+    ctx.check(lib().spock_draft_verify(
+        ctx.h, _dtype_code(logits.dtype), logits.data_ptr(), logits.stride(0) if total > 1 else vocab, total, vocab,
+        batch, start.data_ptr(), tokens.data_ptr(), p(draft_probs),
+        0 if draft_probs is None else draft_probs.stride(0) if total > 1 else vocab, p(temperature),
+        u_accept.data_ptr(), u_sample.data_ptr(), emitted.data_ptr(), out_tokens.data_ptr(), workspace.data_ptr(), n,
+        _stream_of(logits, stream)))
+    return emitted, out_tokens
 
 
 # ---- reference-shaped API (host vectors in, host vectors out) ----------------

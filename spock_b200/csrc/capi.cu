@@ -10,6 +10,7 @@
 #include "chunk_scratch.h"
 #include "common.cuh"
 #include "ops.h"
+#include "ragged.h"
 
 namespace spock {
 std::atomic<uint64_t> g_launches{0};
@@ -91,6 +92,31 @@ struct DeviceGuard {
   }
 };
 
+bool misaligned(const void* p, uintptr_t bytes) { return (uintptr_t)p % bytes != 0; }
+
+// What the two paged-attention calls check of the cache and the packed rows.
+int check_paged(spock_ctx* ctx, const char* op, const spock_paged_kv* kv, int32_t batch, const int32_t* start,
+                int64_t total) {
+  const std::string o(op);
+  if (!kv || !kv->k || !kv->v || !kv->page_table || !kv->kv_len || !start)
+    return fail(ctx, SPOCK_ERR_INVALID, o + "NULL pointer");
+  if (batch <= 0 || total < 0 || total > INT32_MAX || kv->table_width <= 0 || kv->table_stride < kv->table_width ||
+      kv->num_pages <= 0 || kv->page_size <= 0 || kv->kv_heads <= 0 || kv->head_dim <= 0)
+    return fail(ctx, SPOCK_ERR_INVALID, o + "bad arguments");
+  if (kv->dtype != SPOCK_F16 && kv->dtype != SPOCK_BF16)
+    return fail(ctx, SPOCK_ERR_UNSUPPORTED, o + "the cache is fp16 or bf16");
+  if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256)
+    return fail(ctx, SPOCK_ERR_UNSUPPORTED, o + "head_dim is 64, 128 or 256");
+  if (kv->page_size % 8) return fail(ctx, SPOCK_ERR_UNSUPPORTED, o + "page_size must be a multiple of 8");
+  if ((int64_t)kv->table_width * kv->page_size > INT32_MAX)
+    return fail(ctx, SPOCK_ERR_UNSUPPORTED, o + "at most 2^31 - 1 positions per sequence");
+  if (misaligned(kv->k, 16) || misaligned(kv->v, 16) || kv->page_stride <= 0 || kv->pos_stride <= 0 ||
+      kv->head_stride <= 0 || kv->page_stride % 8 || kv->pos_stride % 8 || kv->head_stride % 64)
+    return fail(ctx, SPOCK_ERR_INVALID,
+                o + "k and v must be 16-byte aligned, page and position strides multiples of 8, head strides of 64");
+  return SPOCK_OK;
+}
+
 bool sm100(int dev) {
   cudaDeviceProp p;
   if (cudaGetDeviceProperties(&p, dev) != cudaSuccess) return false;
@@ -171,8 +197,7 @@ __attribute__((visibility("default"))) int spock_sync(spock_ctx* ctx, void* stre
   if (e != cudaSuccess) return fail(ctx, SPOCK_ERR_CUDA, std::string("spock_sync: ") + cudaGetErrorString(e));
   if (flag) {
     cudaMemset(ctx->d_err_flag, 0, sizeof(int));
-    return fail(ctx, SPOCK_ERR_TIMEOUT, "spock_sync: a kernel's bounded wait gave up (code " +
-                                            std::to_string(flag) + ")");
+    return finish(ctx, spock::err_word_status("spock_sync", flag));
   }
   return SPOCK_OK;
 }
@@ -292,6 +317,132 @@ __attribute__((visibility("default"))) int spock_attention_prefill(spock_ctx* ct
   DeviceGuard dg(ctx->device);
   return finish(ctx, spock::op_attention_decode(ctx->ops, exact, proj, q_norm, k_norm, eps, rope_theta, pos, kv_cache,
                                                 max_seq, batch * len, out, (cudaStream_t)stream, len));
+}
+
+__attribute__((visibility("default"))) int spock_paged_attention_prep(
+    spock_ctx* ctx, const spock_paged_kv* kv, int32_t batch, const int32_t* start, int64_t total, const void* proj,
+    int64_t proj_ld, int32_t q_heads, int32_t gated, const void* q_norm, const void* k_norm, float eps,
+    const float* rope, int64_t rope_len, int32_t rotary, void* q_out, void* stream) {
+  const char* const op = "spock_paged_attention_prep: ";
+  if (!ctx) return fail(nullptr, SPOCK_ERR_INVALID, std::string(op) + "ctx is NULL");
+  if (const int rc = check_paged(ctx, op, kv, batch, start, total)) return rc;
+  if (q_heads <= 0 || rotary < 0 || rotary > kv->head_dim || !q_norm != !k_norm || (rotary && (!rope || rope_len <= 0)))
+    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "bad arguments");
+  if (rotary % (kv->head_dim / 16))
+    return fail(ctx, SPOCK_ERR_UNSUPPORTED, std::string(op) + "rotary must be a multiple of head_dim / 16");
+  if (!total) return SPOCK_OK;
+  if (!proj || !q_out) return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "NULL pointer");
+  if (misaligned(proj, 16) || misaligned(q_out, 16) || misaligned(q_norm, 16) || misaligned(k_norm, 16) ||
+      misaligned(rope, 8) || proj_ld % 8)
+    return fail(ctx, SPOCK_ERR_INVALID,
+                std::string(op) + "rows and weights must be 16-byte aligned (proj_ld a multiple of 8), rope 8-byte");
+  if (total * (q_heads + (int64_t)kv->kv_heads) > ((int64_t)1 << 33))
+    return fail(ctx, SPOCK_ERR_UNSUPPORTED, std::string(op) + "too many rows");
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok) return fail(ctx, SPOCK_ERR_CUDA, std::string(op) + "cannot select device");
+  return finish(ctx, spock::launch_paged_prep(*kv, batch, start, total, proj, proj_ld, q_heads, gated != 0, q_norm,
+                                              k_norm, eps, rope, rope_len, rotary, q_out, ctx->d_err_flag,
+                                              (cudaStream_t)stream));
+}
+
+__attribute__((visibility("default"))) int spock_paged_attention_workspace(spock_ctx* ctx, int32_t q_heads,
+                                                                           int32_t kv_heads, int32_t head_dim,
+                                                                           size_t* bytes) {
+  if (!ctx) return fail(nullptr, SPOCK_ERR_INVALID, "spock_paged_attention_workspace: ctx is NULL");
+  if (!bytes || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0)
+    return fail(ctx, SPOCK_ERR_INVALID, "spock_paged_attention_workspace: bad arguments");
+  *bytes = spock::paged_attention_workspace(q_heads, kv_heads, head_dim, ctx->sms);
+  return SPOCK_OK;
+}
+
+__attribute__((visibility("default"))) int spock_paged_attention(
+    spock_ctx* ctx, const spock_paged_kv* kv, int32_t batch, const int32_t* start, int64_t total, int32_t q_heads,
+    const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* gate, int64_t gate_row_stride,
+    int64_t gate_head_stride, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* const op = "spock_paged_attention: ";
+  if (!ctx) return fail(nullptr, SPOCK_ERR_INVALID, std::string(op) + "ctx is NULL");
+  if (const int rc = check_paged(ctx, op, kv, batch, start, total)) return rc;
+  if (q_heads <= 0 || q_heads % kv->kv_heads)
+    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "q_heads must be a multiple of kv_heads");
+  if (q_heads / kv->kv_heads > 128)
+    return fail(ctx, SPOCK_ERR_UNSUPPORTED, std::string(op) + "at most 128 query heads per kv head");
+  if (!total) return SPOCK_OK;
+  if (!q || !out || !workspace) return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "NULL pointer");
+  if (misaligned(q, 16) || misaligned(gate, 16) || misaligned(out, 16) || misaligned(workspace, 16) ||
+      q_row_stride % 8 || q_head_stride % 8 || (gate && (gate_row_stride % 8 || gate_head_stride % 8)))
+    return fail(ctx, SPOCK_ERR_INVALID,
+                std::string(op) + "pointers must be 16-byte aligned and strides multiples of 8");
+  if (workspace_bytes < spock::paged_attention_workspace(q_heads, kv->kv_heads, kv->head_dim, ctx->sms))
+    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "workspace too small");
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok) return fail(ctx, SPOCK_ERR_CUDA, std::string(op) + "cannot select device");
+  return finish(ctx, spock::launch_paged_attention(*kv, batch, start, total, q_heads, q, q_row_stride, q_head_stride,
+                                                   gate, gate_row_stride, gate_head_stride, scale, out, workspace,
+                                                   ctx->sms, ctx->d_err_flag, (cudaStream_t)stream));
+}
+
+__attribute__((visibility("default"))) int spock_deltanet_decode_span(
+    spock_ctx* ctx, const spock_dn_layer* layer, int32_t batch, const int32_t* start, const int32_t* counts,
+    int64_t total, const void* qkv, int64_t qkv_ld, const void* a, const void* b, int64_t ab_ld, const void* z,
+    int64_t z_ld, const void* conv_state, const float* state, void* conv_state_out, float* state_out, void* out,
+    void* stream) {
+  const char* const op = "spock_deltanet_decode_span: ";
+  if (!ctx) return fail(nullptr, SPOCK_ERR_INVALID, std::string(op) + "ctx is NULL");
+  if (!layer || !layer->conv_weight || !layer->a_log_bias || !layer->norm_weight || !start || !conv_state || !state)
+    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "NULL pointer");
+  if (batch <= 0 || total < 0 || total > INT32_MAX || layer->num_heads <= 0 ||
+      (int64_t)layer->num_heads * batch > INT32_MAX)
+    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "bad arguments");
+  if (layer->key_dim != 128 || layer->value_dim != 128 || layer->conv_kernel != 4)
+    return fail(ctx, SPOCK_ERR_UNSUPPORTED, std::string(op) + "key_dim = value_dim = 128 and conv width 4 only");
+  if (!conv_state_out != !state_out)
+    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "state_out and conv_state_out go together");
+  if (total && (!qkv || !a || !b || (out && !z)))
+    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "NULL pointer");
+  if (!out && !state_out && total) return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "neither out nor state_out");
+  if (misaligned(state, 16) || misaligned(state_out, 16) || misaligned(conv_state, 8) ||
+      misaligned(conv_state_out, 8) || misaligned(layer->conv_weight, 8))
+    return fail(ctx, SPOCK_ERR_INVALID,
+                std::string(op) + "state must be 16-byte aligned, conv_state and conv_weight 8-byte");
+  if (!total && !state_out) return SPOCK_OK;
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok) return fail(ctx, SPOCK_ERR_CUDA, std::string(op) + "cannot select device");
+  return finish(ctx, spock::launch_decode_span(*layer, batch, start, counts, total, qkv, qkv_ld, a, b, ab_ld, z, z_ld,
+                                               conv_state, state, conv_state_out, state_out, out, ctx->d_err_flag,
+                                               (cudaStream_t)stream));
+}
+
+__attribute__((visibility("default"))) int spock_draft_verify_workspace(spock_ctx* ctx, int64_t total, int64_t vocab,
+                                                                        int32_t batch, size_t* bytes) {
+  if (!ctx) return fail(nullptr, SPOCK_ERR_INVALID, "spock_draft_verify_workspace: ctx is NULL");
+  if (!bytes || total < 0 || vocab <= 0 || batch <= 0)
+    return fail(ctx, SPOCK_ERR_INVALID, "spock_draft_verify_workspace: bad arguments");
+  *bytes = spock::draft_verify_workspace(total, vocab, batch);
+  return SPOCK_OK;
+}
+
+__attribute__((visibility("default"))) int spock_draft_verify(
+    spock_ctx* ctx, int32_t dtype, const void* logits, int64_t logits_ld, int64_t total, int64_t vocab, int32_t batch,
+    const int32_t* start, const int32_t* tokens, const float* draft_probs, int64_t probs_ld, const float* temperature,
+    const float* u_accept, const float* u_sample, int32_t* emitted, int32_t* out_tokens, void* workspace,
+    size_t workspace_bytes, void* stream) {
+  const char* const op = "spock_draft_verify: ";
+  if (!ctx) return fail(nullptr, SPOCK_ERR_INVALID, std::string(op) + "ctx is NULL");
+  if (dtype < SPOCK_F32 || dtype > SPOCK_BF16) return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "unknown dtype");
+  if (batch <= 0 || total < 0 || total > INT32_MAX || vocab <= 0 || vocab > INT32_MAX || !start || !u_sample ||
+      !emitted || !workspace ||
+      (total && (!logits || !tokens || !u_accept || !out_tokens)) ||
+      (total > 1 && (logits_ld < vocab || (draft_probs && probs_ld < vocab))))
+    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "bad arguments");
+  if (misaligned(logits, dtype == SPOCK_F32 ? 4 : 2) || misaligned(workspace, 16))
+    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "misaligned pointer");
+  if (workspace_bytes < spock::draft_verify_workspace(total, vocab, batch))
+    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "workspace too small");
+  DeviceGuard dg(ctx->device);
+  if (!dg.ok) return fail(ctx, SPOCK_ERR_CUDA, std::string(op) + "cannot select device");
+  spock::VerifyArgs v{logits, logits_ld, total, vocab, batch, start, tokens, draft_probs, probs_ld, temperature,
+                      u_accept, u_sample, emitted, out_tokens, workspace, ctx->d_err_flag};
+  return finish(ctx, spock::launch_draft_verify(dtype, v, (cudaStream_t)stream));
 }
 
 }  // extern "C"

@@ -102,6 +102,18 @@ cudaError_t launch_k_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, dim3
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
+// Error-word codes below this are bounded waits that gave up; this one is an
+// index in device data (page table, lengths, starts, tokens) out of range.
+constexpr int kErrBadIndex = 64;
+// What spock_sync / spock_model_sync report for a set error word.
+inline Status err_word_status(const char* what, int flag) {
+  if (flag == kErrBadIndex)
+    return Status::err(SPOCK_ERR_INVALID,
+                       std::string(what) + ": a start, length, page-table entry or token id was out of range");
+  return Status::err(SPOCK_ERR_TIMEOUT,
+                     std::string(what) + ": a kernel's bounded wait gave up (code " + std::to_string(flag) + ")");
+}
+
 // ---- device helpers -------------------------------------------------------
 
 // IEEE arithmetic with contraction disabled, so per-element updates round

@@ -649,8 +649,8 @@ __attribute__((visibility("default"))) int spock_model_sync(spock_model* m, void
   if (e != cudaSuccess) return mfail(m, SPOCK_ERR_CUDA, std::string("spock_model_sync: ") + cudaGetErrorString(e));
   if (!flag) return SPOCK_OK;
   cudaMemset(m->err_flag, 0, sizeof(int));
-  return mfail(m, SPOCK_ERR_TIMEOUT,
-               "spock_model_sync: a kernel's bounded wait gave up (code " + std::to_string(flag) + ")");
+  const spock::Status s = spock::err_word_status("spock_model_sync", flag);
+  return mfail(m, s.code, s.msg);
 }
 
 __attribute__((visibility("default"))) const char* spock_model_last_error(const spock_model* m) {
