@@ -539,8 +539,10 @@ def test_bad_device_data_is_reported_not_used(cuda_ok):
     q = torch.randn(4, 8, 256, device=DEV, generator=g).half()
     proj = torch.randn(4, 5120, device=DEV, generator=g).half()
     starts = _i32([0, 2, 4])
-    good, ref = (c.table.clone(), c.len.clone()), _ref_attention(q, [0, 2, 4], c, 0.0625, None)
+    good = c.table.clone(), c.len.clone()
     for bad in (-1, c.k.shape[0], 2 ** 31 - 1):
+        c.table.copy_(good[0])
+        ref = _ref_attention(q, [0, 2, 4], c, 0.0625, None)  # the prep below writes new rows each time
         c.table[0, 18] = bad
         out = spock_b200.paged_attention(q, starts, *c.args(), 0.0625)
         refused()
