@@ -138,68 +138,6 @@ __global__ void __launch_bounds__(256)
   store_words(c.v + at, w);
 }
 
-// One warp per (token, query head): positions one by one, online softmax,
-// lane l holding dims l*V .. l*V+V-1.
-template <typename T, int D>
-__global__ void __launch_bounds__(256)
-    paged_attn_kernel(Cache c, int batch, const int32_t* __restrict__ start, int total, int q_heads,
-                      const T* __restrict__ q, int64_t q_row, int64_t q_head, const T* __restrict__ gate,
-                      int64_t g_row, int64_t g_head, float scale, T* __restrict__ out, int* __restrict__ err) {
-  constexpr int V = D / 32;
-  const int lane = threadIdx.x & 31;
-  check_ragged(c, batch, start, total, err);
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= (int64_t)total * q_heads) return;
-  const int row = (int)(item / q_heads), h = (int)(item % q_heads);
-  const int b = seq_of_row(start, batch, row, lane);
-  if (b < 0) return;
-  int len = c.kv_len[b] - (start[b + 1] - start[b]) + (row - start[b]) + 1;
-  if (len > c.table_width * c.page_size) len = 0;  // reported by check_ragged
-  float x[V], acc[V] = {}, m = -INFINITY, l = 0.f;
-  auto load = [&](const void* p, float(&f)[V]) {
-    uint32_t w[V / 2];
-    load_words(p, w);
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      const float2 t = Io<T>::up2(w[i]);
-      f[2 * i] = t.x;
-      f[2 * i + 1] = t.y;
-    }
-  };
-  load(q + row * q_row + h * q_head + lane * V, x);
-  const int kvh = h / (q_heads / c.kv_heads);
-  for (int p = 0; p < len; ++p) {
-    const int page = c.table[b * c.table_stride + p / c.page_size];
-    if (page < 0 || page >= c.num_pages) {
-      if (lane == 0) report_bad_index(err);
-      break;
-    }
-    const int64_t at = page * c.page_stride + (p % c.page_size) * c.pos_stride + kvh * c.head_stride + lane * V * 2;
-    float kf[V], vf[V], dot = 0.f;
-    load(c.k + at, kf);
-    load(c.v + at, vf);
-#pragma unroll
-    for (int i = 0; i < V; ++i) dot = fmaf(x[i], kf[i], dot);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    dot *= scale;
-    const float mn = fmaxf(m, dot), corr = expf(m - mn), pw = expf(dot - mn);
-    m = mn;
-    l = l * corr + pw;
-#pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = fmaf(pw, vf[i], acc[i] * corr);
-  }
-  const float inv = l > 0.f ? 1.0f / l : 0.f;
-  float gf[V];
-  if (gate) load(gate + row * g_row + h * g_head + lane * V, gf);
-#pragma unroll
-  for (int i = 0; i < V; ++i) acc[i] *= gate ? inv / (1.0f + expf(-gf[i])) : inv;
-  uint32_t w[V / 2];
-#pragma unroll
-  for (int i = 0; i < V / 2; ++i) w[i] = Io<T>::down2(acc[2 * i], acc[2 * i + 1]);
-  store_words(out + ((int64_t)row * q_heads + h) * D + lane * V, w);
-}
-
 template <typename F>
 Status by_type(int dtype, int head_dim, F f) {
   if (dtype == SPOCK_F16) {
@@ -226,23 +164,6 @@ Status launch_paged_prep(const spock_paged_kv& kv, int batch, const int32_t* sta
                  (const T*)q_norm, (const T*)k_norm, eps, rope, rope_len, rotary / 2, (T*)q_out, err);
     if (e != cudaSuccess) return cuda_status(e, "paged_prep_kernel");
     SPOCK_LAUNCH_CHECK("paged_prep_kernel");
-    return Status::ok();
-  });
-}
-
-size_t paged_attention_workspace(int, int, int, int) { return 16; }
-
-Status launch_paged_attention(const spock_paged_kv& kv, int batch, const int32_t* start, int64_t total, int q_heads,
-                              const void* q, int64_t q_row, int64_t q_head, const void* gate, int64_t g_row,
-                              int64_t g_head, float scale, void* out, void*, int, int* err, cudaStream_t st) {
-  return by_type(kv.dtype, kv.head_dim, [&](auto t, auto d) -> Status {
-    using T = decltype(t);
-    const cudaError_t e = launch_k(paged_attn_kernel<T, decltype(d)::value>,
-                                   dim3((unsigned)((total * q_heads + 7) / 8)), dim3(256), 0, st, cache_of(kv), batch,
-                                   start, (int)total, q_heads, (const T*)q, q_row, q_head, (const T*)gate, g_row,
-                                   g_head, scale, (T*)out, err);
-    if (e != cudaSuccess) return cuda_status(e, "paged_attn_kernel");
-    SPOCK_LAUNCH_CHECK("paged_attn_kernel");
     return Status::ok();
   });
 }

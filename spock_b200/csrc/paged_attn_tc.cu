@@ -1,0 +1,822 @@
+// Causal attention of several new tokens per sequence over a KV cache in pages
+// (spock_paged_attention) on the tcgen05 tensor cores.
+//
+//   o_r = sum_p w_rp v_p / sum_p w_rp,  w_rp = exp(scale (q_r . k_p) - m_r),
+//   p = 0 .. len - n + t(r);  out_r = o_r sigmoid(gate_r)
+//
+// paged_attn_kernel: one CTA per SM walks its share of the batch
+// (paged_sched.cuh): row tiles of up to 128 (token, query head) rows of one
+// sequence and kv head, times KV tiles of 128 positions. Warp roles:
+//   warp 0      K and V tiles by TMA from the pages into a ring of stages
+//   warp 1      issues the MMAs: S = Q K^T (M128 N128 K=D) into one of two TMEM
+//               buffers, O += P V (M128 N=D K128) with P read from TMEM
+//   warps 2-3   the next row tile's queries, into shared memory
+//   warps 4-11  softmax, two threads per row (64 of a tile's positions each), and
+//               the output of finished row tiles
+// S(i+1) is issued before O += P(i) V(i), so the tensor pipe has work while the
+// softmax of a tile runs; the ring and the walk run on across row tiles. P
+// overwrites its S in TMEM, in the operand type. The running maximum a row's
+// weights refer to moves only when a tile's exceeds it by 2^8 (weights stay
+// below 256, exact sums in fp32), so O is rarely rescaled.
+// A row tile that is one CTA's alone is finished there; a cut one leaves its
+// unnormalised O (fp32), maximum and sum in the workspace, and
+// paged_join_kernel adds the parts in order (no atomics: results repeat).
+//
+// Slots behind kv_len may hold anything: their scores are masked, and their V
+// rows are zeroed in shared memory, since 0 * NaN would reach every row.
+// Every wait is bounded; one that gives up sets the context's error word, and
+// the CTA lets its copies and MMAs land, frees its TMEM and leaves.
+#include <cuda.h>
+
+#include <atomic>
+#include <mutex>
+
+#include "paged_sched.cuh"
+#include "ragged.cuh"
+#include "ragged.h"
+#include "tc.cuh"
+
+namespace spock {
+namespace {
+
+using sched::kTile;
+constexpr uint32_t kWait = 1u << 22;
+constexpr int kThreads = 384;
+constexpr float kLazy = 8.0f;  // log2 of how far weights may exceed 1
+
+template <int D>
+struct Shape {
+  static constexpr int DB = D < 128 ? D : 128;  // dims per stage
+  static constexpr int KS = D / DB;             // stages per K (or V) tile
+  static constexpr int kStage = kTile * DB * 2;
+  static constexpr int kQ = 128 * D * 2;
+  static constexpr int NST = D == 256 ? 5 : D == 128 ? 6 : 8;
+  static constexpr int kBar = kQ + NST * kStage;
+  static constexpr int kRed = kBar + 512;
+  static constexpr int kSmem = kRed + 4 * 128 * 4;
+};
+static_assert(Shape<256>::kSmem <= 227 * 1024 && Shape<128>::kSmem <= 227 * 1024, "shared memory of one SM");
+
+struct AttnArgs {
+  const int32_t *start, *table, *kv_len;
+  int64_t table_stride;
+  int batch, total, table_width, num_pages, page_size, kv_heads, G, tp, piece;
+  int64_t head_blk;  // 64-element blocks from one kv head to the next
+  const uint8_t *q, *gate;
+  int64_t q_row, q_head, g_row, g_head;  // bytes
+  uint8_t* out;
+  float scale_log2;
+  float* ws;
+  int* err;
+};
+
+// Workspace: per CTA a Meta and two parts (its first and its last row tile).
+// A part: O [128][D] fp32, then the reference maxima (log2 units) and sums [128].
+struct Meta {
+  int slot;      // part of the row tile that begins in this CTA and ends in a later one, or -1
+  int row0;      // its first packed row
+  int rows;      // valid rows (token, head of the group)
+  int head;      // kv head
+  int have, nt;  // KV tiles done here, in all
+  int units;     // of this CTA
+  int pad;
+};
+template <int D>
+__host__ __device__ constexpr size_t part_floats() {
+  return (size_t)128 * D + 256;
+}
+__host__ __device__ constexpr size_t meta_bytes(int ctas) { return ((size_t)ctas * sizeof(Meta) + 127) / 128 * 128; }
+
+struct Seq {
+  int lo, n, len;
+};
+__device__ __forceinline__ Seq load_seq(const AttnArgs& A, int b, bool report) {
+  Seq s;
+  s.lo = A.start[b];
+  const int hi = A.start[b + 1];
+  s.n = hi - s.lo;
+  s.len = A.kv_len[b];
+  if (s.lo < 0 || hi < s.lo || hi > A.total) {
+    if (report) report_bad_index(A.err);
+    s.n = 0;
+  }
+  if (s.len < 0 || s.len > A.table_width * A.page_size) {
+    if (report) report_bad_index(A.err);
+    s.len = 0;
+  }
+  return s;
+}
+
+// A role's way through the CTA's units.
+struct Walk {
+  int b, h, rt;
+  int k0, k1, nt;  // KV tiles of the current row tile: [k0, k1) here, nt in all
+  int64_t left;    // units from this row tile's first one on
+  Seq s;
+  __device__ __forceinline__ void fit(const AttnArgs& A) {
+    nt = sched::row_tile_units(s.n, s.len, A.tp, rt);
+    k1 = nt - k0 <= left ? nt : k0 + (int)left;
+  }
+  __device__ __forceinline__ bool next(const AttnArgs& A) {
+    left -= k1 - k0;
+    if (left <= 0) return false;
+    k0 = 0;
+    if (++rt * A.tp >= s.n) {
+      rt = 0;
+      if (++h == A.kv_heads) {
+        h = 0;
+        do s = load_seq(A, ++b, false);
+        while (s.n <= 0 && b + 1 < A.batch);
+      }
+    }
+    fit(A);
+    return true;
+  }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                      const __grid_constant__ AttnArgs A) {
+  using Sh = Shape<D>;
+  constexpr int DB = Sh::DB, KS = Sh::KS, NST = Sh::NST;
+  constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+  extern __shared__ __align__(1024) uint8_t sm[];  // no static shared memory beside it, so it starts on 1024 bytes
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + Sh::kBar);
+  uint64_t* empty = full + NST;
+  uint64_t* q_full = empty + NST;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_full + 2;   // [2]
+  uint64_t* p_full = q_full + 4;   // [2]
+  uint64_t* o_done = q_full + 6;
+  uint64_t* drain = q_full + 7;
+  volatile int* s_fail = reinterpret_cast<volatile int*>(q_full + 8);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(q_full + 8) + 1;
+  int64_t* s_scan = reinterpret_cast<int64_t*>(sm + Sh::kBar + 256);  // [warps]
+  int* s_first = reinterpret_cast<int*>(s_scan + kThreads / 32);      // [4]
+  volatile int* s_issued = s_first + 4;
+  float* red = reinterpret_cast<float*>(sm + Sh::kRed);  // [2 tiles][2 halves][128] maxima (and sums)
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = blockIdx.x, ctas = gridDim.x;
+  Meta* meta = reinterpret_cast<Meta*>(A.ws);
+  float* parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(A.ws) + meta_bytes(ctas));
+
+  if (tc::smem_u32(sm) & 1023) {  // never on this toolchain; the operand layouts need it
+    if (tid == 0) atomicExch(A.err, 6);
+    return;
+  }
+  if (tid == 0) {
+    for (int i = 0; i < NST; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    tc::mbar_init(q_full, 2);
+    tc::mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&s_full[i], 1);
+      tc::mbar_init(&p_full[i], 8);
+    }
+    tc::mbar_init(o_done, 1);
+    tc::mbar_init(drain, 1);
+    *s_fail = 0;
+    *s_issued = 0;
+    tc::fence_mbar_init();
+    tc::prefetch_tmap(&tmk);
+    tc::prefetch_tmap(&tmv);
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(s_tmem, 512);
+    tc::tmem_relinquish();
+  }
+  pdl_wait();
+  pdl_launch();
+
+  // this CTA's first unit: prefix sums of the sequences' units over the block
+  const int per = (A.batch + kThreads - 1) / kThreads;
+  int64_t mine = 0;
+  for (int b = tid * per; b < min(A.batch, (tid + 1) * per); ++b) {
+    const Seq s = load_seq(A, b, cta == 0);
+    mine += sched::head_units(s.n, s.len, A.tp) * A.kv_heads;
+  }
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) s_scan[warp] = incl;
+  __syncthreads();
+  int64_t base = 0, units = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) base += s_scan[w];
+    units += s_scan[w];
+  }
+  const int shares = units < ctas ? (int)units : ctas;  // none of them empty
+  const int64_t u0 = cta < shares ? sched::share_begin(units, cta, shares) : 0;
+  const int64_t u1 = cta < shares ? sched::share_begin(units, cta + 1, shares) : 0;
+  const int64_t from = base + incl - mine;
+  if (u1 > u0 && from <= u0 && u0 < from + mine) {
+    int64_t r = u0 - from;
+    for (int b = tid * per;; ++b) {
+      const Seq s = load_seq(A, b, false);
+      const int64_t hu = sched::head_units(s.n, s.len, A.tp);
+      if (r < hu * A.kv_heads) {
+        s_first[0] = b;
+        s_first[1] = (int)(r / hu);
+        r %= hu;
+        s_first[2] = sched::find_row_tile(s.n, s.len, A.tp, r);
+        s_first[3] = (int)r;
+        break;
+      }
+      r -= hu * A.kv_heads;
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const int N = (int)(u1 - u0);  // KV tiles of this CTA
+  const uint32_t tb = *s_tmem, tO = tb + 256;
+  const uint32_t sbase = tc::smem_u32(sm);
+  Walk w;
+  w.left = N;
+  if (N > 0) {
+    w.b = s_first[0];
+    w.h = s_first[1];
+    w.rt = s_first[2];
+    w.k0 = s_first[3];
+    w.s = load_seq(A, w.b, false);
+    w.fit(A);
+  }
+
+  // bounded wait; gives up at once when another role has
+  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+    for (uint32_t i = 0; i < kWait; ++i) {
+      if (tc::mbar_try_wait(bar, parity)) return true;
+      if (*s_fail) return false;
+    }
+    *s_fail = 1;
+    return false;
+  };
+
+  if (N == 0) {
+    if (tid == 0) meta[cta].slot = -1, meta[cta].units = 0;
+  } else if (warp == 0) {
+    // ---- K and V tiles: order K0, K1, V0, K2, V1, ... ----
+    struct Src {
+      int page, group, h, bytes;
+    };
+    const int pieces = kTile / A.piece;
+    // this lane's piece of KV tile k
+    auto locate = [&](const Walk& at, int k) -> Src {
+      Src r;
+      const int p0 = k * kTile, pos = p0 + lane * A.piece;
+      const bool live = lane < pieces && pos < at.s.len;
+      r.page = -1;
+      r.h = at.h;
+      r.group = 0;
+      if (live) {
+        const int slot = pos / A.page_size;
+        r.page = A.table[at.b * A.table_stride + slot];
+        r.group = (pos - slot * A.page_size) >> 3;
+      }
+      r.bytes = __popc(__ballot_sync(0xffffffffu, live)) * A.piece * DB * 2;
+      if (live && (r.page < 0 || r.page >= A.num_pages)) {
+        report_bad_index(A.err);
+        r.page = 0;
+      } else if (!live) {
+        r.page = -1;
+      }
+      return r;
+    };
+    int ld = 0;
+    auto load = [&](const CUtensorMap* map, const Src& src) -> bool {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int st = ld % NST, round = ld / NST;
+        bool ok = true;
+        if (lane == 0) {
+          ok = round == 0 || wait(&empty[st], (round - 1) & 1);
+          if (ok) {
+            tc::mbar_arrive_expect_tx(&full[st], src.bytes);
+            *s_issued = ld + 1;
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) return false;
+        if (src.page >= 0)
+          tc::tma_load_5d(sm + Sh::kQ + st * Sh::kStage + lane * A.piece * DB * 2, map, &full[st], 0, 0,
+                          (int)(src.h * A.head_blk) + s * (DB / 64), src.group, src.page);
+        ++ld;
+      }
+      return true;
+    };
+    int k = w.k0;
+    Src cur = locate(w, k), nxt = cur;
+    bool ok = load(&tmk, cur);
+    for (int g = 0; g < N && ok; ++g) {
+      if (g + 1 < N) {
+        if (++k == w.k1) {
+          w.next(A);
+          k = w.k0;
+        }
+        nxt = locate(w, k);
+        ok = load(&tmk, nxt);
+      }
+      if (ok) ok = load(&tmv, cur);
+      cur = nxt;
+    }
+  } else if (warp == 1) {
+    // ---- MMAs ----
+    if (lane == 0) {
+      constexpr uint32_t ID_S = tc::idesc_f16(128, kTile, false, false, kBf16);
+      constexpr uint32_t ID_O = tc::idesc_f16(128, DB, false, true, kBf16);
+      constexpr uint32_t kGroup = (DB / 64) * 1024;  // bytes from one 8-position group of a stage to the next
+      int use = 0, item = 0, k = w.k0;
+      bool ok = true;
+      auto issue_s = [&](int g) -> bool {
+        if (k == w.k0 && !wait(q_full, item & 1)) return false;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const int st = use % NST;
+          if (!wait(&full[st], (use / NST) & 1)) return false;
+          tc::tc_fence_after();
+          const uint32_t kb = sbase + Sh::kQ + st * Sh::kStage;
+#pragma unroll
+          for (int ks = 0; ks < DB / 16; ++ks)
+            tc::mma_f16(tb + (g & 1) * kTile,
+                        tc::sdesc(sbase + (s * (DB / 64) + (ks >> 2)) * 16384 + (ks & 3) * 32, 16, 1024),
+                        tc::sdesc(kb + (ks >> 2) * 1024 + (ks & 3) * 32, 16, kGroup), ID_S, (s | ks) > 0);
+          tc::mma_commit(&empty[st]);
+          ++use;
+        }
+        tc::mma_commit(&s_full[g & 1]);
+        if (k + 1 == w.k1) tc::mma_commit(q_empty);
+        return true;
+      };
+      ok = issue_s(0);
+      bool first = true;  // tile g is its row tile's first here: O starts from zero
+      for (int g = 0; g < N && ok; ++g) {
+        bool next_first = false;
+        if (g + 1 < N) {
+          if (++k == w.k1) {
+            w.next(A);
+            k = w.k0;
+            ++item;
+            next_first = true;
+          }
+          ok = issue_s(g + 1);
+          if (!ok) break;
+        }
+        if (!(ok = wait(&p_full[g & 1], (g >> 1) & 1))) break;
+        tc::tc_fence_after();
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const int st = use % NST;
+          if (!(ok = wait(&full[st], (use / NST) & 1))) break;
+          tc::tc_fence_after();
+          const uint32_t vb = sbase + Sh::kQ + st * Sh::kStage;
+#pragma unroll
+          for (int ks = 0; ks < kTile / 16; ++ks)
+            tc::mma_f16_ta(tO + s * DB, tb + (g & 1) * kTile + ks * 8,
+                           tc::sdesc(vb + ks * 2 * kGroup, 1024, kGroup), ID_O, !first || ks > 0);
+          tc::mma_commit(&empty[st]);
+          ++use;
+        }
+        tc::mma_commit(o_done);
+        first = next_first;
+      }
+    }
+    __syncwarp();
+  } else if (warp < 4) {
+    // ---- queries ----
+    for (int item = 0;; ++item) {
+      bool ok = true;
+      if (item > 0) {
+        if (lane == 0) ok = wait(q_empty, (item - 1) & 1);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+      }
+      if (!ok) break;
+      const int t0 = w.rt * A.tp, rows = min(A.tp, w.s.n - t0) * A.G;
+      constexpr int CH = D / 8;               // 16-byte chunks of a row
+      constexpr int RW = CH >= 32 ? 1 : 32 / CH;  // rows per warp instruction
+      const int sub = CH >= 32 ? 0 : lane / CH, c = CH >= 32 ? lane : lane % CH;
+      const int step = 2 * RW;
+      int r = (warp - 2) * RW + sub, tt = r / A.G, gh = r - tt * A.G;
+      for (; r < rows; r += step) {
+        const uint8_t* src = A.q + (int64_t)(w.s.lo + t0 + tt) * A.q_row + (int64_t)(w.h * A.G + gh) * A.q_head + c * 16;
+        cp_async16(sbase + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4), src);
+        gh += step;
+        while (gh >= A.G) gh -= A.G, ++tt;
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      tc::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(q_full);
+      if (!w.next(A)) break;
+    }
+  } else {
+    // ---- softmax and outputs ----
+    const int quad = warp & 3, half = (warp - 4) >> 2, row = quad * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const float c = A.scale_log2;
+    // A wait that gives up does not leave the loop: the warps of a pair meet at
+    // named barriers, so all of them walk on (each later wait returns at once)
+    // and the outputs are unspecified.
+    auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
+      wait(bar, parity);
+      __syncwarp();
+      tc::tc_fence_after();
+    };
+    auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory"); };
+    if (tid == 128) meta[cta].slot = -1, meta[cta].units = N;
+    float m = -INFINITY, l = 0.f;
+    int k = w.k0, item = 0;
+    int t0 = 0, rows = 0, lim = 0, lim0 = 0, tt = 0;
+    auto enter = [&] {
+      t0 = w.rt * A.tp;
+      rows = min(A.tp, w.s.n - t0) * A.G;
+      tt = row / A.G;
+      lim = row < rows ? w.s.len - w.s.n + t0 + tt : 0x7fffffff;
+      lim0 = __shfl_sync(0xffffffffu, lim, 0);
+      m = -INFINITY;
+      l = 0.f;
+    };
+    enter();
+    for (int g = 0; g < N; ++g) {
+      const int buf = g & 1, p0 = k * kTile;
+      const bool live = quad * 32 < rows;
+      wait_warp(&s_full[buf], (g >> 1) & 1);
+      if (p0 + kTile > w.s.len) {  // slots behind the sequence: their V rows become zero
+        const int pos = g + 1 < N ? 2 * g + 2 : 2 * N - 1, first = max(0, w.s.len - p0);
+        // V(g - 1) has been read, so every earlier load of V(g)'s stages is over:
+        // their barriers are at most one phase behind and the parities are V(g)'s
+        if (g > 0) wait_warp(o_done, (g - 1) & 1);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const int use = pos * KS + s, st = use % NST;
+          wait_warp(&full[st], (use / NST) & 1);
+          uint8_t* vb = sm + Sh::kQ + st * Sh::kStage;
+          for (int i = tid - 128; i < (kTile - first) * (DB / 8); i += 256) {
+            const int r = first + i / (DB / 8), ch = i % (DB / 8);
+            *reinterpret_cast<uint4*>(vb + (r >> 3) * (DB / 64) * 1024 + (ch >> 3) * 1024 + (r & 7) * 128 +
+                                      (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        tc::fence_async_smem();
+      }
+      if (live) {
+        float s[64];
+        tc::tmem_ld64(tb + buf * kTile + lane_off + half * 64, s);
+        if (p0 + kTile - 1 > lim0) {
+          const int d = lim - p0 - half * 64;  // the last column this row sees
+#pragma unroll
+          for (int j = 0; j < 64; ++j) s[j] = j <= d ? s[j] : -INFINITY;
+        }
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int j = 4; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        red[buf * 256 + half * 128 + row] = top;
+        pair_sync();  // also: both halves have read S before P overwrites it
+        top = fmaxf(top, red[buf * 256 + (half ^ 1) * 128 + row]);
+        const bool move = (top - m) * c > kLazy;
+        if (__any_sync(0xffffffffu, move)) {
+          const float corr = move ? ex2((m - top) * c) : 1.0f;
+          if (move) m = top;
+          l *= corr;
+          if (k > w.k0) {
+            wait_warp(o_done, (g - 1) & 1);
+#pragma unroll 1
+            for (int cb = 0; cb < D / 64; ++cb) {
+              float o[32];
+              const uint32_t at = tO + lane_off + half * (D / 2) + cb * 32;
+              tc::tmem_ld32(at, o);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] *= corr;
+              tc::tmem_st32(at, o);
+            }
+          }
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c;
+        uint32_t p[32];
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const float a = ex2(fmaf(s[2 * j], c, -mc)), b = ex2(fmaf(s[2 * j + 1], c, -mc));
+          sum[(2 * j) & 3] += a;
+          sum[(2 * j + 1) & 3] += b;
+          p[j] = Io<T>::down2(a, b);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tc::tmem_st32u(tb + buf * kTile + lane_off + half * 32, p);
+        tc::tmem_st_wait();
+      }
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&p_full[buf]);
+      if (++k < w.k1) continue;
+
+      // ---- the row tile's last KV tile here ----
+      // one phase at a time: P(g) may be ready while O += P(g-1) V(g-1) still runs,
+      // and the parity of phase g alone would then be that of phase g - 2
+      if (g > 0) wait_warp(o_done, (g - 1) & 1);
+      wait_warp(o_done, g & 1);
+      const bool whole = w.k0 == 0 && w.k1 == w.nt;
+      const int slot = item == 0 ? 0 : 1;
+      if (!whole && w.k0 == 0 && tid == 128) {
+        Meta& mt = meta[cta];
+        mt.slot = slot;
+        mt.row0 = w.s.lo + t0;
+        mt.rows = rows;
+        mt.head = w.h;
+        mt.have = w.k1;
+        mt.nt = w.nt;
+      }
+      if (live) {
+        float* rl = red + (buf ^ 1) * 256;  // idle: the maxima of the tile before, read by both halves
+        rl[half * 128 + row] = l;
+        pair_sync();
+        const float lt = l + rl[(half ^ 1) * 128 + row];
+        pair_sync();  // read before the next tile's maxima go there
+        if (whole) {
+          const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+          const int64_t tok = w.s.lo + t0 + tt;
+          const int hq = w.h * A.G + row - tt * A.G;
+          uint8_t* op = A.out + (tok * (A.kv_heads * A.G) + hq) * (D * 2) + half * D;
+          const uint8_t* gp = A.gate ? A.gate + tok * A.g_row + hq * A.g_head + half * D : nullptr;
+#pragma unroll 1
+          for (int cb = 0; cb < D / 64; ++cb) {
+            float o[32];
+            tc::tmem_ld32(tO + lane_off + half * (D / 2) + cb * 32, o);
+            if (row < rows) {
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                uint32_t x[4], gw[4];
+                if (gp) load_words(gp + cb * 64 + v * 16, gw);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  float a = o[v * 8 + 2 * e] * inv, b = o[v * 8 + 2 * e + 1] * inv;
+                  if (gp) {
+                    const float2 z = Io<T>::up2(gw[e]);
+                    a = __fdividef(a, 1.0f + __expf(-z.x));
+                    b = __fdividef(b, 1.0f + __expf(-z.y));
+                  }
+                  x[e] = Io<T>::down2(a, b);
+                }
+                store_words(op + cb * 64 + v * 16, x);
+              }
+            }
+          }
+        } else {
+          float* part = parts + ((size_t)cta * 2 + slot) * part_floats<D>();
+          if (half == 0 && row < rows) {
+            part[128 * D + row] = m == -INFINITY ? -INFINITY : m * c;
+            part[128 * D + 128 + row] = lt;
+          }
+#pragma unroll 1
+          for (int cb = 0; cb < D / 64; ++cb) {
+            float o[32];
+            tc::tmem_ld32(tO + lane_off + half * (D / 2) + cb * 32, o);
+            if (row < rows) {
+              float4* dst = reinterpret_cast<float4*>(part + row * D + half * (D / 2) + cb * 32);
+#pragma unroll
+              for (int v = 0; v < 8; ++v) dst[v] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+            }
+          }
+        }
+      }
+      if (w.next(A)) {
+        k = w.k0;
+        ++item;
+        enter();
+      }
+    }
+  }
+  __syncwarp();
+  tc::tc_fence_before();
+  __syncthreads();
+  if (*s_fail) {
+    // let the copies and MMAs in flight land before shared memory and TMEM go
+    if (tid == 0) {
+      atomicExch(A.err, 5);
+      for (int st = 0; st < NST; ++st)
+        if (*s_issued > st) {
+          const int last = (*s_issued - 1 - st) / NST;
+          tc::mbar_wait_bounded(&full[st], last & 1, kWait);
+        }
+    }
+    if (tid == 32) {
+      tc::mma_commit(drain);
+      tc::mbar_wait_bounded(drain, 0, kWait);
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tb, 512);
+  }
+}
+
+// Joins the parts of the row tile that begins in share blockIdx.x and ends in a
+// later one, in share order: o = sum 2^{m_i - m} O_i / sum 2^{m_i - m} l_i.
+// Rows are dealt to the blockIdx.y blocks. Few parts: a warp per row; many (a
+// long sequence over the whole GPU): the block's 8 warps share each row's.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ AttnArgs A) {
+  constexpr int V = D / 32, kMany = 12;
+  const int cta = blockIdx.x, ctas = gridDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ float s_o[8][D];
+  __shared__ float s_l[8];
+  pdl_wait();
+  pdl_launch();
+  const Meta* meta = reinterpret_cast<const Meta*>(A.ws);
+  const Meta mt = meta[cta];
+  if (mt.slot < 0) return;
+  const float* parts = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(A.ws) + meta_bytes(ctas));
+  int n = 1;  // parts
+  for (int have = mt.have; have < mt.nt && cta + n < ctas; ++n) have += meta[cta + n].units;
+  auto part = [&](int i) {
+    return parts + ((size_t)(cta + i) * 2 + (i == 0 ? mt.slot : 0)) * part_floats<D>();
+  };
+  auto finish = [&](int r, float (&acc)[V], float l) {
+    const int tt = r / A.G, hq = mt.head * A.G + r - tt * A.G;
+    const int64_t tok = mt.row0 + tt;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint32_t w[V / 2], gw[V / 2];
+    if (A.gate) load_words(A.gate + tok * A.g_row + hq * A.g_head + lane * V * 2, gw);
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) {
+      float a = acc[2 * e] * inv, b = acc[2 * e + 1] * inv;
+      if (A.gate) {
+        const float2 z = Io<T>::up2(gw[e]);
+        a = __fdividef(a, 1.0f + __expf(-z.x));
+        b = __fdividef(b, 1.0f + __expf(-z.y));
+      }
+      w[e] = Io<T>::down2(a, b);
+    }
+    store_words(A.out + (tok * (A.kv_heads * A.G) + hq) * (D * 2) + lane * V * 2, w);
+  };
+  auto add = [&](int i, int r, float m, float (&acc)[V], float& l) {
+    const float* p = part(i);
+    const float mi = p[128 * D + r];
+    const float f = mi == -INFINITY ? 0.f : ex2(mi - m);
+    if (f == 0.f) return;  // a part that saw nothing (or nothing that counts) may hold anything
+    l += f * p[128 * D + 128 + r];
+#pragma unroll
+    for (int v = 0; v < V; v += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(p + r * D + lane * V + v);
+      acc[v] = fmaf(f, x.x, acc[v]);
+      acc[v + 1] = fmaf(f, x.y, acc[v + 1]);
+    }
+  };
+  const bool many = n > kMany;
+  for (int r = many ? blockIdx.y : blockIdx.y * 8 + warp; r < mt.rows; r += many ? gridDim.y : gridDim.y * 8) {
+    float m = -INFINITY;
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, part(i)[128 * D + r]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float acc[V] = {}, l = 0.f;
+    if (!many) {
+      for (int i = 0; i < n; ++i) add(i, r, m, acc, l);
+      finish(r, acc, l);
+      continue;
+    }
+    for (int i = warp; i < n; i += 8) add(i, r, m, acc, l);
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < V; ++v) s_o[warp][lane * V + v] = acc[v];
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    if (warp == 0) {
+      l = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = 0.f;
+      for (int k = 0; k < 8; ++k) {
+        l += s_l[k];
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] += s_o[k][lane * V + v];
+      }
+      finish(r, acc, l);
+    }
+  }
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                             const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult qr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess &&
+        qr == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(p);
+  });
+  return fn;
+}
+
+// Pages as [page][8-position group][64-dim block][position in group][64]: one
+// box of a piece's groups lands as [group][block][8][128 B], which both the
+// K-major and the MN-major operand layouts read with constant strides whatever
+// the page size. The blocks of head h start at h * head_stride / 64.
+CUresult encode_pages(EncodeFn fn, CUtensorMap* map, const spock_paged_kv& kv, void* base, int piece, int db) {
+  const int64_t blocks = (kv.kv_heads - 1) * (kv.head_stride / 64) + kv.head_dim / 64;
+  cuuint64_t dims[5] = {64, 8, (cuuint64_t)blocks, (cuuint64_t)kv.page_size / 8, (cuuint64_t)kv.num_pages};
+  cuuint64_t strides[4] = {(cuuint64_t)kv.pos_stride * 2, 128, (cuuint64_t)kv.pos_stride * 16,
+                           (cuuint64_t)kv.page_stride * 2};
+  cuuint32_t box[5] = {64, 8, (cuuint32_t)db / 64, (cuuint32_t)piece / 8, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return fn(map, kv.dtype == SPOCK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, base,
+            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+template <typename T, int D>
+Status launch(const spock_paged_kv& kv, AttnArgs& A, int sms, cudaStream_t st) {
+  EncodeFn fn = encode();
+  if (!fn) return Status::err(SPOCK_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  CUtensorMap mk, mv;
+  if (encode_pages(fn, &mk, kv, kv.k, A.piece, Shape<D>::DB) != CUDA_SUCCESS ||
+      encode_pages(fn, &mv, kv, kv.v, A.piece, Shape<D>::DB) != CUDA_SUCCESS)
+    return Status::err(SPOCK_ERR_CUDA, "spock_paged_attention: tensor map encoding failed");
+  // the attribute belongs to the kernel on the current device: set once on each
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e, "spock_paged_attention");
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(done.load() & bit)) {
+    e = cudaFuncSetAttribute(paged_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+    if (e != cudaSuccess) return cuda_status(e, "paged_attn_kernel attribute");
+    done.fetch_or(bit);
+  }
+  e = launch_k(paged_attn_kernel<T, D>, dim3(sms), dim3(kThreads), Shape<D>::kSmem, st, mk, mv, A);
+  if (e != cudaSuccess) return cuda_status(e, "paged_attn_kernel");
+  SPOCK_LAUNCH_CHECK("paged_attn_kernel");
+  pdl_scope overlap;  // the join's launch runs under the main kernel
+  e = launch_k(paged_join_kernel<T, D>, dim3(sms, 4), dim3(256), 0, st, A);
+  if (e != cudaSuccess) return cuda_status(e, "paged_join_kernel");
+  SPOCK_LAUNCH_CHECK("paged_join_kernel");
+  return Status::ok();
+}
+
+int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+}  // namespace
+
+size_t paged_attention_workspace(int, int, int head_dim, int sms) {
+  const size_t part = head_dim == 64 ? part_floats<64>() : head_dim == 128 ? part_floats<128>() : part_floats<256>();
+  return meta_bytes(sms) + (size_t)sms * 2 * part * sizeof(float);
+}
+
+Status launch_paged_attention(const spock_paged_kv& kv, int batch, const int32_t* start, int64_t total, int q_heads,
+                              const void* q, int64_t q_row, int64_t q_head, const void* gate, int64_t g_row,
+                              int64_t g_head, float scale, void* out, void* ws, int sms, int* err, cudaStream_t st) {
+  AttnArgs A{};
+  A.start = start;
+  A.table = kv.page_table;
+  A.kv_len = kv.kv_len;
+  A.table_stride = kv.table_stride;
+  A.batch = batch;
+  A.total = (int)total;
+  A.table_width = kv.table_width;
+  A.num_pages = kv.num_pages;
+  A.page_size = kv.page_size;
+  A.kv_heads = kv.kv_heads;
+  A.G = q_heads / kv.kv_heads;
+  A.tp = 128 / A.G;
+  A.piece = gcd(kv.page_size, kTile);
+  A.head_blk = kv.head_stride / 64;
+  A.q = (const uint8_t*)q;
+  A.gate = (const uint8_t*)gate;
+  A.q_row = q_row * 2;
+  A.q_head = q_head * 2;
+  A.g_row = g_row * 2;
+  A.g_head = g_head * 2;
+  A.out = (uint8_t*)out;
+  A.scale_log2 = scale * 1.44269504088896341f;
+  A.ws = (float*)ws;
+  A.err = err;
+  if (kv.dtype == SPOCK_F16) {
+    if (kv.head_dim == 64) return launch<__half, 64>(kv, A, sms, st);
+    if (kv.head_dim == 128) return launch<__half, 128>(kv, A, sms, st);
+    return launch<__half, 256>(kv, A, sms, st);
+  }
+  if (kv.head_dim == 64) return launch<__nv_bfloat16, 64>(kv, A, sms, st);
+  if (kv.head_dim == 128) return launch<__nv_bfloat16, 128>(kv, A, sms, st);
+  return launch<__nv_bfloat16, 256>(kv, A, sms, st);
+}
+
+}  // namespace spock
