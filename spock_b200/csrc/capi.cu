@@ -436,6 +436,7 @@ __attribute__((visibility("default"))) int spock_draft_verify(
     return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "bad arguments");
   if (misaligned(logits, dtype == SPOCK_F32 ? 4 : 2) || misaligned(workspace, 16))
     return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "misaligned pointer");
+  if (batch > (1 << 27)) return fail(ctx, SPOCK_ERR_UNSUPPORTED, std::string(op) + "at most 2^27 sequences");
   if (workspace_bytes < spock::draft_verify_workspace(total, vocab, batch))
     return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "workspace too small");
   DeviceGuard dg(ctx->device);
