@@ -47,38 +47,49 @@ struct Part {  // of one row, by one CTA
 template <typename T>
 constexpr int kChunk = 16 / (int)sizeof(T);  // elements of a 16-byte load
 
-// Chunk k of a row starts at element k * kChunk - a, a = how far the row's
-// first element is behind a 16-byte boundary, so inner chunks are one aligned
-// load; elements outside [0, vocab) read as -inf, NaN logits too (fix = true).
+// A row in 16-byte chunks: chunk k is elements k C - a .. + C - 1, a = how far
+// the row's first element is behind a 16-byte boundary, so the inner chunks
+// [f0, f1) are one aligned load each; of the others (the first and the last, at
+// most) the elements that do not exist read as -inf.
 template <typename T>
-__device__ __forceinline__ int row_shift(const T* row) {
-  return (int)(((uintptr_t)row & 15) / sizeof(T));
-}
-template <typename T, bool kFix>
-__device__ __forceinline__ void load_chunk(const T* row, int64_t j0, int64_t vocab, float (&x)[kChunk<T>]) {
-  constexpr int C = kChunk<T>;
-  if (j0 >= 0 && j0 + C <= vocab) {
-    const uint4 u = *reinterpret_cast<const uint4*>(row + j0);
+struct Row {
+  static constexpr int C = kChunk<T>;
+  const T* x;
+  const uint4* base;  // chunk 0 (only inner ones are read as such)
+  int a, f0, f1, chunks, vocab;
+  __device__ __forceinline__ Row(const T* row, int n) : x(row), vocab(n) {
+    a = (int)(((uintptr_t)row & 15) / sizeof(T));
+    base = reinterpret_cast<const uint4*>(row - a);
+    chunks = (int)(((int64_t)n + a + C - 1) / C);
+    f0 = a ? 1 : 0;
+    f1 = (int)(((int64_t)n + a) / C);
+  }
+  __device__ __forceinline__ int first(int k) const { return k * C - a; }  // chunk k's first element
+  __device__ __forceinline__ bool inner(int k) const { return k >= f0 && k < f1; }
+  __device__ __forceinline__ void open(const uint4& u, float (&v)[C]) const {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (sizeof(T) == 4) {
-        x[i] = __uint_as_float(w[i]);
+        v[i] = __uint_as_float(w[i]);
       } else {
         const float2 f = Io<T>::up2(w[i]);
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
       }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < C; ++i) x[i] = j0 + i >= 0 && j0 + i < vocab ? load_as_f32(row, j0 + i) : -INFINITY;
   }
-  if constexpr (kFix) {
+  // any chunk
+  __device__ __forceinline__ void load(int k, float (&v)[C]) const {
+    if (inner(k)) {
+      open(__ldg(base + k), v);
+    } else {
+      const int64_t j0 = (int64_t)k * C - a;
 #pragma unroll
-    for (int i = 0; i < C; ++i) x[i] = fmaxf(x[i], -INFINITY);
+      for (int i = 0; i < C; ++i) v[i] = j0 + i >= 0 && j0 + i < vocab ? load_as_f32(x, j0 + i) : -INFINITY;
+    }
   }
-}
+};
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -91,9 +102,9 @@ __device__ __forceinline__ float rebase(float z, float m, float to, float c) {
 }
 
 int stat_splits(int64_t total, int64_t vocab) {
-  // enough CTAs for several waves of 8 an SM, at least 8192 logits each; and no
+  // a wave of 8 CTAs an SM (more cost more than they hide), at least 8192 logits each; and no
   // thread sums more than kThreadTerms terms
-  const int64_t want = total > 0 ? (148 * 32 + total - 1) / total : 1, most = (vocab + 8191) / 8192;
+  const int64_t want = total > 0 ? (148 * 8 + total - 1) / total : 1, most = (vocab + 8191) / 8192;
   const int64_t least = (vocab + kThreadTerms * kT / 2 - 1) / (kThreadTerms * kT / 2);
   return (int)std::max(least, std::min(want, most));
 }
@@ -111,57 +122,83 @@ __global__ void __launch_bounds__(kT) verify_stats_kernel(const VerifyArgs A, in
   const float temp = A.temperature ? A.temperature[b] : 1.0f;
   const bool greedy = !(temp > 0.f);
   const float c = 1.44269504088896341f / temp;
-  const T* x = static_cast<const T*>(A.logits) + row * A.logits_ld;
-  const int a = row_shift(x);
-  const int64_t chunks = (A.vocab + a + C - 1) / C;
-  const int64_t k0 = chunks * part / splits, k1 = chunks * (part + 1) / splits;
+  const Row<T> x(static_cast<const T*>(A.logits) + row * A.logits_ld, (int)A.vocab);
+  const int k0 = (int)((int64_t)x.chunks * part / splits), k1 = (int)((int64_t)x.chunks * (part + 1) / splits);
   float top = -INFINITY, z = 0.f;
-  int64_t at = -1;  // chunk of the thread's first maximum
-  for (int64_t k = k0 + t; k < k1; k += U * kT) {
-    float v[U][C];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (k + u * kT < k1) {
-        load_chunk<T, false>(x, (k + u * kT) * C - a, A.vocab, v[u]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < C; ++i) v[u][i] = -INFINITY;
-      }
+  int at = -1;  // chunk of the thread's first maximum
+  // a thread's chunks are kT apart, U of them in flight at a time
+  auto take = [&](const float(&v)[U][C], int n, int k) {
     float m = top;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float cm = v[u][0];
+      if (u >= n) break;
+      float cm = fmaxf(v[u][0], v[u][1]);
 #pragma unroll
-      for (int i = 1; i < C; ++i) cm = fmaxf(cm, v[u][i]);
+      for (int i = 2; i < C; ++i) cm = fmaxf(cm, v[u][i]);
       if (greedy && cm > m) at = k + u * kT;
       m = fmaxf(m, cm);
     }
     if (!greedy) {
       if (m > top) z = rebase(z, top, m, c);
+      float s[2] = {0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        if (u >= n) break;
 #pragma unroll
-        for (int i = 0; i < C; ++i) z += ex2((v[u][i] - m) * c);
+        for (int i = 0; i < C; ++i) s[i & 1] += ex2((v[u][i] - m) * c);
+      }
+      z += s[0] + s[1];
     }
     top = m;
+  };
+  int k = max(k0, x.f0) + t;
+  const int kf = min(k1, x.f1);
+  float v[U][C];
+  for (; k + (U - 1) * kT < kf; k += U * kT) {
+    uint4 raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = __ldg(x.base + k + u * kT);
+#pragma unroll
+    for (int u = 0; u < U; ++u) x.open(raw[u], v[u]);
+    take(v, U, k);
+  }
+  for (; k < kf; k += kT) {
+    x.open(__ldg(x.base + k), v[0]);
+    take(v, 1, k);
+  }
+  // the row's ragged first and last chunks: threads 0 and 1, where this CTA has them
+  int edge = t == 0 ? 0 : t == 1 && x.chunks > 1 ? x.chunks - 1 : -1;
+  if (edge < k0 || edge >= k1 || x.inner(edge)) edge = -1;
+  if (edge >= 0) {
+    x.load(edge, v[0]);
+    const float was = top;
+    const int before = at;
+    take(v, 1, edge);
+    // among equals the lowest chunk counts, and the first one comes last here
+    if (greedy && edge < before && top == was) {
+      bool tie = false;
+#pragma unroll
+      for (int i = 0; i < C; ++i) tie |= v[0][i] == top;
+      if (tie) at = edge;
+    }
   }
   if (!greedy && !(z < INFINITY)) {  // NaN or +inf among the logits (or none above -inf): once more, with care
     z = 0.f;
-    for (int64_t k = k0 + t; k < k1; k += kT) {
-      float v[C];
-      load_chunk<T, true>(x, k * C - a, A.vocab, v);
+    auto add = [&](int q) {
+      x.load(q, v[0]);
 #pragma unroll
       for (int i = 0; i < C; ++i)
-        if (v[i] > -INFINITY) z += v[i] == top ? 1.0f : ex2((v[i] - top) * c);
-    }
+        if (v[0][i] > -INFINITY) z += v[0][i] == top ? 1.0f : ex2((v[0][i] - top) * c);
+    };
+    for (int q = max(k0, x.f0) + t; q < kf; q += kT) add(q);
+    if (edge >= 0) add(edge);
   }
   int best = 0x7fffffff;
   if (greedy && at >= 0) {
-    float v[C];
-    load_chunk<T, true>(x, at * C - a, A.vocab, v);
+    x.load(at, v[0]);
 #pragma unroll
     for (int i = C - 1; i >= 0; --i)
-      if (v[i] == top) best = (int)(at * C - a + i);
+      if (v[0][i] == top) best = x.first(at) + i;
   }
   // the warp's, then the block's
   const float mine = top;
@@ -192,25 +229,19 @@ __global__ void __launch_bounds__(kT) verify_stats_kernel(const VerifyArgs A, in
   }
 }
 
-// fp32 -> fp64 with integer operations (the conversion instruction runs at a
-// fraction of the fp64 rate); zeros and subnormals become about +-2^-127.
-__device__ __forceinline__ double widen(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return __hiloint2double((int)((u & 0x80000000u) | (((u >> 3) & 0x0fffffffu) + (896u << 20))), (int)(u << 29));
-}
 // 2^(t / 256) for t <= 0: t = n + f with |f| <= 1/2, 2^(n/256) from a table,
-// e^r with r = f ln 2 / 256 (|r| < 2^-9.5) as 1 + r + r^2/2 + r^3/6: the next
-// term, r^4 / 24, is below 1.4e-13.
+// 2^(f/256) as a cubic of f: with r = f ln 2 / 256 (|r| < 2^-9.5) the next term,
+// r^4 / 24, is below 1.4e-13. Exactly 1 at 0; meaningless below -2^18. Entry i of
+// the table is 2^(i/256) with i * 4096 taken off its high word, so that adding
+// n * 4096 (n = 256 e + i) leaves e in the exponent.
 __device__ __forceinline__ double exp2_neg(double t, const double* tab) {
-  if (t < -256000.0) return 0.0;
-  const double big = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
-  const double k = t + big;
+  constexpr double h = 0.69314718055994530942 / 256.0, big = 6755399441055744.0;  // 1.5 * 2^52
+  const double k = t + big;  // rounds to a whole number
   const int n = __double2loint(k);
-  const double r = (t - (k - big)) * (0.69314718055994530942 / 256.0);
-  const double p = fma(fma(r, 1.0 / 6.0, 0.5), r * r, r);
-  const double s = tab[n & 255];
-  const double y = fma(s, p, s);
-  return __hiloint2double(__double2hiint(y) + ((n >> 8) << 20), __double2loint(y));
+  const double f = t - (k - big);
+  const double e = tab[n & 255];
+  const double s = __hiloint2double(__double2hiint(e) + n * 4096, __double2loint(e));
+  return fma(s * f, fma(fma(f, h * h * h / 6.0, h * h / 2.0), f, h), s);
 }
 
 // Combines a row's parts, by one warp.
@@ -244,17 +275,57 @@ __device__ __forceinline__ double warp_sum(double x) {
   return x;
 }
 
+struct Top {
+  double d;    // the largest logit
+  float least; // logits up to this one have no weight
+  bool inf;    // the largest is +inf: each +inf weighs 1
+};
+
+__device__ __forceinline__ double warp_scan(double x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+// 64 sums (two per lane: i = lane, lane + 32) and their running sums: the first
+// positive one whose running sum exceeds `at`, or the last positive one, and the
+// running sum before it; -1 if none is positive.
+__device__ __forceinline__ int first_over(const double (&x)[2], const double (&upto)[2], double at, int lane,
+                                          double& before) {
+  int i = -1;
+#pragma unroll
+  for (int h = 1; h >= 0; --h) {
+    const unsigned over = __ballot_sync(0xffffffffu, x[h] > 0.0 && upto[h] > at);
+    if (over) i = h * 32 + __ffs(over) - 1;
+  }
+  if (i < 0) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const unsigned some = __ballot_sync(0xffffffffu, x[h] > 0.0);
+      if (some) i = h * 32 + 31 - __clz(some);
+    }
+  }
+  const double b = i < 32 ? upto[0] - x[0] : upto[1] - x[1];
+  before = __shfl_sync(0xffffffffu, b, i & 31);
+  return i;
+}
+
 enum { kAccept = 0, kReject = 1, kUnsure = 2 };
 
 template <typename T>
-__global__ void __launch_bounds__(kT) verify_pick_kernel(const VerifyArgs A, int splits) {
+__global__ void __launch_bounds__(kT, 4) verify_pick_kernel(const VerifyArgs A, int splits) {
   constexpr int C = kChunk<T>;
-  __shared__ double s_tab[256], s_step[kW][kSteps], s_warp[kW], s_all[kCluster * kW];
+  __shared__ double s_tab[256], s_step[kW][kSteps], s_warp[kW];
   __shared__ int s_say[kW];
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int b = blockIdx.x / ranks, t = threadIdx.x, warp = t >> 5, lane = t & 31;
-  s_tab[t] = exp2(t / 256.0);
+  {
+    const double e = exp2(t / 256.0);
+    s_tab[t] = __hiloint2double(__double2hiint(e) - t * 4096, __double2loint(e));
+  }
   pdl_wait();
   pdl_launch();
   const RowSpan rows = row_span(A.start, b, (int)A.total, A.err);
@@ -267,35 +338,38 @@ __global__ void __launch_bounds__(kT) verify_pick_kernel(const VerifyArgs A, int
   const float temp = A.temperature ? A.temperature[b] : 1.0f;
   const bool greedy = !(temp > 0.f);
   const float c = 1.44269504088896341f / temp;
-  const double c256 = 256.0 * 1.44269504088896340736 / (double)temp;
+  const double c256 = fmin(256.0 * 1.44269504088896340736 / (double)temp, 1e300);
   __syncthreads();
 
-  // e of one logit: 1 at the top (also where it is +inf), 0 for -inf
-  auto weight = [&](float x, float top) -> double {
-    if (x == -INFINITY) return 0.0;
-    if (x == top) return 1.0;
-    return exp2_neg((widen(x) - widen(top)) * c256, s_tab);
+  // e of one logit, exactly 1 at the top; 0 for -inf, for NaN and where e would
+  // be below 2^-1000
+  auto weight = [&](float x, const Top& top) -> double {
+    const double e = exp2_neg(((double)x - top.d) * c256, s_tab);
+    return x > top.least ? e : 0.0;
+  };
+  auto top_of = [&](float top) -> Top {
+    // +inf: the logits that are +inf count 1, the others 0
+    if (top == INFINITY) return {0.0, 3.4028235e38f, true};
+    if (top == -INFINITY) return {0.0, INFINITY, false};  // no weights
+    const double least = (double)top - 256000.0 / c256;
+    return {(double)top, fminf((float)least, nextafterf(top, -INFINITY)), false};
   };
   const int nw = ranks * kW, me = rank * kW + warp;
-  // Sums f over this warp's chunks of row x, step by step; the cluster's sum is
-  // in s_all afterwards. f(chunk's first element, logits) -> the chunk's sum.
-  int64_t k0 = 0, k1 = 0, per_step = 0;
-  auto sum_row = [&](const T* x, auto f) -> double {
-    const int a = row_shift(x);
-    const int64_t chunks = (A.vocab + a + C - 1) / C;
-    k0 = chunks * me / nw;
-    k1 = chunks * (me + 1) / nw;
-    const int64_t most = (chunks + nw - 1) / nw;  // a warp's most
+  // Sums f(chunk, logits) over this warp's chunks of a row, step by step; the
+  // cluster's sums are in mine2 and upto (running) afterwards.
+  int k0 = 0, k1 = 0, per_step = 0;
+  double mine2[2], upto[2];
+  auto sum_row = [&](const Row<T>& x, auto f) -> double {
+    k0 = (int)((int64_t)x.chunks * me / nw);
+    k1 = (int)((int64_t)x.chunks * (me + 1) / nw);
+    const int most = (x.chunks + nw - 1) / nw;  // a warp's most
     per_step = (most + 32 * kSteps - 1) / (32 * kSteps) * 32;
     double all = 0.0;
     int step = 0;
-    for (int64_t k = k0; k < k1; k += per_step, ++step) {
+    for (int k = k0; k < k1; k += per_step, ++step) {
+      const int end = min(k1, k + per_step);
       double s = 0.0;
-      for (int64_t q = k + lane; q < min(k1, k + per_step); q += 32) {
-        float v[C];
-        load_chunk<T, true>(x, q * C - a, A.vocab, v);
-        s += f(q * C - a, v);
-      }
+      for (int q = k + lane; q < end; q += 32) s += f(q);
       s = warp_sum(s);
       if (lane == 0) s_step[warp][step] = s;
       all += s;
@@ -303,18 +377,28 @@ __global__ void __launch_bounds__(kT) verify_pick_kernel(const VerifyArgs A, int
     cluster.sync();  // the last sums have been read
     if (lane == 0) s_warp[warp] = all;
     cluster.sync();
-    for (int i = t; i < nw; i += kT) s_all[i] = cluster.map_shared_rank(s_warp, i / kW)[i % kW];
-    __syncthreads();
-    double total = 0.0;
-    for (int i = 0; i < nw; ++i) total += s_all[i];
-    return total;
+    // every warp: the sums of warps lane and lane + 32, their running sums
+    mine2[0] = lane < nw ? cluster.map_shared_rank(s_warp, lane / kW)[lane % kW] : 0.0;
+    mine2[1] = lane + 32 < nw ? cluster.map_shared_rank(s_warp, (lane + 32) / kW)[lane % kW] : 0.0;
+    upto[0] = warp_scan(mine2[0], lane);
+    const double half = __shfl_sync(0xffffffffu, upto[0], 31);
+    upto[1] = half + warp_scan(mine2[1], lane);
+    return __shfl_sync(0xffffffffu, upto[1], 31);
   };
-  auto sum_e = [&](int r, float top) -> double {
-    return sum_row(logits + r * A.logits_ld, [&](int64_t, const float(&v)[C]) {
-      double s = 0.0;
+  auto row_of = [&](int r) { return Row<T>(logits + r * A.logits_ld, (int)A.vocab); };
+  auto sum_e = [&](const Row<T>& x, const Top& top) -> double {
+    return sum_row(x, [&](int k) {
+      float v[C];
+      x.load(k, v);
+      double s[2] = {0.0, 0.0};
+      if (top.inf) {
 #pragma unroll
-      for (int i = 0; i < C; ++i) s += weight(v[i], top);
-      return s;
+        for (int i = 0; i < C; ++i) s[0] += v[i] > top.least ? 1.0 : 0.0;
+      } else {
+#pragma unroll
+        for (int i = 0; i < C; ++i) s[i & 1] += weight(v[i], top);
+      }
+      return s[0] + s[1];
     });
   };
   auto draft_of = [&](int i) -> int {
@@ -329,7 +413,9 @@ __global__ void __launch_bounds__(kT) verify_pick_kernel(const VerifyArgs A, int
       return kReject;
     }
     if (greedy) return (p.best == 0x7fffffff ? 0 : p.best) == d ? kAccept : kReject;
-    const double e = weight(fmaxf(load_as_f32(logits + r * A.logits_ld, d), -INFINITY), p.top);
+    const Top top = top_of(p.top);
+    const float x = load_as_f32(logits + r * A.logits_ld, d);
+    const double e = top.inf ? (double)(x > top.least) : weight(x, top);
     const double q = A.probs ? (double)A.probs[r * A.probs_ld + d] : 1.0;
     const double uqz = (double)A.u_accept[r] * q * z;
     if (uqz * (1.0 + sure) < e && uqz * (1.0 - sure) < e) return kAccept;
@@ -357,7 +443,7 @@ __global__ void __launch_bounds__(kT) verify_pick_kernel(const VerifyArgs A, int
     if (s_say[w] == kReject) break;
     // too near to tell in 32 bits: Z again in 64, by the whole cluster
     p = join_parts(parts + (int64_t)(rows.lo + i) * splits, splits, c, lane);
-    const double z = sum_e(rows.lo + i, p.top);
+    const double z = sum_e(row_of(rows.lo + i), top_of(p.top));
     if (say(i, p, z, 0.0) != kAccept) break;
     ++i;
   }
@@ -371,107 +457,107 @@ __global__ void __launch_bounds__(kT) verify_pick_kernel(const VerifyArgs A, int
   if (greedy) {
     pick = p.best == 0x7fffffff ? 0 : p.best;
   } else {
-    const T* x = logits + r * A.logits_ld;
-    const float* q = drafted && A.probs ? A.probs + r * A.probs_ld : nullptr;
-    const double inv_z = q ? 1.0 / sum_e(r, p.top) : 0.0;
-    bool rest = drafted;
-    auto weights = [&](int64_t j0, const float(&v)[C], double(&w)[C]) {
+    const Row<T> x = row_of(r);
+    const float* q = drafted && A.probs ? A.probs + r * A.probs_ld - x.a : nullptr;  // chunk k's start at q + k C
+    const Top top = top_of(p.top);
+    const double inv_z = q ? 1.0 / sum_e(x, top) : 0.0;
+    const bool q16 = ((uintptr_t)q & 15) == 0;  // whether they are aligned too
+    // a chunk's weights: e; e without the draft's; max(e / Z - q, 0)
+    auto plain = [&](int k, double(&w)[C]) {
+      float v[C];
+      x.load(k, v);
+      if (top.inf) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) w[i] = v[i] > top.least ? 1.0 : 0.0;
+      } else {
+#pragma unroll
+        for (int i = 0; i < C; ++i) w[i] = weight(v[i], top);
+      }
+    };
+    auto without = [&](int k, double(&w)[C]) {
+      plain(k, w);
+      const int64_t at = (int64_t)drop + x.a - (int64_t)k * C;
+      if (at >= 0 && at < C) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) w[i] = i == at ? 0.0 : w[i];
+      }
+    };
+    auto beyond = [&](int k, double(&w)[C]) {
       float qv[C];
-      if (rest && q) {
-        if (j0 >= 0 && j0 + C <= A.vocab && ((uintptr_t)(q + j0) & 15) == 0) {
+      if (q16 && x.inner(k)) {
 #pragma unroll
-          for (int k = 0; k < C; k += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(q + j0 + k);
-            qv[k] = f.x, qv[k + 1] = f.y, qv[k + 2] = f.z, qv[k + 3] = f.w;
-          }
-        } else {
+        for (int i = 0; i < C; i += 4) {
+          const float4 f = __ldg(reinterpret_cast<const float4*>(q + (int64_t)k * C + i));
+          qv[i] = f.x, qv[i + 1] = f.y, qv[i + 2] = f.z, qv[i + 3] = f.w;
+        }
+      } else {
 #pragma unroll
-          for (int k = 0; k < C; ++k) qv[k] = j0 + k >= 0 && j0 + k < A.vocab ? q[j0 + k] : 0.f;
+        for (int i = 0; i < C; ++i) {
+          const int64_t j = (int64_t)k * C - x.a + i;
+          qv[i] = j >= 0 && j < A.vocab ? __ldg(q + (int64_t)k * C + i) : 0.f;
         }
       }
+      plain(k, w);
 #pragma unroll
-      for (int k = 0; k < C; ++k) {
-        const double e = weight(v[k], p.top);
-        w[k] = !rest ? e : q ? fmax(fma(e, inv_z, -(double)qv[k]), 0.0) : j0 + k == drop ? 0.0 : e;
+      for (int i = 0; i < C; ++i) {
+        const double y = fma(w[i], inv_z, -(double)qv[i]);
+        w[i] = y > 0.0 ? y : 0.0;
       }
     };
-    auto sum_w = [&]() {
-      return sum_row(x, [&](int64_t j0, const float(&v)[C]) {
-        double w[C], s = 0.0;
-        weights(j0, v, w);
+    auto sum_of = [&](auto weights) {
+      return sum_row(x, [&](int k) {
+        double w[C], s[2] = {0.0, 0.0};
+        weights(k, w);
 #pragma unroll
-        for (int k = 0; k < C; ++k) s += w[k];
-        return s;
+        for (int i = 0; i < C; ++i) s[i & 1] += w[i];
+        return s[0] + s[1];
       });
     };
-    double W = sum_w();
+    bool rest = drafted;
+    double W = rest ? (q ? sum_of(beyond) : sum_of(without)) : sum_of(plain);
     if (rest && !(W > 0.0)) {
       rest = false;
-      W = sum_w();
+      W = sum_of(plain);
     }
     // the warp whose sums cross u W, or the last that has any weight
     const double at = (double)A.u_sample[b] * W;
-    double before = 0.0, b4 = 0.0;
-    int owner = -1, last = -1;
-    for (int k = 0; k < nw; ++k) {
-      if (s_all[k] > 0.0) {
-        if (before + s_all[k] > at) {
-          owner = k;
-          break;
-        }
-        last = k;
-        b4 = before;
-      }
-      before += s_all[k];
-    }
-    if (owner < 0) owner = last, before = b4;
+    double before = 0.0;
+    int owner = first_over(mine2, upto, at, lane, before);
     mine = owner < 0 ? mine : me == owner;
     if (owner < 0) pick = 0;  // no weight anywhere
     if (owner >= 0 && mine) {
-      const int steps = (int)((k1 - k0 + per_step - 1) / per_step);
-      int step = -1, back = -1;
-      double sb = before, bb = before;
-      for (int k = 0; k < steps; ++k) {
-        if (s_step[warp][k] > 0.0) {
-          if (sb + s_step[warp][k] > at) {
-            step = k;
-            break;
-          }
-          back = k;
-          bb = sb;
-        }
-        sb += s_step[warp][k];
-      }
-      if (step < 0) step = back, sb = bb;
+      const int steps = (k1 - k0 + per_step - 1) / per_step;
+      const double sums[2] = {lane < steps ? s_step[warp][lane] : 0.0, lane + 32 < steps ? s_step[warp][lane + 32] : 0.0};
+      double run2[2], sb = 0.0;
+      run2[0] = before + warp_scan(sums[0], lane);
+      run2[1] = __shfl_sync(0xffffffffu, run2[0], 31) + warp_scan(sums[1], lane);
+      const int step = max(first_over(sums, run2, at, lane, sb), 0);
       // one step's chunks again, in order
-      const int a = row_shift(x);
-      const int64_t end = min(k1, k0 + (step + 1) * per_step);
+      const int end = min(k1, k0 + (step + 1) * per_step);
       int found = 0x7fffffff, seen = -1;
-      for (int64_t k = k0 + step * per_step; k < end && found == 0x7fffffff; k += 32) {
-        float v[C];
+      for (int k = k0 + step * per_step; k < end && found == 0x7fffffff; k += 32) {
         double w[C], s = 0.0;
 #pragma unroll
         for (int e = 0; e < C; ++e) w[e] = 0.0;
-        const int64_t j0 = (k + lane) * C - a;
+        const int j0 = x.first(k + lane);
         if (k + lane < end) {
-          load_chunk<T, true>(x, j0, A.vocab, v);
-          weights(j0, v, w);
+          if (!rest)
+            plain(k + lane, w);
+          else if (q)
+            beyond(k + lane, w);
+          else
+            without(k + lane, w);
         }
 #pragma unroll
         for (int e = 0; e < C; ++e) s += w[e];
-        double incl = s;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double y = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += y;
-        }
+        const double incl = warp_scan(s, lane);
         double run = sb + (incl - s);
         int here = 0x7fffffff, tail = -1;
 #pragma unroll
         for (int e = 0; e < C; ++e) {
           if (w[e] > 0.0) {
             run += w[e];
-            tail = (int)(j0 + e);
+            tail = j0 + e;
             if (run > at && here == 0x7fffffff) here = tail;
           }
         }
@@ -501,9 +587,10 @@ Status launch(const VerifyArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return cuda_status(e, "verify_stats_kernel");
     SPOCK_LAUNCH_CHECK("verify_stats_kernel");
   }
-  // a CTA per 8192 logits of a row, at most the portable cluster size
+  // a CTA per 8192 logits of a row, up to the portable cluster size, while all
+  // are resident at once (4 an SM)
   int ranks = 1;
-  while (ranks < kCluster && (int64_t)ranks * 8192 < a.vocab) ranks *= 2;
+  while (ranks < kCluster && (int64_t)ranks * 8192 < a.vocab && (int64_t)a.batch * ranks * 2 <= 148 * 4) ranks *= 2;
   pdl_scope overlap;  // its launch and table run under the first kernel
   e = launch_k_cluster(verify_pick_kernel<T>, dim3((unsigned)a.batch * ranks), dim3(kT), dim3(ranks), 0, st, a,
                        splits);
