@@ -391,7 +391,7 @@ __attribute__((visibility("default"))) int spock_deltanet_decode_span(
   if (!layer || !layer->conv_weight || !layer->a_log_bias || !layer->norm_weight || !start || !conv_state || !state)
     return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "NULL pointer");
   if (batch <= 0 || total < 0 || total > INT32_MAX || layer->num_heads <= 0 ||
-      (int64_t)layer->num_heads * batch > INT32_MAX)
+      (int64_t)layer->num_heads * batch > (INT32_MAX >> 8))
     return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "bad arguments");
   if (layer->key_dim != 128 || layer->value_dim != 128 || layer->conv_kernel != 4)
     return fail(ctx, SPOCK_ERR_UNSUPPORTED, std::string(op) + "key_dim = value_dim = 128 and conv width 4 only");
@@ -408,7 +408,7 @@ __attribute__((visibility("default"))) int spock_deltanet_decode_span(
   DeviceGuard dg(ctx->device);
   if (!dg.ok) return fail(ctx, SPOCK_ERR_CUDA, std::string(op) + "cannot select device");
   return finish(ctx, spock::launch_decode_span(*layer, batch, start, counts, total, qkv, qkv_ld, a, b, ab_ld, z, z_ld,
-                                               conv_state, state, conv_state_out, state_out, out, ctx->d_err_flag,
+                                               conv_state, state, conv_state_out, state_out, out, ctx->sms, ctx->d_err_flag,
                                                (cudaStream_t)stream));
 }
 

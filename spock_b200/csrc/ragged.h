@@ -17,7 +17,7 @@ Status launch_paged_attention(const spock_paged_kv& kv, int batch, const int32_t
 Status launch_decode_span(const spock_dn_layer& L, int batch, const int32_t* start, const int32_t* counts,
                           int64_t total, const void* qkv, int64_t qkv_ld, const void* a, const void* b, int64_t ab_ld,
                           const void* z, int64_t z_ld, const void* conv, const float* state, void* conv_out,
-                          float* state_out, void* out, int* err, cudaStream_t st);
+                          float* state_out, void* out, int sms, int* err, cudaStream_t st);
 
 struct VerifyArgs {
   const void* logits;
