@@ -45,7 +45,6 @@ namespace spock {
 namespace {
 
 using chunk::mma_tf32;
-using chunk::split_tf32;
 
 constexpr int kDim = 128, kThreads = 256, kChunk = 8;
 
@@ -93,6 +92,13 @@ __device__ __forceinline__ float warp_sum(float x) {
 }
 __device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
 
+// x as two tf32 parts, hi rounded towards zero and lo what remains, likewise:
+// 3 instructions where the rounding conversion takes several more (it was two
+// thirds of the products' instructions).
+__device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(x) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
+}
 // The three products of a split tile, each into sums of its own: a chain of
 // dependent MMAs costs their latency.
 struct Acc3 {
@@ -231,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 2) dn_span_kernel(const __grid_const
             m.v[j][t] = y;
           } else if (kOut || t >= kDim) {
             uint32_t hi, lo;
-            split_tf32(y, hi, lo);
+            split(y, hi, lo);
             dst[j * kRow * 4] = __uint_as_float(hi);
             dst[j * kRow * 4 + 2] = __uint_as_float(lo);
           }
@@ -316,10 +322,10 @@ __global__ void __launch_bounds__(kThreads, 2) dn_span_kernel(const __grid_const
         for (int x = 0; x < 16; ++x) {
           const float2 r0 = *state_at(x, 0), r1 = *state_at(x, 1);
           uint32_t ah[4], al[4];
-          split_tf32(r0.x, ah[0], al[0]);
-          split_tf32(r0.y, ah[1], al[1]);
-          split_tf32(r1.x, ah[2], al[2]);
-          split_tf32(r1.y, ah[3], al[3]);
+          split(r0.x, ah[0], al[0]);
+          split(r0.y, ah[1], al[1]);
+          split(r1.x, ah[2], al[2]);
+          split(r1.y, ah[3], al[3]);
           pk.add(ah, al, m.k[g][4 * x + c]);
           if (kOut) pq.add(ah, al, m.q[g][4 * x + c]);
         }
@@ -364,10 +370,10 @@ __global__ void __launch_bounds__(kThreads, 2) dn_span_kernel(const __grid_const
         uint32_t ah[4], al[4];
         const float2 d0 = *reinterpret_cast<const float2*>(&m.dd[c][col]);
         const float2 d1 = *reinterpret_cast<const float2*>(&m.dd[c + 4][col]);
-        split_tf32(d0.x, ah[0], al[0]);
-        split_tf32(d0.y, ah[1], al[1]);
-        split_tf32(d1.x, ah[2], al[2]);
-        split_tf32(d1.y, ah[3], al[3]);
+        split(d0.x, ah[0], al[0]);
+        split(d0.y, ah[1], al[1]);
+        split(d1.x, ah[2], al[2]);
+        split(d1.y, ah[3], al[3]);
         const float* k0 = reinterpret_cast<const float*>(&m.k[c][g >> 1]) + (g & 1);
         const float* k1 = reinterpret_cast<const float*>(&m.k[c + 4][g >> 1]) + (g & 1);
         float* p = A.state_out ? A.state_out + (size_t)item * kDim * kDim + (size_t)(2 * c) * kDim + col : nullptr;
