@@ -17,6 +17,7 @@ Reference interfaces mirrored here:
 """
 import ctypes
 import os
+import struct
 from dataclasses import dataclass, field
 from typing import List, Optional
 
@@ -340,8 +341,8 @@ def _bad(msg):
     raise SpockError(SPOCK_ERR_INVALID, msg)
 
 
-def _ragged(first, tensors):
-    """Checks (name, tensor, dtype, ndim, contiguous) entries against `first`'s device; the device's context."""
+def _refuse(first, tensors):
+    """Says which of the (name, tensor, dtype, ndim, contiguous) entries a call cannot take."""
     dev = first.device
     for name, t, dtype, ndim, contiguous in tensors:
         if t is None:
@@ -352,25 +353,36 @@ def _ragged(first, tensors):
             _bad(f"{name}: expected {dtype}, got {t.dtype}")
         if t.dim() != ndim:
             _bad(f"{name}: expected {ndim} dimensions, got {t.dim()}")
-        if contiguous:
-            if not t.is_contiguous():
-                _bad(f"{name}: expected a contiguous tensor")
-        elif ndim and t.shape[-1] > 1 and t.stride(-1) != 1:
+        if contiguous and not t.is_contiguous():
+            _bad(f"{name}: expected a contiguous tensor")
+        if not contiguous and t.shape[-1] > 1 and t.stride(-1) != 1:
             _bad(f"{name}: expected a contiguous last dimension")
-    if dev.type != "cuda":
-        _bad("expected CUDA tensors")
-    return Context.get(dev.index or 0)
+    _bad("expected CUDA tensors")
 
 
-def _stream_of(t, stream):
+# The checks that every call passes, as cheap as they can be made: at decode
+# sizes the host's time per call is what counts. `d` is the device index.
+def _rows(t, dtype, ndim, d):
+    """A tensor of contiguous rows (any strides before the last dimension)."""
+    return t.dtype is dtype and t.dim() == ndim and t.get_device() == d and (t.stride(-1) == 1 or t.shape[-1] <= 1)
+
+
+def _whole(t, dtype, ndim, d):
+    """A contiguous tensor."""
+    return t.dtype is dtype and t.dim() == ndim and t.get_device() == d and t.is_contiguous()
+
+
+def _stream_of(d, stream):
+    """The stream's handle; None: device d's current stream."""
+    if stream is not None:
+        return stream.cuda_stream
     import torch
-    return stream.cuda_stream if stream is not None else torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(d)
 
 
 def _new(shape, dtype, like, stream):
     """An uninitialised tensor for work on `stream` (None: the current one)."""
-    import torch
-    t = torch.empty(shape, dtype=dtype, device=like.device)
+    t = like.new_empty(shape, dtype=dtype)
     if stream is not None:  # allocated on the current stream: not to be reused before `stream` is done with it
         t.record_stream(stream)
     return t
@@ -381,24 +393,40 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else (t.shape[-1] + 7) // 8 * 8 if t.dim() == 2 else t.shape[1] * t.shape[2]
 
 
-def _paged_kv(k_pages, v_pages, page_table, kv_len, start):
+_PAGED = struct.Struct("@PPqqqPqPiiiiii")  # spock_paged_kv
+
+
+def _paged_kv(k_pages, v_pages, page_table, kv_len, batch):
     """spock_paged_kv over pages [num_pages, page_size, kv_heads, head_dim] (any strides, head_dim contiguous)."""
     import torch
-    batch = start.shape[0] - 1
-    if k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride():
+    st, dt = k_pages.stride(), k_pages.dtype
+    if k_pages.shape != v_pages.shape or st != v_pages.stride():
         _bad("k_pages and v_pages must have the same shape and strides")
+    width = page_table.shape[1]
     if batch < 1 or page_table.shape[0] != batch or kv_len.shape[0] != batch:
         _bad("start, page_table and kv_len disagree on the batch")
-    pages, page, heads, dim = k_pages.shape
-    if k_pages.dtype not in (torch.float16, torch.bfloat16):
+    if dt is not torch.float16 and dt is not torch.bfloat16:
         raise SpockError(SPOCK_ERR_UNSUPPORTED, "the cache is fp16 or bf16")
-    st = k_pages.stride()
+    pages, page, heads, dim = k_pages.shape
+    table_stride = page_table.stride(0)
     # strides of dimensions of one element say nothing
-    return PagedKv(k_pages.data_ptr(), v_pages.data_ptr(), st[0] if pages > 1 else page * heads * dim,
-                   st[1] if page > 1 else heads * dim, st[2] if heads > 1 else dim, page_table.data_ptr(),
-                   max(page_table.stride(0), page_table.shape[1]) if batch == 1 else page_table.stride(0),
-                   kv_len.data_ptr(), page_table.shape[1], pages, page, heads, dim,
-                   F16 if k_pages.dtype == torch.float16 else BF16)
+    return _PAGED.pack(k_pages.data_ptr(), v_pages.data_ptr(), st[0] if pages > 1 else page * heads * dim,
+                       st[1] if page > 1 else heads * dim, st[2] if heads > 1 else dim, page_table.data_ptr(),
+                       table_stride if batch > 1 or table_stride > width else width, kv_len.data_ptr(), width, pages,
+                       page, heads, dim, F16 if dt is torch.float16 else BF16), heads, dim
+
+
+def _workspace(ctx, query, key, like, stream):
+    """A workspace tensor from the caching allocator (so a captured graph keeps its own)."""
+    import torch
+    n = ctx.ws_bytes.get(key)
+    if n is None:
+        size = ctypes.c_size_t()
+        ctx.check(query(ctx.h, *key[1:], ctypes.byref(size)))
+        n = size.value
+        if len(ctx.ws_bytes) < 1024:  # sizes only, by shape
+            ctx.ws_bytes[key] = n
+    return _new((n,), torch.uint8, like, stream), n
 
 
 def paged_attention_prep(proj, start, k_pages, v_pages, page_table, kv_len, rope=None, q_norm=None, k_norm=None,
@@ -410,19 +438,24 @@ def paged_attention_prep(proj, start, k_pages, v_pages, page_table, kv_len, rope
     kv_len int32 [batch], the new tokens included; rope fp32 [positions, rotary / 2, 2] (cos, sin) or None;
     q_norm, k_norm [head_dim] ((1 + w) RMSNorm) or None. Returns q [total, q_heads, head_dim]."""
     import torch
-    i32, f32, dt = torch.int32, torch.float32, k_pages.dtype
-    ctx = _ragged(proj, (("proj", proj, dt, 2, False), ("start", start, i32, 1, True),
-                         ("k_pages", k_pages, dt, 4, False), ("v_pages", v_pages, dt, 4, False),
-                         ("page_table", page_table, i32, 2, False), ("kv_len", kv_len, i32, 1, True),
-                         ("rope", rope, f32, 3, True), ("q_norm", q_norm, dt, 1, True),
-                         ("k_norm", k_norm, dt, 1, True), ("q_out", q_out, dt, 3, True)))
-    kv = _paged_kv(k_pages, v_pages, page_table, kv_len, start)
-    dim, total, per = kv.head_dim, proj.shape[0], 2 if gated else 1
-    heads = proj.shape[1] // dim - 2 * kv.kv_heads
+    i32, f32, dt, d = torch.int32, torch.float32, k_pages.dtype, proj.get_device()
+    if not (d >= 0 and _rows(proj, dt, 2, d) and _whole(start, i32, 1, d) and _rows(k_pages, dt, 4, d) and
+            _rows(v_pages, dt, 4, d) and _rows(page_table, i32, 2, d) and _whole(kv_len, i32, 1, d) and
+            (rope is None or _whole(rope, f32, 3, d)) and (q_norm is None or _whole(q_norm, dt, 1, d)) and
+            (k_norm is None or _whole(k_norm, dt, 1, d)) and (q_out is None or _whole(q_out, dt, 3, d))):
+        _refuse(proj, (("proj", proj, dt, 2, False), ("start", start, i32, 1, True),
+                       ("k_pages", k_pages, dt, 4, False), ("v_pages", v_pages, dt, 4, False),
+                       ("page_table", page_table, i32, 2, False), ("kv_len", kv_len, i32, 1, True),
+                       ("rope", rope, f32, 3, True), ("q_norm", q_norm, dt, 1, True),
+                       ("k_norm", k_norm, dt, 1, True), ("q_out", q_out, dt, 3, True)))
+    ctx, batch = Context.get(d), start.shape[0] - 1
+    kv, kv_heads, dim = _paged_kv(k_pages, v_pages, page_table, kv_len, batch)
+    (total, width), per = proj.shape, 2 if gated else 1
+    heads = width // dim - 2 * kv_heads
     q_heads = heads // per
-    if proj.shape[1] % dim or heads <= 0 or heads % per:
+    if width % dim or heads <= 0 or heads % per:
         _bad("proj: the row is not q heads (with gates), k heads and v heads")
-    if any(w is not None and w.shape[0] != dim for w in (q_norm, k_norm)):
+    if (q_norm is not None and q_norm.shape[0] != dim) or (k_norm is not None and k_norm.shape[0] != dim):
         _bad("q_norm and k_norm have head_dim elements")
     if rope is not None and rope.shape[2] != 2:
         _bad("rope: expected [positions, rotary / 2, 2]")
@@ -431,11 +464,10 @@ def paged_attention_prep(proj, start, k_pages, v_pages, page_table, kv_len, rope
     elif q_out.shape != (total, q_heads, dim):
         _bad("q_out: expected [total, q_heads, head_dim]")
     ctx.check(lib().spock_paged_attention_prep(
-        ctx.h, ctypes.byref(kv), start.shape[0] - 1, start.data_ptr(), total, proj.data_ptr(), _row_stride(proj),
-        q_heads, int(bool(gated)), None if q_norm is None else q_norm.data_ptr(),
+        ctx.h, kv, batch, start.data_ptr(), total, proj.data_ptr(), _row_stride(proj), q_heads, int(bool(gated)), None if q_norm is None else q_norm.data_ptr(),
         None if k_norm is None else k_norm.data_ptr(), eps, None if rope is None else rope.data_ptr(),
         0 if rope is None else rope.shape[0], 0 if rope is None else 2 * rope.shape[1], q_out.data_ptr(),
-        _stream_of(proj, stream)))
+        _stream_of(d, stream)))
     return q_out
 
 
@@ -449,7 +481,7 @@ def _workspace(ctx, query, key, like, stream):
         n = size.value
         if len(ctx.ws_bytes) < 1024:  # sizes only, by shape
             ctx.ws_bytes[key] = n
-    return _new(n, torch.uint8, like, stream), n
+    return _new((n,), torch.uint8, like, stream), n
 
 
 def paged_attention(q, start, k_pages, v_pages, page_table, kv_len, scale, gate=None, out=None, workspace=None,
@@ -461,31 +493,37 @@ def paged_attention(q, start, k_pages, v_pages, page_table, kv_len, scale, gate=
     times sigmoid(gate); rows behind start[batch] are left as they are. `workspace`: a uint8 tensor of
     the caller's instead of one from the caching allocator."""
     import torch
-    i32, dt = torch.int32, k_pages.dtype
-    ctx = _ragged(q, (("q", q, dt, 3, False), ("start", start, i32, 1, True), ("k_pages", k_pages, dt, 4, False),
-                      ("v_pages", v_pages, dt, 4, False), ("page_table", page_table, i32, 2, False),
-                      ("kv_len", kv_len, i32, 1, True), ("gate", gate, dt, 3, False), ("out", out, dt, 3, True)))
-    kv = _paged_kv(k_pages, v_pages, page_table, kv_len, start)
-    total, q_heads, dim = q.shape
-    if dim != kv.head_dim:
+    i32, dt, d = torch.int32, k_pages.dtype, q.get_device()
+    if not (d >= 0 and _rows(q, dt, 3, d) and _whole(start, i32, 1, d) and _rows(k_pages, dt, 4, d) and
+            _rows(v_pages, dt, 4, d) and _rows(page_table, i32, 2, d) and _whole(kv_len, i32, 1, d) and
+            (gate is None or _rows(gate, dt, 3, d)) and (out is None or _whole(out, dt, 3, d)) and
+            (workspace is None or _whole(workspace, torch.uint8, 1, d))):
+        _refuse(q, (("q", q, dt, 3, False), ("start", start, i32, 1, True), ("k_pages", k_pages, dt, 4, False),
+                    ("v_pages", v_pages, dt, 4, False), ("page_table", page_table, i32, 2, False),
+                    ("kv_len", kv_len, i32, 1, True), ("gate", gate, dt, 3, False), ("out", out, dt, 3, True),
+                    ("workspace", workspace, torch.uint8, 1, True)))
+    ctx, batch, shape = Context.get(d), start.shape[0] - 1, q.shape
+    kv, kv_heads, dim = _paged_kv(k_pages, v_pages, page_table, kv_len, batch)
+    total, q_heads, q_dim = shape
+    if q_dim != dim:
         _bad("q: expected head_dim elements per head")
-    if gate is not None and gate.shape != q.shape:
+    if gate is not None and gate.shape != shape:
         _bad("gate: expected the shape of q")
     if out is None:
-        out = _new((total, q_heads, dim), dt, q, stream)
-    elif out.shape != q.shape:
+        out = _new(shape, dt, q, stream)
+    elif out.shape != shape:
         _bad("out: expected the shape of q")
     if workspace is None:
-        workspace, n = _workspace(ctx, lib().spock_paged_attention_workspace, ("attn", q_heads, kv.kv_heads, dim), q,
+        workspace, n = _workspace(ctx, lib().spock_paged_attention_workspace, ("attn", q_heads, kv_heads, dim), q,
                                   stream)
     else:
-        _ragged(q, (("workspace", workspace, torch.uint8, 1, True),))
         n = workspace.shape[0]
+    g = gate is not None
     ctx.check(lib().spock_paged_attention(
-        ctx.h, ctypes.byref(kv), start.shape[0] - 1, start.data_ptr(), total, q_heads, q.data_ptr(), _row_stride(q),
-        q.stride(1) if q_heads > 1 else dim, None if gate is None else gate.data_ptr(),
-        0 if gate is None else _row_stride(gate), 0 if gate is None else gate.stride(1) if q_heads > 1 else dim, scale,
-        out.data_ptr(), workspace.data_ptr(), n, _stream_of(q, stream)))
+        ctx.h, kv, batch, start.data_ptr(), total, q_heads, q.data_ptr(), _row_stride(q),
+        q.stride(1) if q_heads > 1 else dim, gate.data_ptr() if g else None, _row_stride(gate) if g else 0,
+        (gate.stride(1) if q_heads > 1 else dim) if g else 0, scale, out.data_ptr(), workspace.data_ptr(), n,
+        _stream_of(d, stream)))
     return out
 
 
@@ -498,14 +536,22 @@ def deltanet_decode_span(layer, qkv, conv_state, state, a, b, z, start, counts=N
     else is asked for) the gated outputs [total, heads * 128] are written and returned; with state_out and conv_out
     (which may be state and conv_state) the state after each sequence's first counts[b] rows (None: all)."""
     import torch
-    f16, f32, i32 = torch.float16, torch.float32, torch.int32
-    ctx = _ragged(qkv, (("qkv", qkv, f16, 2, False), ("a", a, f16, 2, False), ("b", b, f16, 2, False),
-                        ("z", z, f16, 2, False), ("conv_state", conv_state, f16, 3, True),
-                        ("state", state, f32, 4, True), ("start", start, i32, 1, True),
-                        ("counts", counts, i32, 1, True), ("state_out", state_out, f32, 4, True),
-                        ("conv_out", conv_out, f16, 3, True), ("out", out, f16, 2, True),
-                        ("conv_weight", layer.conv_weight, layer.conv_weight.dtype, layer.conv_weight.dim(), True),
-                        ("a_log_bias", layer.a_log_bias, f32, 2, True), ("norm_weight", layer.norm_weight, f32, 1, True)))
+    f16, f32, i32, d = torch.float16, torch.float32, torch.int32, qkv.get_device()
+    cw = layer.conv_weight
+    if not (d >= 0 and _rows(qkv, f16, 2, d) and _rows(a, f16, 2, d) and _rows(b, f16, 2, d) and
+            (z is None or _rows(z, f16, 2, d)) and _whole(conv_state, f16, 3, d) and _whole(state, f32, 4, d) and
+            _whole(start, i32, 1, d) and (counts is None or _whole(counts, i32, 1, d)) and
+            (state_out is None or _whole(state_out, f32, 4, d)) and (conv_out is None or _whole(conv_out, f16, 3, d)) and
+            (out is None or _whole(out, f16, 2, d)) and _whole(cw, cw.dtype, cw.dim(), d) and
+            _whole(layer.a_log_bias, f32, 2, d) and _whole(layer.norm_weight, f32, 1, d)):
+        _refuse(qkv, (("qkv", qkv, f16, 2, False), ("a", a, f16, 2, False), ("b", b, f16, 2, False),
+                      ("z", z, f16, 2, False), ("conv_state", conv_state, f16, 3, True),
+                      ("state", state, f32, 4, True), ("start", start, i32, 1, True),
+                      ("counts", counts, i32, 1, True), ("state_out", state_out, f32, 4, True),
+                      ("conv_out", conv_out, f16, 3, True), ("out", out, f16, 2, True),
+                      ("conv_weight", cw, cw.dtype, cw.dim(), True),
+                      ("a_log_bias", layer.a_log_bias, f32, 2, True), ("norm_weight", layer.norm_weight, f32, 1, True)))
+    ctx = Context.get(d)
     h, total, batch = layer.num_heads, qkv.shape[0], start.shape[0] - 1
     inner = h * layer.value_dim
     if out is None and state_out is None:
@@ -517,7 +563,7 @@ def deltanet_decode_span(layer, qkv, conv_state, state, a, b, z, start, counts=N
     for t, shape in shapes:
         if t is not None and t.shape != shape:
             _bad(f"expected a tensor of shape {shape}, got {tuple(t.shape)}")
-    if layer.conv_weight.numel() != 3 * inner * layer.conv_kernel or layer.conv_weight.element_size() != 2:
+    if cw.numel() != 3 * inner * layer.conv_kernel or cw.element_size() != 2:
         _bad("conv_weight: expected fp16 [conv_dim, conv_kernel]")
     if total > 1 and a.stride(0) != b.stride(0):
         _bad("a and b must have the same row stride")
@@ -526,7 +572,7 @@ def deltanet_decode_span(layer, qkv, conv_state, state, a, b, z, start, counts=N
     ctx.check(lib().spock_deltanet_decode_span(
         ctx.h, ctypes.byref(st), batch, start.data_ptr(), p(counts), total, qkv.data_ptr(), _row_stride(qkv),
         a.data_ptr(), b.data_ptr(), _row_stride(a), p(z), 0 if z is None else _row_stride(z), conv_state.data_ptr(),
-        state.data_ptr(), p(conv_out), p(state_out), p(out), _stream_of(qkv, stream)))
+        state.data_ptr(), p(conv_out), p(state_out), p(out), _stream_of(d, stream)))
     return out if out is not None else (state_out, conv_out)
 
 
@@ -540,14 +586,21 @@ def draft_verify(logits, tokens, start, u_accept, u_sample, temperature=None, dr
     from, or None for drafts without one. Returns (emitted int32 [batch], out_tokens int32 [total]): the accepted
     drafts, the next token, then -1."""
     import torch
-    f32, i32 = torch.float32, torch.int32
-    if logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    f32, i32, dt, d = torch.float32, torch.int32, logits.dtype, logits.get_device()
+    if dt not in (f32, torch.float16, torch.bfloat16):
         raise SpockError(SPOCK_ERR_UNSUPPORTED, "logits are fp32, fp16 or bf16")
-    ctx = _ragged(logits, (("logits", logits, logits.dtype, 2, False), ("tokens", tokens, i32, 1, True),
-                           ("start", start, i32, 1, True), ("u_accept", u_accept, f32, 1, True),
-                           ("u_sample", u_sample, f32, 1, True), ("temperature", temperature, f32, 1, True),
-                           ("draft_probs", draft_probs, f32, 2, False), ("emitted", emitted, i32, 1, True),
-                           ("out_tokens", out_tokens, i32, 1, True)))
+    if not (d >= 0 and _rows(logits, dt, 2, d) and _whole(tokens, i32, 1, d) and _whole(start, i32, 1, d) and
+            _whole(u_accept, f32, 1, d) and _whole(u_sample, f32, 1, d) and
+            (temperature is None or _whole(temperature, f32, 1, d)) and
+            (draft_probs is None or _rows(draft_probs, f32, 2, d)) and (emitted is None or _whole(emitted, i32, 1, d)) and
+            (out_tokens is None or _whole(out_tokens, i32, 1, d)) and
+            (workspace is None or _whole(workspace, torch.uint8, 1, d))):
+        _refuse(logits, (("logits", logits, dt, 2, False), ("tokens", tokens, i32, 1, True),
+                         ("start", start, i32, 1, True), ("u_accept", u_accept, f32, 1, True),
+                         ("u_sample", u_sample, f32, 1, True), ("temperature", temperature, f32, 1, True),
+                         ("draft_probs", draft_probs, f32, 2, False), ("emitted", emitted, i32, 1, True),
+                         ("out_tokens", out_tokens, i32, 1, True), ("workspace", workspace, torch.uint8, 1, True)))
+    ctx = Context.get(d)
     (total, vocab), batch = logits.shape, start.shape[0] - 1
     if (tokens.shape[0] != total or u_accept.shape[0] != total or u_sample.shape[0] != batch or
             (temperature is not None and temperature.shape[0] != batch) or
@@ -556,14 +609,13 @@ def draft_verify(logits, tokens, start, u_accept, u_sample, temperature=None, dr
             (out_tokens is not None and out_tokens.shape[0] != total)):
         _bad("tokens, u_accept and out_tokens have a value per row, u_sample, temperature and emitted one per sequence")
     if emitted is None:
-        emitted = _new(batch, i32, logits, stream)
+        emitted = _new((batch,), i32, logits, stream)
     if out_tokens is None:
-        out_tokens = _new(total, i32, logits, stream)
+        out_tokens = _new((total,), i32, logits, stream)
     if workspace is None:
         workspace, n = _workspace(ctx, lib().spock_draft_verify_workspace, ("verify", total, vocab, batch), logits,
                                   stream)
     else:
-        _ragged(logits, (("workspace", workspace, torch.uint8, 1, True),))
         n = workspace.shape[0]
     p = lambda t: None if t is None else t.data_ptr()
     ctx.check(lib().spock_draft_verify(
@@ -571,7 +623,7 @@ def draft_verify(logits, tokens, start, u_accept, u_sample, temperature=None, dr
         batch, start.data_ptr(), tokens.data_ptr(), p(draft_probs),
         0 if draft_probs is None else draft_probs.stride(0) if total > 1 else vocab, p(temperature),
         u_accept.data_ptr(), u_sample.data_ptr(), emitted.data_ptr(), out_tokens.data_ptr(), workspace.data_ptr(), n,
-        _stream_of(logits, stream)))
+        _stream_of(d, stream)))
     return emitted, out_tokens
 
 
