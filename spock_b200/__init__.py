@@ -80,6 +80,7 @@ def build(force=False):
     from . import builder as _b
     lib_path = _b.build(force=force)
     _b.build_apps(force=force)
+    _b.build_binding(force=force)
     return lib_path
 
 
@@ -330,6 +331,26 @@ def deltanet_recurrent(q, k, v, g, beta, state, num_heads=16, key_dim=128, value
     return out
 
 
+_BINDING = None
+
+
+def _binding():
+    """The ragged steps' short way into the library (csrc/binding.cpp), built in-tree when absent."""
+    global _BINDING
+    if _BINDING is None:
+        lib()
+        import importlib.machinery
+        import importlib.util
+        import torch  # noqa: F401  (its libraries are loaded first)
+        from . import builder
+        path = builder.build_binding()
+        loader = importlib.machinery.ExtensionFileLoader("spock_b200._binding", path)
+        spec = importlib.util.spec_from_file_location("spock_b200._binding", path, loader=loader)
+        _BINDING = importlib.util.module_from_spec(spec)
+        loader.exec_module(_BINDING)
+    return _BINDING
+
+
 # ---- ragged steps: several new tokens per sequence, packed rows ----------------
 # `start` int32 [batch + 1]: sequence b owns rows start[b] .. start[b + 1] - 1 of
 # every row-shaped tensor. All tensors of a call are on one device; the work goes
@@ -360,8 +381,15 @@ def _refuse(first, tensors):
     _bad("expected CUDA tensors")
 
 
-# The checks that every call passes, as cheap as they can be made: at decode
-# sizes the host's time per call is what counts. `d` is the device index.
+def _checked(d, r):
+    """A result of the binding: a status that is not SPOCK_OK raises."""
+    if type(r) is int:
+        Context.get(d).check(r)
+    return r
+
+
+# The wrappers' own checks. The binding makes them first; what it does not take
+# (a named stream, an argument to refuse) goes on here. `d` is the device index.
 def _rows(t, dtype, ndim, d):
     """A tensor of contiguous rows (any strides before the last dimension)."""
     return t.dtype is dtype and t.dim() == ndim and t.get_device() == d and (t.stride(-1) == 1 or t.shape[-1] <= 1)
@@ -438,7 +466,13 @@ def paged_attention_prep(proj, start, k_pages, v_pages, page_table, kv_len, rope
     kv_len int32 [batch], the new tokens included; rope fp32 [positions, rotary / 2, 2] (cos, sin) or None;
     q_norm, k_norm [head_dim] ((1 + w) RMSNorm) or None. Returns q [total, q_heads, head_dim]."""
     import torch
-    i32, f32, dt, d = torch.int32, torch.float32, k_pages.dtype, proj.get_device()
+    d = proj.get_device()
+    if d >= 0 and stream is None:
+        r = _binding().paged_attention_prep(Context.get(d).h.value, proj, start, k_pages, v_pages, page_table, kv_len,
+                                            rope, q_norm, k_norm, gated, eps, q_out)
+        if r is not None:
+            return _checked(d, r)
+    i32, f32, dt = torch.int32, torch.float32, k_pages.dtype
     if not (d >= 0 and _rows(proj, dt, 2, d) and _whole(start, i32, 1, d) and _rows(k_pages, dt, 4, d) and
             _rows(v_pages, dt, 4, d) and _rows(page_table, i32, 2, d) and _whole(kv_len, i32, 1, d) and
             (rope is None or _whole(rope, f32, 3, d)) and (q_norm is None or _whole(q_norm, dt, 1, d)) and
@@ -493,7 +527,13 @@ def paged_attention(q, start, k_pages, v_pages, page_table, kv_len, scale, gate=
     times sigmoid(gate); rows behind start[batch] are left as they are. `workspace`: a uint8 tensor of
     the caller's instead of one from the caching allocator."""
     import torch
-    i32, dt, d = torch.int32, k_pages.dtype, q.get_device()
+    d = q.get_device()
+    if d >= 0 and stream is None:
+        r = _binding().paged_attention(Context.get(d).h.value, q, start, k_pages, v_pages, page_table, kv_len, scale,
+                                       gate, out, workspace)
+        if r is not None:
+            return _checked(d, r)
+    i32, dt = torch.int32, k_pages.dtype
     if not (d >= 0 and _rows(q, dt, 3, d) and _whole(start, i32, 1, d) and _rows(k_pages, dt, 4, d) and
             _rows(v_pages, dt, 4, d) and _rows(page_table, i32, 2, d) and _whole(kv_len, i32, 1, d) and
             (gate is None or _rows(gate, dt, 3, d)) and (out is None or _whole(out, dt, 3, d)) and
@@ -536,7 +576,15 @@ def deltanet_decode_span(layer, qkv, conv_state, state, a, b, z, start, counts=N
     else is asked for) the gated outputs [total, heads * 128] are written and returned; with state_out and conv_out
     (which may be state and conv_state) the state after each sequence's first counts[b] rows (None: all)."""
     import torch
-    f16, f32, i32, d = torch.float16, torch.float32, torch.int32, qkv.get_device()
+    d = qkv.get_device()
+    if d >= 0 and stream is None:
+        r = _binding().deltanet_decode_span(Context.get(d).h.value, layer.num_heads, layer.key_dim, layer.value_dim,
+                                            layer.conv_kernel, layer.eps, layer.conv_weight, layer.a_log_bias,
+                                            layer.norm_weight, qkv, conv_state, state, a, b, z, start, counts,
+                                            state_out, conv_out, out)
+        if r is not None:
+            return _checked(d, r)
+    f16, f32, i32 = torch.float16, torch.float32, torch.int32
     cw = layer.conv_weight
     if not (d >= 0 and _rows(qkv, f16, 2, d) and _rows(a, f16, 2, d) and _rows(b, f16, 2, d) and
             (z is None or _rows(z, f16, 2, d)) and _whole(conv_state, f16, 3, d) and _whole(state, f32, 4, d) and
@@ -586,7 +634,13 @@ def draft_verify(logits, tokens, start, u_accept, u_sample, temperature=None, dr
     from, or None for drafts without one. Returns (emitted int32 [batch], out_tokens int32 [total]): the accepted
     drafts, the next token, then -1."""
     import torch
-    f32, i32, dt, d = torch.float32, torch.int32, logits.dtype, logits.get_device()
+    d = logits.get_device()
+    if d >= 0 and stream is None:
+        r = _binding().draft_verify(Context.get(d).h.value, logits, tokens, start, u_accept, u_sample, temperature,
+                                    draft_probs, emitted, out_tokens, workspace)
+        if r is not None:
+            return _checked(d, r)
+    f32, i32, dt = torch.float32, torch.int32, logits.dtype
     if dt not in (f32, torch.float16, torch.bfloat16):
         raise SpockError(SPOCK_ERR_UNSUPPORTED, "logits are fp32, fp16 or bf16")
     if not (d >= 0 and _rows(logits, dt, 2, d) and _whole(tokens, i32, 1, d) and _whole(start, i32, 1, d) and

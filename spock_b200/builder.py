@@ -70,6 +70,37 @@ def build_apps(force=False, verbose=False):
             raise RuntimeError("nvcc failed on " + src)
 
 
+BINDING = os.path.join(HERE, "_binding.so")
+
+
+def build_binding(force=False, verbose=False):
+    """The Python wrappers' short way into the library (csrc/binding.cpp): a
+    CPython extension over torch's tensors, linked against libspock_b200.so."""
+    src = os.path.join(CSRC, "binding.cpp")
+    deps = [src, os.path.join(HERE, "..", "include", "spock_b200.h")]
+    if not force and os.path.exists(BINDING) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in deps):
+        return BINDING
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
+    libdir = os.path.join(root, "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+    cmd += ["-isystem" + i for i in inc]
+    cmd += [src, "-o", BINDING, "-L" + HERE, "-l:libspock_b200.so", "-Wl,-rpath,$ORIGIN", "-L" + libdir, "-lc10",
+            "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath," + libdir]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or r.returncode:
+        sys.stderr.write(r.stdout + r.stderr)
+    if r.returncode:
+        raise RuntimeError("g++ failed on binding.cpp")
+    return BINDING
+
+
 if __name__ == "__main__":
     build(force="--force" in sys.argv, verbose="-v" in sys.argv)
     build_apps(force="--force" in sys.argv, verbose="-v" in sys.argv)
+    build_binding(force="--force" in sys.argv, verbose="-v" in sys.argv)

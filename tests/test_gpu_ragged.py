@@ -711,3 +711,32 @@ def test_one_speculative_step(cuda_ok):
             assert float((kp[ids, slot].float() - kp2[ids, slot].float()).abs().max()) <= 2 * 2.0 ** -10 * 4
             assert float((vp[ids, slot].float() - vp2[ids, slot].float()).abs().max()) <= 2 * 2.0 ** -10 * 4
         last = torch.stack([out[int(starts[b]) + int(emitted[b]) - 1] for b in range(3)])
+
+
+def test_wrappers_and_binding_agree(cuda_ok):
+    """The binding's short way and the wrappers' own (taken when a stream is named) give the same bits."""
+    g = _gen(21)
+    c = Cache([70, 9], 16, 2, 64, F16, g)
+    s = _i32([0, 3, 4])
+    rows = torch.randn(4, 4, 2, 64, device=DEV, generator=g).half()
+    cur = torch.cuda.current_stream()
+    a = spock_b200.paged_attention(rows[:, :, 0], s, *c.args(), 0.125, gate=rows[:, :, 1])
+    b = spock_b200.paged_attention(rows[:, :, 0], s, *c.args(), 0.125, gate=rows[:, :, 1], stream=cur)
+    assert torch.equal(a, b)
+    proj = torch.randn(4, 12 * 64, device=DEV, generator=g).half()
+    c2 = Cache([70, 9], 16, 2, 64, F16, _gen(21))
+    a = spock_b200.paged_attention_prep(proj, s, *c.args(), rope=_table(80, 64))
+    b = spock_b200.paged_attention_prep(proj, s, *c2.args(), rope=_table(80, 64), stream=cur)
+    assert torch.equal(a, b) and torch.equal(c.k.view(torch.int16), c2.k.view(torch.int16))
+    layer, qkv, conv, state, ga, gb, z = _span_inputs([3, 1], 4, seed=3)
+    a = spock_b200.deltanet_decode_span(layer, qkv, conv, state, ga, gb, z, s)
+    assert torch.equal(a, spock_b200.deltanet_decode_span(layer, qkv, conv, state, ga, gb, z, s, stream=cur))
+    new = [torch.empty_like(state), torch.empty_like(conv), torch.empty_like(state), torch.empty_like(conv)]
+    spock_b200.deltanet_decode_span(layer, qkv, conv, state, ga, gb, None, s, state_out=new[0], conv_out=new[1])
+    spock_b200.deltanet_decode_span(layer, qkv, conv, state, ga, gb, None, s, state_out=new[2], conv_out=new[3],
+                                    stream=cur)
+    assert torch.equal(new[0], new[2]) and torch.equal(new[1], new[3])
+    logits, tokens, ua, us, q = _verify_inputs([3, 1], 500, F16, 2, True)
+    a = spock_b200.draft_verify(logits, tokens, s, ua, us, None, q)
+    b = spock_b200.draft_verify(logits, tokens, s, ua, us, None, q, stream=cur)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
