@@ -1,0 +1,526 @@
+// spock_paged_attention for few query rows a sequence (decode tokens, drafts):
+// the tensor-core tile turned over.
+//
+// With 128 query rows on the M side (paged_attn_tc.cu) a decode token's 4 rows
+// would leave 124 lanes of every softmax and output instruction idle: it was
+// bound by those (133 us for 256 sequences), not by the cache it reads. Here M is
+// the cache's side, and N the rows, 16 or 32:
+//   S^T = K Q^T   M = 128 positions  N = rows  K = head dims
+//   O^T += V^T P^T  M = 128 dims (twice at head size 256)  N = rows  K = positions
+// K and V come straight from their tiles as the A operands (V M-major), the
+// queries and the weights are the small B operands in shared memory. A softmax
+// thread holds one position's scores of all rows; no maximum crosses lanes unless
+// a score exceeds its row's reference by 2^8, which one barrier with a vote finds
+// out for the block. O^T has dims on the lanes, so outputs and gates are read and
+// written in whole rows. Bound by the cache's bytes: an SM streams a tile (128
+// positions, 128 KB at head size 256) in some 5700 cycles of HBM's time, its MMAs
+// take 2300.
+//
+// One CTA per SM walks its share (paged_attn.cuh). Warp roles:
+//   warp 0      K and V tiles by TMA into a ring
+//   warp 1, 2   issue S^T = K Q^T and O^T += V^T P^T
+//   warp 3      queries of the next row tile (two buffers)
+//   warps 4-7   softmax, a position per thread
+//   warps 8-11  outputs of the finished row tile (O^T has two buffers), while the
+//               others are at the next one
+// Parts of cut row tiles, masked slots and bounded waits as in paged_attn_tc.cu.
+#include <atomic>
+
+#include "paged_attn.cuh"
+#include "ragged.h"
+
+namespace spock {
+namespace {
+
+using namespace paged;
+
+template <int D, int NR>
+struct Few {
+  static constexpr int DB = 128, KS = D / DB, VP = kTile / KS;
+  static constexpr int kStage = kTile * DB * 2;
+  static constexpr int kQ = NR * D * 2;       // one of two query buffers: [64-dim block][row][128 B]
+  static constexpr int kP = NR * kTile * 2;   // one of two weight buffers: [64-position block][row][128 B]
+  static constexpr int NST = NR == 32 && D == 256 ? 5 : 6;
+  static constexpr int kRing = 2 * kQ + 2 * kP;
+  static constexpr int kBar = kRing + NST * kStage;
+  static constexpr int kStat = kBar + 512;    // [2 row tiles][4 warps][NR] sums, [2][NR] references
+  static constexpr int kMax = kStat + 2 * 5 * NR * 4;  // [4 warps][NR] maxima
+  static constexpr int kSmem = kMax + 4 * NR * 4;
+  static constexpr int kBlocks = D / 128;     // M blocks of O^T
+  static constexpr int kO = 2 * NR;           // TMEM: S^T [2][NR], then O^T [2][kBlocks][NR]
+};
+static_assert(Few<256, 32>::kSmem <= 227 * 1024 && Few<256, 16>::kSmem <= 227 * 1024, "shared memory of one SM");
+
+template <int NR>
+__device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[NR]) {
+  if constexpr (NR == 16)
+    tc::tmem_ld16(at, v);
+  else
+    tc::tmem_ld32(at, v);
+}
+template <int NR>
+__device__ __forceinline__ void tmem_store(uint32_t at, const float (&v)[NR]) {
+  if constexpr (NR == 16)
+    tc::tmem_st16(at, v);
+  else
+    tc::tmem_st32(at, v);
+}
+
+template <typename T, int D, int NR>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_few_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                     const __grid_constant__ AttnArgs A) {
+  using Sh = Few<D, NR>;
+  constexpr int DB = Sh::DB, KS = Sh::KS, NST = Sh::NST, NB = Sh::kBlocks;
+  constexpr bool kBf16 = !std::is_same<T, __half>::value;
+  extern __shared__ __align__(1024) uint8_t sm[];  // no static shared memory beside it, so it starts on 1024 bytes
+  // [2] barriers are indexed by a tile's or row tile's parity, so that a waiter
+  // that comes late never finds one a whole phase further on
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + Sh::kBar);
+  uint64_t* empty = full + NST;
+  uint64_t* q_full = empty + NST;    // [2]
+  uint64_t* q_empty = q_full + 2;    // [2]
+  uint64_t* s_full = q_full + 4;     // [2]
+  uint64_t* s_free = q_full + 6;     // [2]
+  uint64_t* p_full = q_full + 8;     // [2]
+  uint64_t* p_free = q_full + 10;    // [2] also: O^T += V^T P^T of the tile is done
+  uint64_t* o_full = q_full + 12;    // [2]
+  uint64_t* o_free = q_full + 14;    // [2]
+  uint64_t* stats = q_full + 16;     // [2]
+  uint64_t* drain = q_full + 18;
+  volatile int* s_fail = reinterpret_cast<volatile int*>(q_full + 19);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(q_full + 19) + 1;
+  int64_t* s_scan = reinterpret_cast<int64_t*>(sm + Sh::kBar + 264);  // [warps + 2]
+  int* s_first = reinterpret_cast<int*>(s_scan + kThreads / 32 + 2);  // [4]
+  volatile int* s_issued = s_first + 4;
+  static_assert((2 * NST + 20) * 8 <= 264 && 264 + (kThreads / 32 + 2) * 8 + 20 <= 512, "barrier area");
+  float* s_sum = reinterpret_cast<float*>(sm + Sh::kStat);
+  float* s_ref = s_sum + 2 * 4 * NR;
+  float* s_max = reinterpret_cast<float*>(sm + Sh::kMax);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = blockIdx.x, ctas = gridDim.x;
+  Meta* meta = reinterpret_cast<Meta*>(A.ws);
+  float* parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(A.ws) + meta_bytes(ctas));
+
+  if (tc::smem_u32(sm) & 1023) {  // never on this toolchain; the operand layouts need it
+    if (tid == 0) atomicExch(A.err, 6);
+    return;
+  }
+  if (tid == 0) {
+    for (int i = 0; i < NST; ++i) {
+      tc::mbar_init(&full[i], 1);
+      tc::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&q_full[i], 1);
+      tc::mbar_init(&q_empty[i], 1);
+      tc::mbar_init(&s_full[i], 1);
+      tc::mbar_init(&s_free[i], 4);
+      tc::mbar_init(&p_full[i], 4);
+      tc::mbar_init(&p_free[i], 1);
+      tc::mbar_init(&o_full[i], 1);
+      tc::mbar_init(&o_free[i], 4);
+      tc::mbar_init(&stats[i], 4);
+    }
+    tc::mbar_init(drain, 2);
+    *s_fail = 0;
+    *s_issued = 0;
+    tc::fence_mbar_init();
+    tc::prefetch_tmap(&tmk);
+    tc::prefetch_tmap(&tmv);
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(s_tmem, 256);
+    tc::tmem_relinquish();
+  }
+  pdl_wait();
+  pdl_launch();
+
+  Walk w;
+  const int N = enter_share(A, s_scan, s_first, w);  // KV tiles of this CTA
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tb = *s_tmem;
+  const uint32_t sbase = tc::smem_u32(sm);
+  auto o_at = [&](int item, int blk) { return tb + Sh::kO + ((item & 1) * NB + blk) * NR; };
+
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(tc::smem_u32(bar), parity, s_fail); };
+  // For warps that meet at named barriers: a wait that gives up does not leave
+  // the loop (each later wait returns at once; the outputs are unspecified).
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
+    if (lane == 0) wait(bar, parity);  // one lane polls: 32 would crowd the pipe that MMAs and loads go through
+    __syncwarp();
+    tc::tc_fence_after();
+  };
+
+  if (N == 0) {
+    if (tid == 0) meta[cta].slot = -1, meta[cta].units = 0;
+  } else if (warp == 0) {
+    load_tiles<D, NST, Sh::kStage>(tmk, tmv, A, w, N, sm + Sh::kRing, full, empty, s_issued, wait);
+  } else if (warp == 1) {
+    // ---- S^T = K Q^T ----
+    if (lane == 0) {
+      constexpr uint32_t ID_S = tc::idesc_f16(128, NR, false, false, kBf16);
+      int item = 0, k = w.k0;
+      for (int g = 0; g < N; ++g) {
+        if (k == w.k0 && !wait(&q_full[item & 1], (item >> 1) & 1)) break;
+        if (g >= 2 && !wait(&s_free[g & 1], ((g - 2) >> 1) & 1)) break;
+        bool ok = true;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const int use = load_of_k(g, KS) + s, st = use % NST;
+          if (!(ok = wait(&full[st], (use / NST) & 1))) break;
+          tc::tc_fence_after();
+          const uint32_t kd = tc::sdesc_lo(sbase + Sh::kRing + st * Sh::kStage, 16);
+          const uint32_t qd = tc::sdesc_lo(sbase + (item & 1) * Sh::kQ + s * 2 * NR * 128, 16);
+#pragma unroll
+          for (int ks = 0; ks < DB / 16; ++ks)
+            tc::mma_f16(tb + (g & 1) * NR, kd + (ks >> 2) * 64 + (ks & 3) * 2, tc::sdesc_hi((DB / 64) * 1024),
+                        qd + (ks >> 2) * NR * 8 + (ks & 3) * 2, tc::sdesc_hi(1024), ID_S, (s | ks) > 0);
+          tc::mma_commit(&empty[st]);
+        }
+        if (!ok) break;
+        tc::mma_commit(&s_full[g & 1]);
+        if (++k == w.k1) {
+          tc::mma_commit(&q_empty[item & 1]);
+          if (w.next(A)) k = w.k0;
+          ++item;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // ---- O^T += V^T P^T ----
+    if (lane == 0) {
+      constexpr uint32_t ID_O = tc::idesc_f16(128, NR, true, false, kBf16);
+      constexpr uint32_t kGroup = (D / 64) * 1024;  // bytes from one 8-position group of a stage to the next
+      int item = 0, k = w.k0;
+      bool first = true;
+      for (int g = 0; g < N; ++g) {
+        if (!wait(&p_full[g & 1], (g >> 1) & 1)) break;
+        if (first && item >= 2 && !wait(&o_free[item & 1], ((item - 2) >> 1) & 1)) break;
+        tc::tc_fence_after();
+        bool ok = true;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const int use = load_of_v(g, N, KS) + s, st = use % NST;
+          if (!(ok = wait(&full[st], (use / NST) & 1))) break;
+          tc::tc_fence_after();
+          const uint32_t vd = tc::sdesc_lo(sbase + Sh::kRing + st * Sh::kStage, 1024);
+          const uint32_t pd = tc::sdesc_lo(sbase + 2 * Sh::kQ + (g & 1) * Sh::kP, 16);
+          const uint32_t od = o_at(item, 0);
+#pragma unroll
+          for (int ks = 0; ks < Sh::VP / 16; ++ks) {
+            const int kk = s * (Sh::VP / 16) + ks;
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+              tc::mma_f16(od + blk * NR, vd + (ks * 2 * kGroup + blk * 2048) / 16, tc::sdesc_hi(kGroup),
+                          pd + (kk >> 2) * NR * 8 + (kk & 3) * 2, tc::sdesc_hi(1024), ID_O, kk > 0 || !first);
+          }
+          tc::mma_commit(&empty[st]);
+        }
+        if (!ok) break;
+        tc::mma_commit(&p_free[g & 1]);
+        first = false;
+        if (++k == w.k1) {
+          tc::mma_commit(&o_full[item & 1]);
+          if (w.next(A)) k = w.k0;
+          ++item;
+          first = true;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    // ---- queries: rows behind the row tile's last are zero ----
+    for (int item = 0;; ++item) {
+      bool ok = true;
+      if (item >= 2) {
+        if (lane == 0) ok = wait(&q_empty[item & 1], ((item - 2) >> 1) & 1);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+      }
+      if (!ok) break;
+      const int t0 = w.rt * A.tp, rows = min(A.tp, w.s.n - t0) * A.G;
+      constexpr int CH = D / 8, RW = 32 / CH > 0 ? 32 / CH : 1;  // 16-byte chunks of a row; rows per warp instruction
+      const int sub = lane / (CH < 32 ? CH : 32), c = lane % CH;
+      const uint32_t qb = sbase + (item & 1) * Sh::kQ;
+      int r = sub, tt = r / A.G, gh = r - tt * A.G;
+#pragma unroll 4
+      for (; r < NR; r += RW) {
+        const uint32_t dst = qb + (c >> 3) * NR * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+        if (r < rows) {
+          cp_async16(dst, A.q + (int64_t)(w.s.lo + t0 + tt) * A.q_row + (int64_t)(w.h * A.G + gh) * A.q_head + c * 16);
+        } else {
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
+        }
+        gh += RW;
+        while (gh >= A.G) gh -= A.G, ++tt;
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      tc::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&q_full[item & 1]);
+      if (!w.next(A)) break;
+    }
+  } else if (warp < 8) {
+    // ---- softmax: thread = position of the tile ----
+    const int quad = warp & 3, at = quad * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    const float c = A.scale_log2;
+    float ref[NR], l[NR];  // log2 units; a row that has seen nothing yet refers to -1e30
+    int k = w.k0, item = 0;
+    auto enter = [&] {
+#pragma unroll
+      for (int r = 0; r < NR; ++r) ref[r] = -1e30f, l[r] = 0.f;
+    };
+    enter();
+    for (int g = 0; g < N; ++g) {
+      const int buf = g & 1, p0 = k * kTile;
+      const int t0 = w.rt * A.tp, lim0 = w.s.len - w.s.n + t0;  // the last position the first row sees
+      wait_warp(&s_full[buf], (g >> 1) & 1);
+      float s[NR];
+      tmem_load<NR>(tb + buf * NR + lane_off, s);
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&s_free[buf]);
+      if (p0 + kTile > w.s.len) {  // slots behind the sequence: their V rows become zero
+        const int first = max(0, w.s.len - p0);
+        // O^T of tile g - 1 is done, so every earlier load of V(g)'s stages is over:
+        // their barriers are at most one phase behind and the parities are V(g)'s
+        if (g > 0) wait_warp(&p_free[buf ^ 1], ((g - 1) >> 1) & 1);
+#pragma unroll
+        for (int st = 0; st < KS; ++st) {
+          const int use = load_of_v(g, N, KS) + st;
+          wait_warp(&full[use % NST], (use / NST) & 1);
+          zero_rows<D, Sh::VP>(sm + Sh::kRing + use % NST * Sh::kStage, max(0, first - st * Sh::VP), at, 128);
+        }
+        tc::fence_async_smem();
+      }
+#pragma unroll
+      for (int r = 0; r < NR; ++r) s[r] *= c;
+      if (p0 + kTile - 1 > lim0) {
+        int lim = lim0 - (p0 + at), n = 0;  // >= 0: this position is seen by the row
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          s[r] = lim >= 0 ? s[r] : -INFINITY;
+          if (++n == A.G) n = 0, ++lim;
+        }
+      }
+      bool over = false;
+#pragma unroll
+      for (int r = 0; r < NR; ++r) over |= s[r] - ref[r] > kLazy;
+      uint32_t any;
+      asm volatile(
+          "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
+          : "=r"(any)
+          : "r"((uint32_t)over)
+          : "memory");
+      if (any) {  // some row's reference moves: the rows' maxima over the tile
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          float m = s[r];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          if (lane == 0) s_max[quad * NR + r] = m;
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        float corr[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          const float m = fmaxf(fmaxf(s_max[r], s_max[NR + r]), fmaxf(s_max[2 * NR + r], s_max[3 * NR + r]));
+          const bool move = m - ref[r] > kLazy;
+          corr[r] = move ? ex2(ref[r] - m) : 1.0f;
+          ref[r] = move ? m : ref[r];
+          l[r] *= corr[r];
+        }
+        if (k > w.k0) {
+          wait_warp(&p_free[buf ^ 1], ((g - 1) >> 1) & 1);
+#pragma unroll 1
+          for (int blk = 0; blk < NB; ++blk) {
+            float o[NR];
+            tmem_load<NR>(o_at(item, blk) + lane_off, o);
+#pragma unroll
+            for (int r = 0; r < NR; ++r) o[r] *= corr[r];
+            tmem_store<NR>(o_at(item, blk) + lane_off, o);
+          }
+          tc::tmem_st_wait();
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");  // the maxima have been read
+      }
+      if (g >= 2) wait_warp(&p_free[buf], ((g - 2) >> 1) & 1);
+      uint8_t* pw = sm + 2 * Sh::kQ + buf * Sh::kP + (at >> 6) * NR * 128 + (at & 7) * 2;
+      const int ch = (at & 63) >> 3;
+#pragma unroll
+      for (int r = 0; r < NR; r += 2) {
+        const float a = ex2(s[r] - ref[r]), b = ex2(s[r + 1] - ref[r + 1]);
+        l[r] += a;
+        l[r + 1] += b;
+        const uint32_t u = Io<T>::down2(a, b);
+        *reinterpret_cast<uint16_t*>(pw + r * 128 + ((ch ^ (r & 7)) << 4)) = (uint16_t)u;
+        *reinterpret_cast<uint16_t*>(pw + (r + 1) * 128 + ((ch ^ ((r + 1) & 7)) << 4)) = (uint16_t)(u >> 16);
+      }
+      tc::fence_async_smem();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&p_full[buf]);
+      if (++k < w.k1) continue;
+
+      // ---- the row tile's last KV tile here: sums over this warp's positions, row r's in lane r (and r + 16) ----
+      if (item >= 2) wait_warp(&o_free[item & 1], ((item - 2) >> 1) & 1);
+      if constexpr (NR == 16) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) l[r] += __shfl_xor_sync(0xffffffffu, l[r], 16);
+      }
+#pragma unroll
+      for (int o = NR / 2; o > 0; o >>= 1) {
+#pragma unroll
+        for (int r = 0; r < o; ++r) {
+          const float keep = lane & o ? l[r + o] : l[r], send = lane & o ? l[r] : l[r + o];
+          l[r] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+      }
+      if (lane < NR) s_sum[((item & 1) * 4 + quad) * NR + lane] = l[0];
+      if (quad == 0) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+          if (lane == r) s_ref[(item & 1) * NR + r] = ref[r];
+      }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&stats[item & 1]);
+      if (w.next(A)) {
+        k = w.k0;
+        ++item;
+        enter();
+      }
+    }
+  } else {
+    // ---- outputs: thread = dim ----
+    const int quad = warp & 3, dim = quad * 32 + lane, heads = A.kv_heads * A.G;
+    const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    if (tid == 256) meta[cta].slot = -1, meta[cta].units = N;
+    for (int item = 0;; ++item) {
+      const int t0 = w.rt * A.tp, rows = min(A.tp, w.s.n - t0) * A.G, row0 = w.s.lo + t0;
+      const bool whole = w.k0 == 0 && w.k1 == w.nt;
+      const int slot = item == 0 ? 0 : 1;
+      if (!whole && w.k0 == 0 && tid == 256) {
+        Meta& mt = meta[cta];
+        mt.slot = slot;
+        mt.row0 = row0;
+        mt.rows = rows;
+        mt.head = w.h;
+        mt.have = w.k1;
+        mt.nt = w.nt;
+      }
+      wait_warp(&stats[item & 1], (item >> 1) & 1);
+      wait_warp(&o_full[item & 1], (item >> 1) & 1);
+      const float* sums = s_sum + (item & 1) * 4 * NR;
+      float* part = parts + ((size_t)cta * 2 + slot) * part_floats<D>();
+#pragma unroll 1
+      for (int blk = 0; blk < NB; ++blk) {
+        T gate[NR];
+        if (A.gate && whole) {
+          const uint8_t* gp = A.gate + row0 * A.g_row + (int64_t)w.h * A.G * A.g_head + (blk * 128 + dim) * 2;
+          int n = 0;
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            if (r < rows) {
+              gate[r] = *reinterpret_cast<const T*>(gp);
+              gp += A.g_head;
+              if (++n == A.G) n = 0, gp += A.g_row - A.G * A.g_head;
+            }
+          }
+        }
+        float o[NR];
+        tmem_load<NR>(o_at(item, blk) + lane_off, o);
+        T* op = reinterpret_cast<T*>(A.out) + ((int64_t)row0 * heads + w.h * A.G) * D + blk * 128 + dim;
+        float* pp = part + blk * 128 + dim;
+        int n = 0;
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          if (r < rows) {
+            if (whole) {
+              const float lt = (sums[r] + sums[NR + r]) + (sums[2 * NR + r] + sums[3 * NR + r]);
+              float x = lt == 0.f ? 0.f : __fdividef(o[r], lt);
+              if (A.gate) x = __fdividef(x, 1.0f + __expf(-to_float(gate[r])));
+              *op = from_float<T>(x);
+              op += D;
+              if (++n == A.G) n = 0, op += (int64_t)(heads - A.G) * D;
+            } else {
+              pp[r * D] = o[r];
+            }
+          }
+        }
+      }
+      if (!whole && dim < rows) {  // the part's references and sums, a row per thread
+        const float ref = s_ref[(item & 1) * NR + dim];
+        part[128 * D + dim] = ref <= -1e29f ? -INFINITY : ref;
+        part[128 * D + 128 + dim] = (sums[dim] + sums[NR + dim]) + (sums[2 * NR + dim] + sums[3 * NR + dim]);
+      }
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&o_free[item & 1]);
+      if (!w.next(A)) break;
+    }
+  }
+  __syncwarp();
+  tc::tc_fence_before();
+  __syncthreads();
+  if (*s_fail) {
+    // let the copies and MMAs in flight land before shared memory and TMEM go
+    if (tid == 0) {
+      atomicExch(A.err, 5);
+      for (int st = 0; st < NST; ++st)
+        if (*s_issued > st) {
+          const int last = (*s_issued - 1 - st) / NST;
+          tc::mbar_wait_bounded(&full[st], last & 1, kWait);
+        }
+    }
+    if (tid == 32 || tid == 64) {
+      tc::mma_commit(drain);
+      tc::mbar_wait_bounded(drain, 0, kWait);
+    }
+    __syncthreads();
+  }
+  if (warp == 1) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tb, 256);
+  }
+}
+
+template <typename T, int D, int NR>
+Status launch(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& A, int sms, cudaStream_t st) {
+  // the attribute belongs to the kernel on the current device: set once on each
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e, "spock_paged_attention");
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(done.load() & bit)) {
+    e = cudaFuncSetAttribute(paged_few_kernel<T, D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<D, NR>::kSmem);
+    if (e != cudaSuccess) return cuda_status(e, "paged_few_kernel attribute");
+    done.fetch_or(bit);
+  }
+  e = launch_k(paged_few_kernel<T, D, NR>, dim3(sms), dim3(kThreads), Few<D, NR>::kSmem, st, mk, mv, A);
+  if (e != cudaSuccess) return cuda_status(e, "paged_few_kernel");
+  SPOCK_LAUNCH_CHECK("paged_few_kernel");
+  return Status::ok();
+}
+
+template <typename T>
+Status by_size(int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& A, int rows, int sms,
+               cudaStream_t st) {
+  if (head_dim == 128)
+    return rows == 16 ? launch<T, 128, 16>(mk, mv, A, sms, st) : launch<T, 128, 32>(mk, mv, A, sms, st);
+  return rows == 16 ? launch<T, 256, 16>(mk, mv, A, sms, st) : launch<T, 256, 32>(mk, mv, A, sms, st);
+}
+
+}  // namespace
+
+Status launch_paged_few(int dtype, int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const paged::AttnArgs& A,
+                        int rows, int sms, cudaStream_t st) {
+  if (dtype == SPOCK_F16) return by_size<__half>(head_dim, mk, mv, A, rows, sms, st);
+  return by_size<__nv_bfloat16>(head_dim, mk, mv, A, rows, sms, st);
+}
+
+}  // namespace spock

@@ -31,23 +31,24 @@
 #include <atomic>
 #include <mutex>
 
-#include "paged_sched.cuh"
-#include "ragged.cuh"
+#include "paged_attn.cuh"
 #include "ragged.h"
-#include "tc.cuh"
 
 namespace spock {
+Status launch_paged_few(int dtype, int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const paged::AttnArgs& A,
+                        int rows, int sms, cudaStream_t st);
+
 namespace {
 
-using sched::kTile;
-constexpr uint32_t kWait = 1u << 22;
-constexpr int kThreads = 384;
-constexpr float kLazy = 8.0f;  // log2 of how far weights may exceed 1
+using namespace paged;
 
 template <int D>
 struct Shape {
-  static constexpr int DB = D < 128 ? D : 128;  // dims per stage
-  static constexpr int KS = D / DB;             // stages per K (or V) tile
+  // A stage is 32 KB (16 KB at head size 64): of K 128 positions x DB dims, of V
+  // VP positions x all dims, so that each MMA of O += P V is as wide as O.
+  static constexpr int DB = D < 128 ? D : 128;
+  static constexpr int KS = D / DB;  // stages per K (or V) tile
+  static constexpr int VP = kTile / KS;
   static constexpr int kStage = kTile * DB * 2;
   static constexpr int kQ = 128 * D * 2;
   static constexpr int NST = D == 256 ? 5 : D == 128 ? 6 : 8;
@@ -56,92 +57,6 @@ struct Shape {
   static constexpr int kSmem = kRed + 4 * 128 * 4;
 };
 static_assert(Shape<256>::kSmem <= 227 * 1024 && Shape<128>::kSmem <= 227 * 1024, "shared memory of one SM");
-
-struct AttnArgs {
-  const int32_t *start, *table, *kv_len;
-  int64_t table_stride;
-  int batch, total, table_width, num_pages, page_size, kv_heads, G, tp, piece;
-  int64_t head_blk;  // 64-element blocks from one kv head to the next
-  const uint8_t *q, *gate;
-  int64_t q_row, q_head, g_row, g_head;  // bytes
-  uint8_t* out;
-  float scale_log2;
-  float* ws;
-  int* err;
-};
-
-// Workspace: per CTA a Meta and two parts (its first and its last row tile).
-// A part: O [128][D] fp32, then the reference maxima (log2 units) and sums [128].
-struct Meta {
-  int slot;      // part of the row tile that begins in this CTA and ends in a later one, or -1
-  int row0;      // its first packed row
-  int rows;      // valid rows (token, head of the group)
-  int head;      // kv head
-  int have, nt;  // KV tiles done here, in all
-  int units;     // of this CTA
-  int pad;
-};
-template <int D>
-__host__ __device__ constexpr size_t part_floats() {
-  return (size_t)128 * D + 256;
-}
-__host__ __device__ constexpr size_t meta_bytes(int ctas) { return ((size_t)ctas * sizeof(Meta) + 127) / 128 * 128; }
-
-struct Seq {
-  int lo, n, len;
-};
-__device__ __forceinline__ Seq load_seq(const AttnArgs& A, int b, bool report) {
-  Seq s;
-  s.lo = A.start[b];
-  const int hi = A.start[b + 1];
-  s.n = hi - s.lo;
-  s.len = A.kv_len[b];
-  if (s.lo < 0 || hi < s.lo || hi > A.total) {
-    if (report) report_bad_index(A.err);
-    s.n = 0;
-  }
-  if (s.len < 0 || s.len > A.table_width * A.page_size) {
-    if (report) report_bad_index(A.err);
-    s.len = 0;
-  }
-  return s;
-}
-
-// A role's way through the CTA's units.
-struct Walk {
-  int b, h, rt;
-  int k0, k1, nt;  // KV tiles of the current row tile: [k0, k1) here, nt in all
-  int64_t left;    // units from this row tile's first one on
-  Seq s;
-  __device__ __forceinline__ void fit(const AttnArgs& A) {
-    nt = sched::row_tile_units(s.n, s.len, A.tp, rt);
-    k1 = nt - k0 <= left ? nt : k0 + (int)left;
-  }
-  __device__ __forceinline__ bool next(const AttnArgs& A) {
-    left -= k1 - k0;
-    if (left <= 0) return false;
-    k0 = 0;
-    if (++rt * A.tp >= s.n) {
-      rt = 0;
-      if (++h == A.kv_heads) {
-        h = 0;
-        do s = load_seq(A, ++b, false);
-        while (s.n <= 0 && b + 1 < A.batch);
-      }
-    }
-    fit(A);
-    return true;
-  }
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -157,12 +72,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_full + 2;   // [2]
   uint64_t* p_full = q_full + 4;   // [2]
+  // [2], by tile parity: a waiter that comes late must not find the barrier a
+  // whole phase further on
   uint64_t* o_done = q_full + 6;
-  uint64_t* drain = q_full + 7;
-  volatile int* s_fail = reinterpret_cast<volatile int*>(q_full + 8);
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(q_full + 8) + 1;
-  int64_t* s_scan = reinterpret_cast<int64_t*>(sm + Sh::kBar + 256);  // [warps]
-  int* s_first = reinterpret_cast<int*>(s_scan + kThreads / 32);      // [4]
+  uint64_t* drain = q_full + 8;
+  volatile int* s_fail = reinterpret_cast<volatile int*>(q_full + 9);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(q_full + 9) + 1;
+  int64_t* s_scan = reinterpret_cast<int64_t*>(sm + Sh::kBar + 256);  // [warps + 2]
+  int* s_first = reinterpret_cast<int*>(s_scan + kThreads / 32 + 2);  // [4]
   volatile int* s_issued = s_first + 4;
   float* red = reinterpret_cast<float*>(sm + Sh::kRed);  // [2 tiles][2 halves][128] maxima (and sums)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -184,8 +101,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&s_full[i], 1);
       tc::mbar_init(&p_full[i], 8);
+      tc::mbar_init(&o_done[i], 1);
     }
-    tc::mbar_init(o_done, 1);
     tc::mbar_init(drain, 1);
     *s_fail = 0;
     *s_issued = 0;
@@ -200,199 +117,81 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   pdl_launch();
 
-  // this CTA's first unit: prefix sums of the sequences' units over the block
-  const int per = (A.batch + kThreads - 1) / kThreads;
-  int64_t mine = 0;
-  for (int b = tid * per; b < min(A.batch, (tid + 1) * per); ++b) {
-    const Seq s = load_seq(A, b, cta == 0);
-    mine += sched::head_units(s.n, s.len, A.tp) * A.kv_heads;
-  }
-  int64_t incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
-  }
-  if (lane == 31) s_scan[warp] = incl;
-  __syncthreads();
-  int64_t base = 0, units = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) base += s_scan[w];
-    units += s_scan[w];
-  }
-  const int shares = units < ctas ? (int)units : ctas;  // none of them empty
-  const int64_t u0 = cta < shares ? sched::share_begin(units, cta, shares) : 0;
-  const int64_t u1 = cta < shares ? sched::share_begin(units, cta + 1, shares) : 0;
-  const int64_t from = base + incl - mine;
-  if (u1 > u0 && from <= u0 && u0 < from + mine) {
-    int64_t r = u0 - from;
-    for (int b = tid * per;; ++b) {
-      const Seq s = load_seq(A, b, false);
-      const int64_t hu = sched::head_units(s.n, s.len, A.tp);
-      if (r < hu * A.kv_heads) {
-        s_first[0] = b;
-        s_first[1] = (int)(r / hu);
-        r %= hu;
-        s_first[2] = sched::find_row_tile(s.n, s.len, A.tp, r);
-        s_first[3] = (int)r;
-        break;
-      }
-      r -= hu * A.kv_heads;
-    }
-  }
+  Walk w;
+  const int N = enter_share(A, s_scan, s_first, w);  // KV tiles of this CTA
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  const int N = (int)(u1 - u0);  // KV tiles of this CTA
   const uint32_t tb = *s_tmem, tO = tb + 256;
   const uint32_t sbase = tc::smem_u32(sm);
-  Walk w;
-  w.left = N;
-  if (N > 0) {
-    w.b = s_first[0];
-    w.h = s_first[1];
-    w.rt = s_first[2];
-    w.k0 = s_first[3];
-    w.s = load_seq(A, w.b, false);
-    w.fit(A);
-  }
 
-  // bounded wait; gives up at once when another role has
-  auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    for (uint32_t i = 0; i < kWait; ++i) {
-      if (tc::mbar_try_wait(bar, parity)) return true;
-      if (*s_fail) return false;
-    }
-    *s_fail = 1;
-    return false;
-  };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(tc::smem_u32(bar), parity, s_fail); };
 
   if (N == 0) {
     if (tid == 0) meta[cta].slot = -1, meta[cta].units = 0;
   } else if (warp == 0) {
-    // ---- K and V tiles: order K0, K1, V0, K2, V1, ... ----
-    struct Src {
-      int page, group, h, bytes;
-    };
-    const int pieces = kTile / A.piece;
-    // this lane's piece of KV tile k
-    auto locate = [&](const Walk& at, int k) -> Src {
-      Src r;
-      const int p0 = k * kTile, pos = p0 + lane * A.piece;
-      const bool live = lane < pieces && pos < at.s.len;
-      r.page = -1;
-      r.h = at.h;
-      r.group = 0;
-      if (live) {
-        const int slot = pos / A.page_size;
-        r.page = A.table[at.b * A.table_stride + slot];
-        r.group = (pos - slot * A.page_size) >> 3;
-      }
-      r.bytes = __popc(__ballot_sync(0xffffffffu, live)) * A.piece * DB * 2;
-      if (live && (r.page < 0 || r.page >= A.num_pages)) {
-        report_bad_index(A.err);
-        r.page = 0;
-      } else if (!live) {
-        r.page = -1;
-      }
-      return r;
-    };
-    int ld = 0;
-    auto load = [&](const CUtensorMap* map, const Src& src) -> bool {
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int st = ld % NST, round = ld / NST;
-        bool ok = true;
-        if (lane == 0) {
-          ok = round == 0 || wait(&empty[st], (round - 1) & 1);
-          if (ok) {
-            tc::mbar_arrive_expect_tx(&full[st], src.bytes);
-            *s_issued = ld + 1;
-          }
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) return false;
-        if (src.page >= 0)
-          tc::tma_load_5d(sm + Sh::kQ + st * Sh::kStage + lane * A.piece * DB * 2, map, &full[st], 0, 0,
-                          (int)(src.h * A.head_blk) + s * (DB / 64), src.group, src.page);
-        ++ld;
-      }
-      return true;
-    };
-    int k = w.k0;
-    Src cur = locate(w, k), nxt = cur;
-    bool ok = load(&tmk, cur);
-    for (int g = 0; g < N && ok; ++g) {
-      if (g + 1 < N) {
-        if (++k == w.k1) {
-          w.next(A);
-          k = w.k0;
-        }
-        nxt = locate(w, k);
-        ok = load(&tmk, nxt);
-      }
-      if (ok) ok = load(&tmv, cur);
-      cur = nxt;
-    }
+    load_tiles<D, NST, Sh::kStage>(tmk, tmv, A, w, N, sm + Sh::kQ, full, empty, s_issued, wait);
   } else if (warp == 1) {
     // ---- MMAs ----
     if (lane == 0) {
       constexpr uint32_t ID_S = tc::idesc_f16(128, kTile, false, false, kBf16);
-      constexpr uint32_t ID_O = tc::idesc_f16(128, DB, false, true, kBf16);
-      constexpr uint32_t kGroup = (DB / 64) * 1024;  // bytes from one 8-position group of a stage to the next
-      int use = 0, item = 0, k = w.k0;
-      bool ok = true;
+      constexpr uint32_t ID_O = tc::idesc_f16(128, D, false, true, kBf16);
+      constexpr uint32_t kGroup = (D / 64) * 1024;  // bytes from one 8-position group of a V stage to the next
+      int item = 0, k = w.k0;
       auto issue_s = [&](int g) -> bool {
         if (k == w.k0 && !wait(q_full, item & 1)) return false;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          const int st = use % NST;
+          const int use = load_of_k(g, KS) + s, st = use % NST;
           if (!wait(&full[st], (use / NST) & 1)) return false;
           tc::tc_fence_after();
-          const uint32_t kb = sbase + Sh::kQ + st * Sh::kStage;
+          const uint32_t kd = tc::sdesc_lo(sbase + Sh::kQ + st * Sh::kStage, 16);
+          const uint32_t qd = tc::sdesc_lo(sbase + s * (DB / 64) * 16384, 16);
 #pragma unroll
           for (int ks = 0; ks < DB / 16; ++ks)
-            tc::mma_f16(tb + (g & 1) * kTile,
-                        tc::sdesc(sbase + (s * (DB / 64) + (ks >> 2)) * 16384 + (ks & 3) * 32, 16, 1024),
-                        tc::sdesc(kb + (ks >> 2) * 1024 + (ks & 3) * 32, 16, kGroup), ID_S, (s | ks) > 0);
+            tc::mma_f16(tb + (g & 1) * kTile, qd + (ks >> 2) * 1024 + (ks & 3) * 2, tc::sdesc_hi(1024),
+                        kd + (ks >> 2) * 64 + (ks & 3) * 2, tc::sdesc_hi((DB / 64) * 1024), ID_S, (s | ks) > 0);
           tc::mma_commit(&empty[st]);
-          ++use;
         }
         tc::mma_commit(&s_full[g & 1]);
         if (k + 1 == w.k1) tc::mma_commit(q_empty);
         return true;
       };
-      ok = issue_s(0);
-      bool first = true;  // tile g is its row tile's first here: O starts from zero
+      auto issue_o = [&](int g, bool first) -> bool {  // first: O starts from zero
+        if (!wait(&p_full[g & 1], (g >> 1) & 1)) return false;
+        tc::tc_fence_after();
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const int use = load_of_v(g, N, KS) + s, st = use % NST;
+          if (!wait(&full[st], (use / NST) & 1)) return false;
+          tc::tc_fence_after();
+          const uint32_t vd = tc::sdesc_lo(sbase + Sh::kQ + st * Sh::kStage, 1024);
+#pragma unroll
+          for (int ks = 0; ks < Sh::VP / 16; ++ks)
+            tc::mma_f16_ta(tO, tb + (g & 1) * kTile + (s * (Sh::VP / 16) + ks) * 8, vd + ks * 2 * kGroup / 16,
+                           tc::sdesc_hi(kGroup), ID_O, (s | ks) > 0 || !first);
+          tc::mma_commit(&empty[st]);
+        }
+        tc::mma_commit(&o_done[g & 1]);
+        return true;
+      };
+      bool ok = issue_s(0), first = true;
       for (int g = 0; g < N && ok; ++g) {
         bool next_first = false;
         if (g + 1 < N) {
-          if (++k == w.k1) {
+          if (++k == w.k1) {  // the next row tile's queries may be on their way: this one's O goes first
+            ok = issue_o(g, first);
             w.next(A);
             k = w.k0;
             ++item;
             next_first = true;
+            ok = ok && issue_s(g + 1);
+          } else {
+            ok = issue_s(g + 1) && issue_o(g, first);
           }
-          ok = issue_s(g + 1);
-          if (!ok) break;
+        } else {
+          ok = issue_o(g, first);
         }
-        if (!(ok = wait(&p_full[g & 1], (g >> 1) & 1))) break;
-        tc::tc_fence_after();
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const int st = use % NST;
-          if (!(ok = wait(&full[st], (use / NST) & 1))) break;
-          tc::tc_fence_after();
-          const uint32_t vb = sbase + Sh::kQ + st * Sh::kStage;
-#pragma unroll
-          for (int ks = 0; ks < kTile / 16; ++ks)
-            tc::mma_f16_ta(tO + s * DB, tb + (g & 1) * kTile + ks * 8,
-                           tc::sdesc(vb + ks * 2 * kGroup, 1024, kGroup), ID_O, !first || ks > 0);
-          tc::mma_commit(&empty[st]);
-          ++use;
-        }
-        tc::mma_commit(o_done);
         first = next_first;
       }
     }
@@ -407,10 +206,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       const int t0 = w.rt * A.tp, rows = min(A.tp, w.s.n - t0) * A.G;
-      constexpr int CH = D / 8;               // 16-byte chunks of a row
+      constexpr int CH = D / 8;                   // 16-byte chunks of a row
       constexpr int RW = CH >= 32 ? 1 : 32 / CH;  // rows per warp instruction
+      constexpr int step = 2 * RW;
       const int sub = CH >= 32 ? 0 : lane / CH, c = CH >= 32 ? lane : lane % CH;
-      const int step = 2 * RW;
       int r = (warp - 2) * RW + sub, tt = r / A.G, gh = r - tt * A.G;
       for (; r < rows; r += step) {
         const uint8_t* src = A.q + (int64_t)(w.s.lo + t0 + tt) * A.q_row + (int64_t)(w.h * A.G + gh) * A.q_head + c * 16;
@@ -433,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // named barriers, so all of them walk on (each later wait returns at once)
     // and the outputs are unspecified.
     auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
-      wait(bar, parity);
+      if (lane == 0) wait(bar, parity);  // one lane polls: 32 would crowd the pipe that MMAs and loads go through
       __syncwarp();
       tc::tc_fence_after();
     };
@@ -457,20 +256,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool live = quad * 32 < rows;
       wait_warp(&s_full[buf], (g >> 1) & 1);
       if (p0 + kTile > w.s.len) {  // slots behind the sequence: their V rows become zero
-        const int pos = g + 1 < N ? 2 * g + 2 : 2 * N - 1, first = max(0, w.s.len - p0);
+        const int first = max(0, w.s.len - p0);
         // V(g - 1) has been read, so every earlier load of V(g)'s stages is over:
         // their barriers are at most one phase behind and the parities are V(g)'s
-        if (g > 0) wait_warp(o_done, (g - 1) & 1);
+        if (g > 0) wait_warp(&o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-          const int use = pos * KS + s, st = use % NST;
+          const int use = load_of_v(g, N, KS) + s, st = use % NST, from = max(0, first - s * Sh::VP);
           wait_warp(&full[st], (use / NST) & 1);
-          uint8_t* vb = sm + Sh::kQ + st * Sh::kStage;
-          for (int i = tid - 128; i < (kTile - first) * (DB / 8); i += 256) {
-            const int r = first + i / (DB / 8), ch = i % (DB / 8);
-            *reinterpret_cast<uint4*>(vb + (r >> 3) * (DB / 64) * 1024 + (ch >> 3) * 1024 + (r & 7) * 128 +
-                                      (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
+          zero_rows<D, Sh::VP>(sm + Sh::kQ + st * Sh::kStage, from, tid - 128, 256);
         }
         tc::fence_async_smem();
       }
@@ -495,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (move) m = top;
           l *= corr;
           if (k > w.k0) {
-            wait_warp(o_done, (g - 1) & 1);
+            wait_warp(&o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
 #pragma unroll 1
             for (int cb = 0; cb < D / 64; ++cb) {
               float o[32];
@@ -527,11 +321,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (++k < w.k1) continue;
 
       // ---- the row tile's last KV tile here ----
-      // one phase at a time: P(g) may be ready while O += P(g-1) V(g-1) still runs,
-      // and the parity of phase g alone would then be that of phase g - 2
-      if (g > 0) wait_warp(o_done, (g - 1) & 1);
-      wait_warp(o_done, g & 1);
       const bool whole = w.k0 == 0 && w.k1 == w.nt;
+      const int64_t tok = w.s.lo + t0 + tt;
+      const int hq = w.h * A.G + row - tt * A.G;
+      wait_warp(&o_done[buf], (g >> 1) & 1);
       const int slot = item == 0 ? 0 : 1;
       if (!whole && w.k0 == 0 && tid == 128) {
         Meta& mt = meta[cta];
@@ -550,24 +343,26 @@ __global__ void __launch_bounds__(kThreads, 1)
         pair_sync();  // read before the next tile's maxima go there
         if (whole) {
           const float inv = lt == 0.f ? 0.f : 1.0f / lt;
-          const int64_t tok = w.s.lo + t0 + tt;
-          const int hq = w.h * A.G + row - tt * A.G;
           uint8_t* op = A.out + (tok * (A.kv_heads * A.G) + hq) * (D * 2) + half * D;
-          const uint8_t* gp = A.gate ? A.gate + tok * A.g_row + hq * A.g_head + half * D : nullptr;
+          const uint8_t* gp = A.gate + tok * A.g_row + hq * A.g_head + half * D;
 #pragma unroll 1
           for (int cb = 0; cb < D / 64; ++cb) {
+            uint32_t gw[16];
+            if (A.gate && row < rows) {
+#pragma unroll
+              for (int v = 0; v < 4; ++v) load_words(gp + cb * 64 + v * 16, reinterpret_cast<uint32_t(&)[4]>(gw[4 * v]));
+            }
             float o[32];
             tc::tmem_ld32(tO + lane_off + half * (D / 2) + cb * 32, o);
             if (row < rows) {
 #pragma unroll
               for (int v = 0; v < 4; ++v) {
-                uint32_t x[4], gw[4];
-                if (gp) load_words(gp + cb * 64 + v * 16, gw);
+                uint32_t x[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   float a = o[v * 8 + 2 * e] * inv, b = o[v * 8 + 2 * e + 1] * inv;
-                  if (gp) {
-                    const float2 z = Io<T>::up2(gw[e]);
+                  if (A.gate) {
+                    const float2 z = Io<T>::up2(gw[v * 4 + e]);
                     a = __fdividef(a, 1.0f + __expf(-z.x));
                     b = __fdividef(b, 1.0f + __expf(-z.y));
                   }
@@ -731,48 +526,57 @@ EncodeFn encode() {
 // box of a piece's groups lands as [group][block][8][128 B], which both the
 // K-major and the MN-major operand layouts read with constant strides whatever
 // the page size. The blocks of head h start at h * head_stride / 64.
-CUresult encode_pages(EncodeFn fn, CUtensorMap* map, const spock_paged_kv& kv, void* base, int piece, int db) {
+CUresult encode_pages(EncodeFn fn, CUtensorMap* map, const spock_paged_kv& kv, void* base, int piece, int dims_box) {
   const int64_t blocks = (kv.kv_heads - 1) * (kv.head_stride / 64) + kv.head_dim / 64;
   cuuint64_t dims[5] = {64, 8, (cuuint64_t)blocks, (cuuint64_t)kv.page_size / 8, (cuuint64_t)kv.num_pages};
   cuuint64_t strides[4] = {(cuuint64_t)kv.pos_stride * 2, 128, (cuuint64_t)kv.pos_stride * 16,
                            (cuuint64_t)kv.page_stride * 2};
-  cuuint32_t box[5] = {64, 8, (cuuint32_t)db / 64, (cuuint32_t)piece / 8, 1};
+  cuuint32_t box[5] = {64, 8, (cuuint32_t)dims_box / 64, (cuuint32_t)piece / 8, 1};
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   return fn(map, kv.dtype == SPOCK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, base,
             dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
+int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
 template <typename T, int D>
-Status launch(const spock_paged_kv& kv, AttnArgs& A, int sms, cudaStream_t st) {
+Status launch(const spock_paged_kv& kv, AttnArgs& A, int few, int sms, cudaStream_t st) {
   EncodeFn fn = encode();
   if (!fn) return Status::err(SPOCK_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  A.tp = (few ? few : 128) / A.G;
+  A.piece_k = gcd(kv.page_size, kTile);
+  A.piece_v = gcd(kv.page_size, Shape<D>::VP);
   CUtensorMap mk, mv;
-  if (encode_pages(fn, &mk, kv, kv.k, A.piece, Shape<D>::DB) != CUDA_SUCCESS ||
-      encode_pages(fn, &mv, kv, kv.v, A.piece, Shape<D>::DB) != CUDA_SUCCESS)
+  if (encode_pages(fn, &mk, kv, kv.k, A.piece_k, Shape<D>::DB) != CUDA_SUCCESS ||
+      encode_pages(fn, &mv, kv, kv.v, A.piece_v, D) != CUDA_SUCCESS)
     return Status::err(SPOCK_ERR_CUDA, "spock_paged_attention: tensor map encoding failed");
-  // the attribute belongs to the kernel on the current device: set once on each
-  static std::atomic<uint64_t> done{0};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return cuda_status(e, "spock_paged_attention");
-  const uint64_t bit = 1ull << (dev & 63);
-  if (!(done.load() & bit)) {
-    e = cudaFuncSetAttribute(paged_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
-    if (e != cudaSuccess) return cuda_status(e, "paged_attn_kernel attribute");
-    done.fetch_or(bit);
+  cudaError_t e;
+  if (few) {
+    const Status s = launch_paged_few(kv.dtype, D, mk, mv, A, few, sms, st);
+    if (s.code) return s;
+  } else {
+    // the attribute belongs to the kernel on the current device: set once on each
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return cuda_status(e, "spock_paged_attention");
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(done.load() & bit)) {
+      e = cudaFuncSetAttribute(paged_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+      if (e != cudaSuccess) return cuda_status(e, "paged_attn_kernel attribute");
+      done.fetch_or(bit);
+    }
+    e = launch_k(paged_attn_kernel<T, D>, dim3(sms), dim3(kThreads), Shape<D>::kSmem, st, mk, mv, A);
+    if (e != cudaSuccess) return cuda_status(e, "paged_attn_kernel");
+    SPOCK_LAUNCH_CHECK("paged_attn_kernel");
   }
-  e = launch_k(paged_attn_kernel<T, D>, dim3(sms), dim3(kThreads), Shape<D>::kSmem, st, mk, mv, A);
-  if (e != cudaSuccess) return cuda_status(e, "paged_attn_kernel");
-  SPOCK_LAUNCH_CHECK("paged_attn_kernel");
   pdl_scope overlap;  // the join's launch runs under the main kernel
   e = launch_k(paged_join_kernel<T, D>, dim3(sms, 4), dim3(256), 0, st, A);
   if (e != cudaSuccess) return cuda_status(e, "paged_join_kernel");
   SPOCK_LAUNCH_CHECK("paged_join_kernel");
   return Status::ok();
 }
-
-int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 }  // namespace
 
@@ -796,8 +600,6 @@ Status launch_paged_attention(const spock_paged_kv& kv, int batch, const int32_t
   A.page_size = kv.page_size;
   A.kv_heads = kv.kv_heads;
   A.G = q_heads / kv.kv_heads;
-  A.tp = 128 / A.G;
-  A.piece = gcd(kv.page_size, kTile);
   A.head_blk = kv.head_stride / 64;
   A.q = (const uint8_t*)q;
   A.gate = (const uint8_t*)gate;
@@ -809,14 +611,25 @@ Status launch_paged_attention(const spock_paged_kv& kv, int batch, const int32_t
   A.scale_log2 = scale * 1.44269504088896341f;
   A.ws = (float*)ws;
   A.err = err;
-  if (kv.dtype == SPOCK_F16) {
-    if (kv.head_dim == 64) return launch<__half, 64>(kv, A, sms, st);
-    if (kv.head_dim == 128) return launch<__half, 128>(kv, A, sms, st);
-    return launch<__half, 256>(kv, A, sms, st);
+  // Either kernel is right for every batch; the rows a sequence brings on average
+  // decide. A row tile of 32 rows costs half of one of 128 (all of the cache's
+  // side, little of the rows'), so a few long chunks among many decode tokens lose
+  // less than the decode tokens gain.
+  int few = 0;
+  if (kv.head_dim >= 128) {
+    if (total <= batch && A.G <= 16)
+      few = 16;
+    else if (total * A.G <= 32 * (int64_t)batch && A.G <= 32)
+      few = 32;
   }
-  if (kv.head_dim == 64) return launch<__nv_bfloat16, 64>(kv, A, sms, st);
-  if (kv.head_dim == 128) return launch<__nv_bfloat16, 128>(kv, A, sms, st);
-  return launch<__nv_bfloat16, 256>(kv, A, sms, st);
+  if (kv.dtype == SPOCK_F16) {
+    if (kv.head_dim == 64) return launch<__half, 64>(kv, A, few, sms, st);
+    if (kv.head_dim == 128) return launch<__half, 128>(kv, A, few, sms, st);
+    return launch<__half, 256>(kv, A, few, sms, st);
+  }
+  if (kv.head_dim == 64) return launch<__nv_bfloat16, 64>(kv, A, few, sms, st);
+  if (kv.head_dim == 128) return launch<__nv_bfloat16, 128>(kv, A, few, sms, st);
+  return launch<__nv_bfloat16, 256>(kv, A, few, sms, st);
 }
 
 }  // namespace spock

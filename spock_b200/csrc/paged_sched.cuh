@@ -1,13 +1,15 @@
 // How spock_paged_attention cuts a ragged batch into equal shares.
 //
-// A row tile is `tp` = 128 / G whole tokens of one sequence times the G query
-// heads of one kv head (at most 128 rows); its work is the KV tiles of kTile
+// A row tile is `tp` whole tokens of one sequence times the G query heads of one
+// kv head (tp = R / G, at most R = 128 rows, or 16 or 32 in the kernel for few
+// rows); its work is the KV tiles of kTile
 // positions that its last token sees, at least one (a row tile that sees
 // nothing still has zeros to write). All row tiles' KV tiles, in the order
 // sequence, kv head, row tile, KV tile, form one line of units; share c of C
-// is units [U c / C, U (c + 1) / C). A row tile cut by a border is computed in
-// parts and joined afterwards, so one long sequence, many short ones and any
-// mix all keep every SM busy without the host knowing any length.
+// is units [U c / C, U (c + 1) / C), its borders moved off short row tiles. A row
+// tile cut by a border is computed in parts and joined afterwards, so one long
+// sequence, many short ones and any mix all keep every SM busy without the host
+// knowing any length.
 #pragma once
 #include <stdint.h>
 
@@ -17,7 +19,7 @@ namespace sched {
 constexpr int kTile = 128;
 
 // sum of floor((b + i a) / m) over i in [0, n): Euclid's steps on (a, m)
-__host__ __device__ inline int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+__host__ __device__ __noinline__ inline int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
   int64_t s = 0;
   while (n > 0) {
     if (a >= m) {
@@ -46,7 +48,8 @@ __host__ __device__ inline int row_tile_units(int n, int len, int tp, int j) {
   return seen <= kTile ? 1 : (int)((seen + kTile - 1) / kTile);
 }
 // the same summed over row tiles 0 .. j-1, none of them the last
-__host__ __device__ inline int64_t units_before(int n, int len, int tp, int64_t j) {
+__host__ __device__ __noinline__ inline int64_t units_before(int n, int len, int tp, int64_t j) {
+  if (j == 0) return 0;
   const int64_t off = (int64_t)len - n;
   int64_t j0 = off < 0 ? -off / tp : 0;  // row tiles that see nothing: one unit each
   if (j0 > j) j0 = j;
@@ -56,6 +59,7 @@ __host__ __device__ inline int64_t units_before(int n, int len, int tp, int64_t 
 __host__ __device__ inline int64_t head_units(int n, int len, int tp) {
   if (n <= 0) return 0;
   const int last = (n + tp - 1) / tp - 1;
+  if (last == 0) return row_tile_units(n, len, tp, 0);
   return units_before(n, len, tp, last) + row_tile_units(n, len, tp, last);
 }
 // the row tile that unit r of a head falls into (r becomes the unit within it)

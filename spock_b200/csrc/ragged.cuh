@@ -59,6 +59,15 @@ struct Io<__nv_bfloat16> {
   }
 };
 
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
 // N 32-bit words (2 N values) at a 4 N-byte aligned address.
 template <int N>
 __device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[N]) {
