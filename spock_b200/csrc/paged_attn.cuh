@@ -15,12 +15,13 @@ using sched::kTile;
 constexpr uint32_t kWait = 1u << 20;    // polls before a wait gives up
 constexpr uint32_t kSleep = 20000;      // ns that one poll may sleep
 constexpr int kThreads = 384;
+constexpr int kFewRows = 16;  // rows of a row tile of the few-row kernel
 constexpr float kLazy = 8.0f;  // log2 of how far weights may exceed 1
 
 struct AttnArgs {
   const int32_t *start, *table, *kv_len;
   int64_t table_stride;
-  int batch, total, table_width, num_pages, page_size, kv_heads, G, tp, piece_k, piece_v;
+  int batch, total, table_width, num_pages, page_size, kv_heads, G, tp, piece_k, piece_v, whole;
   int64_t head_blk;  // 64-element blocks from one kv head to the next
   const uint8_t *q, *gate;
   int64_t q_row, q_head, g_row, g_head;  // bytes
@@ -137,10 +138,12 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 // This CTA's share: the first row tile and KV tile in w; the KV tiles it has. All
 // threads (it synchronises). scan: kThreads / 32 + 2 words, first: 4.
 //
-// Prefix sums of the sequences' units over the block, then the borders. A border
-// inside a row tile of at most half a share moves to the row tile's nearer end:
-// shares grow or shrink by a quarter at most, and short row tiles are not cut
-// (a part costs a round trip through the workspace and the join).
+// Prefix sums of the sequences' units over the block, then the borders. Where a
+// part is dear (A.whole: 128 rows of it make a round trip through the workspace)
+// a border inside a row tile of at most half a share moves to the row tile's
+// nearer end: shares grow or shrink by a quarter at most, and short row tiles are
+// not cut. Parts of few rows are cheap, and equal shares worth more (256 decode
+// tokens: 18 KV tiles a CTA, 24 at most with moved borders).
 static __device__ __noinline__ int enter_share(const AttnArgs& A, int64_t* scan, int* first, Walk& w) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x, ctas = gridDim.x;
   const int per = (A.batch + kThreads - 1) / kThreads;
@@ -167,40 +170,36 @@ static __device__ __noinline__ int enter_share(const AttnArgs& A, int64_t* scan,
   const int shares = units < ctas ? (int)units : ctas;  // none of them empty
   if (cta >= shares) return 0;
   int64_t* border = scan + kThreads / 32;
-  // sequence, head, row tile and KV tile of unit u (in this thread's range); the row tile's units
-  auto locate = [&](int64_t u, int& b, int& h, int& rt, int& k) -> int {
-    int64_t r = u - from;
-    for (b = tid * per;; ++b) {
-      const Seq s = load_seq(A, b, false);
-      const int64_t hu = sched::head_units(s.n, s.len, A.tp);
-      if (r < hu * A.kv_heads) {
-        for (h = 0; r >= hu; ++h) r -= hu;
-        rt = sched::find_row_tile(s.n, s.len, A.tp, r);
-        k = (int)r;
-        return sched::row_tile_units(s.n, s.len, A.tp, rt);
-      }
-      r -= hu * A.kv_heads;
-    }
-  };
+  if (tid < 2) border[tid] = sched::share_begin(units, cta + tid, shares);
+  __syncthreads();
+  // 0, 1: move the borders (where parts are dear); 2: the first row tile
 #pragma unroll 1
-  for (int i = 0; i < 2; ++i) {
-    const int64_t u = sched::share_begin(units, cta + i, shares);
-    if (u == 0 || u == units) {
-      if (tid == 0) border[i] = u;
-    } else if (from <= u && u < from + mine) {
-      int b, h, rt, k;
-      const int nt = locate(u, b, h, rt, k);
-      border[i] = 2 * nt > units / shares ? u : 2 * k <= nt ? u - k : u - k + nt;
+  for (int i = A.whole ? 0 : 2; i < 3; ++i) {
+    const int64_t u = border[i < 2 ? i : 0];
+    if (A.whole) __syncthreads();  // all have read it before its finder moves it
+    if (from <= u && u < from + mine && (i == 2 || u > 0)) {
+      int64_t r = u - from;
+      int b = tid * per, h = 0;
+      Seq s;
+#pragma unroll 1
+      for (;; ++b) {
+        s = load_seq(A, b, false);
+        const int64_t hu = sched::head_units(s.n, s.len, A.tp);
+#pragma unroll 1
+        for (h = 0; h < A.kv_heads && r >= hu; ++h) r -= hu;
+        if (h < A.kv_heads) break;
+      }
+      const int rt = sched::find_row_tile(s.n, s.len, A.tp, r), k = (int)r;
+      if (i == 2) {
+        first[0] = b, first[1] = h, first[2] = rt, first[3] = k;
+      } else {
+        const int nt = sched::row_tile_units(s.n, s.len, A.tp, rt);
+        if (2 * nt <= units / shares) border[i] = 2 * k <= nt ? u - k : u - k + nt;
+      }
     }
+    __syncthreads();
   }
-  __syncthreads();
   const int64_t u0 = border[0], u1 = border[1];
-  if (from <= u0 && u0 < from + mine && u1 > u0) {
-    int b, h, rt, k;
-    locate(u0, b, h, rt, k);
-    first[0] = b, first[1] = h, first[2] = rt, first[3] = k;
-  }
-  __syncthreads();
   const int n = (int)(u1 - u0);
   w.left = n;
   if (n > 0) {
@@ -214,27 +213,38 @@ static __device__ __noinline__ int enter_share(const AttnArgs& A, int64_t* scan,
   return n;
 }
 
-// The loads of a share's K and V tiles, by one warp, in the order K0, K1, V0,
-// K2, V1, .. A stage is KP positions x KD dims of K or VP positions x all dims
+// The loads of a share's K (or V) tiles into the ring, by one warp each: issuing
+// a copy costs its thread some 190 cycles and a wait as much, and one warp for
+// both was slower than HBM. The ring's order is K0, K1, V0, K2, V1, .. (load_of_k,
+// load_of_v); a stage is 128 positions x DB dims of K or VP positions x all dims
 // of V, in [8-position group][64-dim block][8][128 B].
 //
-// A tile is fetched in pieces that lie in one page: of V piece_v positions, one
-// lane each, of K piece_k (a multiple, since a V stage has fewer positions). The
-// page table is read two tiles ahead and looked at only when the tile is loaded:
-// a lookup is a memory latency away.
-template <int D, int NST, int kStage, class Wait>
-__device__ __forceinline__ void load_tiles(const CUtensorMap& tmk, const CUtensorMap& tmv, const AttnArgs& A, Walk& w,
-                                           int N, uint8_t* ring, uint64_t* full, uint64_t* empty, volatile int* issued,
-                                           Wait wait) {
-  constexpr int DB = D < 128 ? D : 128, KS = D / DB, VP = kTile / KS;
+// A barrier must not be waited for while it is two phases behind (the parities
+// would agree). With 5 stages and two per tile, or 6 or 8 and one per tile, the
+// load before the last one into a stage is always known to have been read by
+// then: by the loads that the same warp has already made, and because O += P V of
+// tile g is issued after S of tiles <= g, and S of tile g after O += P V of tile
+// g - 2. (Not so with 6 stages and two per tile.)
+//
+// A tile is fetched in pieces that lie in one page, a lane each. The page table is
+// read two tiles ahead and looked at only when the tile is loaded: a lookup is a
+// memory latency away. armed[st]: loads into the stage so far.
+template <bool kV, int D, int NST, int kStage, class Wait>
+__device__ __forceinline__ void load_tiles(const CUtensorMap& map, const AttnArgs& A, Walk& w, int N, uint8_t* ring,
+                                           uint64_t* full, uint64_t* empty, volatile int* armed, Wait wait) {
+  constexpr int DB = D < 128 ? D : 128, KS = D / DB;
+  constexpr int kPos = kV ? kTile / KS : kTile;  // positions of a stage
+  constexpr int kRow = kV ? D * 2 : DB * 2;      // bytes of a position in it
+  static_assert((KS == 2 && NST == 5) || (KS == 1 && (NST == 6 || NST == 8)), "see above");
   const int lane = threadIdx.x & 31;
+  const int piece = kV ? A.piece_v : A.piece_k, per_stage = kPos / piece;
   struct Src {
     int page, group, live, h;  // of this lane's piece; pieces that hold positions; kv head
   };
   auto look_up = [&](int k) -> Src {
-    const int pos = k * kTile + lane * A.piece_v;
+    const int pos = k * kTile + lane * piece;
     Src r{-1, 0, 0, w.h};
-    const bool live = lane * A.piece_v < kTile && pos < w.s.len;
+    const bool live = lane * piece < kTile && pos < w.s.len;
     if (live) {
       const int slot = pos / A.page_size;
       r.page = A.table[w.b * A.table_stride + slot];
@@ -242,53 +252,6 @@ __device__ __forceinline__ void load_tiles(const CUtensorMap& tmk, const CUtenso
     }
     r.live = __popc(__ballot_sync(0xffffffffu, live));
     return r;
-  };
-  const int per_k = A.piece_k / A.piece_v, per_stage = VP / A.piece_v;  // V pieces per K piece, per V stage
-  auto check = [&](Src& r) {  // an entry out of range is reported and page 0 read in its place
-    if (lane < r.live && (r.page < 0 || r.page >= A.num_pages)) {
-      report_bad_index(A.err);
-      r.page = 0;
-    }
-  };
-  int ld = 0;
-  auto stage = [&](int bytes) -> int {  // the next load's stage, once it is free; -1: gave up
-    const int st = ld % NST, round = ld / NST;
-    bool ok = true;
-    if (lane == 0) {
-      ok = round == 0 || wait(&empty[st], (round - 1) & 1);
-      if (ok) {
-        tc::mbar_arrive_expect_tx(&full[st], bytes);
-        *issued = ld + 1;
-      }
-    }
-    ++ld;
-    return __shfl_sync(0xffffffffu, ok, 0) ? st : -1;
-  };
-  auto load_k = [&](const Src& src) -> bool {
-    const int n = (src.live + per_k - 1) / per_k;  // K pieces
-    const int page = __shfl_sync(0xffffffffu, src.page, (lane * per_k) & 31);
-    const int group = __shfl_sync(0xffffffffu, src.group, (lane * per_k) & 31);
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int st = stage(n * A.piece_k * DB * 2);
-      if (st < 0) return false;
-      if (lane < n)
-        tc::tma_load_5d(ring + st * kStage + lane * A.piece_k * DB * 2, &tmk, &full[st], 0, 0,
-                        (int)(src.h * A.head_blk) + s * (DB / 64), group, page);
-    }
-    return true;
-  };
-  auto load_v = [&](const Src& src) -> bool {
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int n = max(0, min(src.live - s * per_stage, per_stage)), i = lane - s * per_stage;
-      const int st = stage(n * A.piece_v * D * 2);
-      if (st < 0) return false;
-      if (i >= 0 && i < n)
-        tc::tma_load_5d(ring + st * kStage + i * A.piece_v * D * 2, &tmv, &full[st], 0, 0, (int)(src.h * A.head_blk),
-                        src.group, src.page);
-    }
-    return true;
   };
   int k = w.k0, seen = 1;
   auto advance = [&](Src& into) {
@@ -301,20 +264,41 @@ __device__ __forceinline__ void load_tiles(const CUtensorMap& tmk, const CUtenso
   };
   Src cur = look_up(k), nxt = cur, far = cur;
   advance(nxt);
-  check(cur);
-  bool ok = load_k(cur);
-  for (int g = 0; g < N && ok; ++g) {
+#pragma unroll 1
+  for (int g = 0; g < N; ++g) {
     advance(far);
-    if (g + 1 < N) {
-      check(nxt);
-      ok = load_k(nxt);
+    if (lane < cur.live && (cur.page < 0 || cur.page >= A.num_pages)) {  // reported, and page 0 read in its place
+      report_bad_index(A.err);
+      cur.page = 0;
     }
-    if (ok) ok = load_v(cur);
+    const int first = kV ? (g + 1 < N ? 2 * g + 2 : 2 * N - 1) * KS : (g == 0 ? 0 : 2 * g - 1) * KS;
+#pragma unroll 1
+    for (int s = 0; s < KS; ++s) {
+      const int use = first + s, st = use % NST, round = use / NST;
+      const int n = kV ? max(0, min(cur.live - s * per_stage, per_stage)) : cur.live;
+      if (lane == 0) {
+        if (round == 0 || wait(&empty[st], (round - 1) & 1)) {
+          armed[st] = round + 1;
+          tc::mbar_arrive_expect_tx(&full[st], n * piece * kRow);
+        }
+      }
+      __syncwarp();
+      if (armed[st] <= round) return;  // gave up
+      const int i = kV ? lane - s * per_stage : lane;
+      if (i >= 0 && i < n)
+        tc::tma_load_5d(ring + st * kStage + i * piece * kRow, &map, &full[st], 0, 0,
+                        (int)(cur.h * A.head_blk) + (kV ? 0 : s * (DB / 64)), cur.group, cur.page);
+    }
     cur = nxt;
     nxt = far;
   }
 }
-// The number of a tile's first load in that order.
+// After a wait that gave up: lets every stage's last copy land.
+__device__ __forceinline__ void drain_ring(uint64_t* full, const volatile int* armed, int stages) {
+  for (int st = 0; st < stages; ++st)
+    if (armed[st]) tc::mbar_wait_bounded(&full[st], (armed[st] - 1) & 1, kWait);
+}
+// The number of a tile's first load in the ring's order.
 __device__ __forceinline__ int load_of_k(int g, int KS) { return (g == 0 ? 0 : 2 * g - 1) * KS; }
 __device__ __forceinline__ int load_of_v(int g, int N, int KS) { return (g + 1 < N ? 2 * g + 2 : 2 * N - 1) * KS; }
 

@@ -4,7 +4,7 @@
 // With 128 query rows on the M side (paged_attn_tc.cu) a decode token's 4 rows
 // would leave 124 lanes of every softmax and output instruction idle: it was
 // bound by those (133 us for 256 sequences), not by the cache it reads. Here M is
-// the cache's side, and N the rows, 16 or 32:
+// the cache's side, and N the rows, 16:
 //   S^T = K Q^T   M = 128 positions  N = rows  K = head dims
 //   O^T += V^T P^T  M = 128 dims (twice at head size 256)  N = rows  K = positions
 // K and V come straight from their tiles as the A operands (V M-major), the
@@ -17,12 +17,11 @@
 // take 2300.
 //
 // One CTA per SM walks its share (paged_attn.cuh). Warp roles:
-//   warp 0      K and V tiles by TMA into a ring
-//   warp 1, 2   issue S^T = K Q^T and O^T += V^T P^T
-//   warp 3      queries of the next row tile (two buffers)
+//   warps 0, 3  K tiles and V tiles by TMA into a ring
+//   warps 1, 2  issue S^T = K Q^T and O^T += V^T P^T
 //   warps 4-7   softmax, a position per thread
-//   warps 8-11  outputs of the finished row tile (O^T has two buffers), while the
-//               others are at the next one
+//   warps 8-11  the queries of the row tile after the next, and the outputs of the
+//               finished one (O^T has two buffers), while the others are at the next
 // Parts of cut row tiles, masked slots and bounded waits as in paged_attn_tc.cu.
 #include <atomic>
 
@@ -34,13 +33,15 @@ namespace {
 
 using namespace paged;
 
-template <int D, int NR>
+constexpr int NR = kFewRows;
+
+template <int D>
 struct Few {
   static constexpr int DB = 128, KS = D / DB, VP = kTile / KS;
   static constexpr int kStage = kTile * DB * 2;
   static constexpr int kQ = NR * D * 2;       // one of two query buffers: [64-dim block][row][128 B]
   static constexpr int kP = NR * kTile * 2;   // one of two weight buffers: [64-position block][row][128 B]
-  static constexpr int NST = NR == 32 && D == 256 ? 5 : 6;
+  static constexpr int NST = D == 256 ? 5 : 6;
   static constexpr int kRing = 2 * kQ + 2 * kP;
   static constexpr int kBar = kRing + NST * kStage;
   static constexpr int kStat = kBar + 512;    // [2 row tiles][4 warps][NR] sums, [2][NR] references
@@ -49,28 +50,13 @@ struct Few {
   static constexpr int kBlocks = D / 128;     // M blocks of O^T
   static constexpr int kO = 2 * NR;           // TMEM: S^T [2][NR], then O^T [2][kBlocks][NR]
 };
-static_assert(Few<256, 32>::kSmem <= 227 * 1024 && Few<256, 16>::kSmem <= 227 * 1024, "shared memory of one SM");
+static_assert(Few<256>::kSmem <= 227 * 1024, "shared memory of one SM");
 
-template <int NR>
-__device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[NR]) {
-  if constexpr (NR == 16)
-    tc::tmem_ld16(at, v);
-  else
-    tc::tmem_ld32(at, v);
-}
-template <int NR>
-__device__ __forceinline__ void tmem_store(uint32_t at, const float (&v)[NR]) {
-  if constexpr (NR == 16)
-    tc::tmem_st16(at, v);
-  else
-    tc::tmem_st32(at, v);
-}
-
-template <typename T, int D, int NR>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_few_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                      const __grid_constant__ AttnArgs A) {
-  using Sh = Few<D, NR>;
+  using Sh = Few<D>;
   constexpr int DB = Sh::DB, KS = Sh::KS, NST = Sh::NST, NB = Sh::kBlocks;
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) uint8_t sm[];  // no static shared memory beside it, so it starts on 1024 bytes
@@ -81,19 +67,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_full = empty + NST;    // [2]
   uint64_t* q_empty = q_full + 2;    // [2]
   uint64_t* s_full = q_full + 4;     // [2]
-  uint64_t* s_free = q_full + 6;     // [2]
-  uint64_t* p_full = q_full + 8;     // [2]
-  uint64_t* p_free = q_full + 10;    // [2] also: O^T += V^T P^T of the tile is done
-  uint64_t* o_full = q_full + 12;    // [2]
-  uint64_t* o_free = q_full + 14;    // [2]
-  uint64_t* stats = q_full + 16;     // [2]
-  uint64_t* drain = q_full + 18;
-  volatile int* s_fail = reinterpret_cast<volatile int*>(q_full + 19);
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(q_full + 19) + 1;
+  uint64_t* p_full = q_full + 6;     // [2]
+  uint64_t* p_free = q_full + 8;     // [2] also: O^T += V^T P^T of the tile is done
+  uint64_t* o_full = q_full + 10;    // [2]
+  uint64_t* o_free = q_full + 12;    // [2]
+  uint64_t* stats = q_full + 14;     // [2]
+  uint64_t* drain = q_full + 16;
+  volatile int* s_fail = reinterpret_cast<volatile int*>(q_full + 17);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(q_full + 17) + 1;
   int64_t* s_scan = reinterpret_cast<int64_t*>(sm + Sh::kBar + 264);  // [warps + 2]
   int* s_first = reinterpret_cast<int*>(s_scan + kThreads / 32 + 2);  // [4]
-  volatile int* s_issued = s_first + 4;
-  static_assert((2 * NST + 20) * 8 <= 264 && 264 + (kThreads / 32 + 2) * 8 + 20 <= 512, "barrier area");
+  volatile int* s_armed = s_first + 4;  // [NST]
+  static_assert((2 * NST + 20) * 8 <= 264 && 264 + (kThreads / 32 + 2) * 8 + (4 + NST) * 4 <= 512, "barrier area");
   float* s_sum = reinterpret_cast<float*>(sm + Sh::kStat);
   float* s_ref = s_sum + 2 * 4 * NR;
   float* s_max = reinterpret_cast<float*>(sm + Sh::kMax);
@@ -112,10 +97,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&q_full[i], 1);
+      tc::mbar_init(&q_full[i], 4);
       tc::mbar_init(&q_empty[i], 1);
       tc::mbar_init(&s_full[i], 1);
-      tc::mbar_init(&s_free[i], 4);
       tc::mbar_init(&p_full[i], 4);
       tc::mbar_init(&p_free[i], 1);
       tc::mbar_init(&o_full[i], 1);
@@ -124,7 +108,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc::mbar_init(drain, 2);
     *s_fail = 0;
-    *s_issued = 0;
+    for (int i = 0; i < NST; ++i) s_armed[i] = 0;
     tc::fence_mbar_init();
     tc::prefetch_tmap(&tmk);
     tc::prefetch_tmap(&tmv);
@@ -157,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (N == 0) {
     if (tid == 0) meta[cta].slot = -1, meta[cta].units = 0;
   } else if (warp == 0) {
-    load_tiles<D, NST, Sh::kStage>(tmk, tmv, A, w, N, sm + Sh::kRing, full, empty, s_issued, wait);
+    load_tiles<false, D, NST, Sh::kStage>(tmk, A, w, N, sm + Sh::kRing, full, empty, s_armed, wait);
   } else if (warp == 1) {
     // ---- S^T = K Q^T ----
     if (lane == 0) {
@@ -165,16 +149,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       int item = 0, k = w.k0;
       for (int g = 0; g < N; ++g) {
         if (k == w.k0 && !wait(&q_full[item & 1], (item >> 1) & 1)) break;
-        if (g >= 2 && !wait(&s_free[g & 1], ((g - 2) >> 1) & 1)) break;
+        if (g >= 2 && !wait(&p_free[g & 1], ((g - 2) >> 1) & 1)) break;  // S^T(g - 2) has been read long before
         bool ok = true;
-#pragma unroll
+#pragma unroll 1
         for (int s = 0; s < KS; ++s) {
           const int use = load_of_k(g, KS) + s, st = use % NST;
           if (!(ok = wait(&full[st], (use / NST) & 1))) break;
           tc::tc_fence_after();
           const uint32_t kd = tc::sdesc_lo(sbase + Sh::kRing + st * Sh::kStage, 16);
           const uint32_t qd = tc::sdesc_lo(sbase + (item & 1) * Sh::kQ + s * 2 * NR * 128, 16);
-#pragma unroll
+#pragma unroll 2
           for (int ks = 0; ks < DB / 16; ++ks)
             tc::mma_f16(tb + (g & 1) * NR, kd + (ks >> 2) * 64 + (ks & 3) * 2, tc::sdesc_hi((DB / 64) * 1024),
                         qd + (ks >> 2) * NR * 8 + (ks & 3) * 2, tc::sdesc_hi(1024), ID_S, (s | ks) > 0);
@@ -202,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (first && item >= 2 && !wait(&o_free[item & 1], ((item - 2) >> 1) & 1)) break;
         tc::tc_fence_after();
         bool ok = true;
-#pragma unroll
+#pragma unroll 1
         for (int s = 0; s < KS; ++s) {
           const int use = load_of_v(g, N, KS) + s, st = use % NST;
           if (!(ok = wait(&full[st], (use / NST) & 1))) break;
@@ -210,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t vd = tc::sdesc_lo(sbase + Sh::kRing + st * Sh::kStage, 1024);
           const uint32_t pd = tc::sdesc_lo(sbase + 2 * Sh::kQ + (g & 1) * Sh::kP, 16);
           const uint32_t od = o_at(item, 0);
-#pragma unroll
+#pragma unroll 1
           for (int ks = 0; ks < Sh::VP / 16; ++ks) {
             const int kk = s * (Sh::VP / 16) + ks;
 #pragma unroll
@@ -233,63 +217,43 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 3) {
-    // ---- queries: rows behind the row tile's last are zero ----
-    for (int item = 0;; ++item) {
-      bool ok = true;
-      if (item >= 2) {
-        if (lane == 0) ok = wait(&q_empty[item & 1], ((item - 2) >> 1) & 1);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-      }
-      if (!ok) break;
-      const int t0 = w.rt * A.tp, rows = min(A.tp, w.s.n - t0) * A.G;
-      constexpr int CH = D / 8, RW = 32 / CH > 0 ? 32 / CH : 1;  // 16-byte chunks of a row; rows per warp instruction
-      const int sub = lane / (CH < 32 ? CH : 32), c = lane % CH;
-      const uint32_t qb = sbase + (item & 1) * Sh::kQ;
-      int r = sub, tt = r / A.G, gh = r - tt * A.G;
-#pragma unroll 4
-      for (; r < NR; r += RW) {
-        const uint32_t dst = qb + (c >> 3) * NR * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-        if (r < rows) {
-          cp_async16(dst, A.q + (int64_t)(w.s.lo + t0 + tt) * A.q_row + (int64_t)(w.h * A.G + gh) * A.q_head + c * 16);
-        } else {
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0) : "memory");
-        }
-        gh += RW;
-        while (gh >= A.G) gh -= A.G, ++tt;
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      tc::fence_async_smem();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&q_full[item & 1]);
-      if (!w.next(A)) break;
-    }
+    load_tiles<true, D, NST, Sh::kStage>(tmv, A, w, N, sm + Sh::kRing, full, empty, s_armed, wait);
   } else if (warp < 8) {
     // ---- softmax: thread = position of the tile ----
     const int quad = warp & 3, at = quad * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const float c = A.scale_log2;
+    // Rows in blocks of 4, and of those only the ones that the row tile has: with
+    // 4 rows of 16 the rest would be most of the instructions.
     float ref[NR], l[NR];  // log2 units; a row that has seen nothing yet refers to -1e30
-    int k = w.k0, item = 0;
+    int k = w.k0, item = 0, rows = 0;
+    auto each = [&](auto f) {
+#pragma unroll
+      for (int r0 = 0; r0 < NR; r0 += 4)
+        if (r0 < rows) {
+#pragma unroll
+          for (int r = r0; r < r0 + 4; ++r) f(r);
+        }
+    };
     auto enter = [&] {
+      rows = min(A.tp, w.s.n - w.rt * A.tp) * A.G;
 #pragma unroll
       for (int r = 0; r < NR; ++r) ref[r] = -1e30f, l[r] = 0.f;
     };
     enter();
+#pragma unroll 1
     for (int g = 0; g < N; ++g) {
       const int buf = g & 1, p0 = k * kTile;
-      const int t0 = w.rt * A.tp, lim0 = w.s.len - w.s.n + t0;  // the last position the first row sees
+      const int lim0 = w.s.len - w.s.n + w.rt * A.tp;  // the last position the first row sees
       wait_warp(&s_full[buf], (g >> 1) & 1);
       float s[NR];
-      tmem_load<NR>(tb + buf * NR + lane_off, s);
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(&s_free[buf]);
+      tc::tmem_ld16(tb + buf * NR + lane_off, s);
       if (p0 + kTile > w.s.len) {  // slots behind the sequence: their V rows become zero
         const int first = max(0, w.s.len - p0);
         // O^T of tile g - 1 is done, so every earlier load of V(g)'s stages is over:
         // their barriers are at most one phase behind and the parities are V(g)'s
         if (g > 0) wait_warp(&p_free[buf ^ 1], ((g - 1) >> 1) & 1);
-#pragma unroll
+#pragma unroll 1
         for (int st = 0; st < KS; ++st) {
           const int use = load_of_v(g, N, KS) + st;
           wait_warp(&full[use % NST], (use / NST) & 1);
@@ -297,19 +261,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc::fence_async_smem();
       }
-#pragma unroll
-      for (int r = 0; r < NR; ++r) s[r] *= c;
+      each([&](int r) { s[r] *= c; });
       if (p0 + kTile - 1 > lim0) {
         int lim = lim0 - (p0 + at), n = 0;  // >= 0: this position is seen by the row
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
+        each([&](int r) {
           s[r] = lim >= 0 ? s[r] : -INFINITY;
           if (++n == A.G) n = 0, ++lim;
-        }
+        });
       }
       bool over = false;
-#pragma unroll
-      for (int r = 0; r < NR; ++r) over |= s[r] - ref[r] > kLazy;
+      each([&](int r) { over |= s[r] - ref[r] > kLazy; });
       uint32_t any;
       asm volatile(
           "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
@@ -317,32 +278,32 @@ __global__ void __launch_bounds__(kThreads, 1)
           : "r"((uint32_t)over)
           : "memory");
       if (any) {  // some row's reference moves: the rows' maxima over the tile
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
+        each([&](int r) {
           float m = s[r];
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
           if (lane == 0) s_max[quad * NR + r] = m;
-        }
+        });
         asm volatile("bar.sync 1, 128;" ::: "memory");
         float corr[NR];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
+        for (int r = 0; r < NR; ++r) corr[r] = 1.0f;
+        each([&](int r) {
           const float m = fmaxf(fmaxf(s_max[r], s_max[NR + r]), fmaxf(s_max[2 * NR + r], s_max[3 * NR + r]));
           const bool move = m - ref[r] > kLazy;
           corr[r] = move ? ex2(ref[r] - m) : 1.0f;
           ref[r] = move ? m : ref[r];
           l[r] *= corr[r];
-        }
+        });
         if (k > w.k0) {
           wait_warp(&p_free[buf ^ 1], ((g - 1) >> 1) & 1);
 #pragma unroll 1
           for (int blk = 0; blk < NB; ++blk) {
             float o[NR];
-            tmem_load<NR>(o_at(item, blk) + lane_off, o);
+            tc::tmem_ld16(o_at(item, blk) + lane_off, o);
 #pragma unroll
             for (int r = 0; r < NR; ++r) o[r] *= corr[r];
-            tmem_store<NR>(o_at(item, blk) + lane_off, o);
+            tc::tmem_st16(o_at(item, blk) + lane_off, o);
           }
           tc::tmem_st_wait();
         }
@@ -351,15 +312,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (g >= 2) wait_warp(&p_free[buf], ((g - 2) >> 1) & 1);
       uint8_t* pw = sm + 2 * Sh::kQ + buf * Sh::kP + (at >> 6) * NR * 128 + (at & 7) * 2;
       const int ch = (at & 63) >> 3;
-#pragma unroll
-      for (int r = 0; r < NR; r += 2) {
-        const float a = ex2(s[r] - ref[r]), b = ex2(s[r + 1] - ref[r + 1]);
-        l[r] += a;
-        l[r + 1] += b;
-        const uint32_t u = Io<T>::down2(a, b);
-        *reinterpret_cast<uint16_t*>(pw + r * 128 + ((ch ^ (r & 7)) << 4)) = (uint16_t)u;
-        *reinterpret_cast<uint16_t*>(pw + (r + 1) * 128 + ((ch ^ ((r + 1) & 7)) << 4)) = (uint16_t)(u >> 16);
-      }
+      each([&](int r) {
+        const float x = ex2(s[r] - ref[r]);
+        l[r] += x;
+        *reinterpret_cast<T*>(pw + r * 128 + ((ch ^ (r & 7)) << 4)) = from_float<T>(x);
+      });
       tc::fence_async_smem();
       tc::tc_fence_before();
       __syncwarp();
@@ -368,10 +325,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
       // ---- the row tile's last KV tile here: sums over this warp's positions, row r's in lane r (and r + 16) ----
       if (item >= 2) wait_warp(&o_free[item & 1], ((item - 2) >> 1) & 1);
-      if constexpr (NR == 16) {
 #pragma unroll
-        for (int r = 0; r < NR; ++r) l[r] += __shfl_xor_sync(0xffffffffu, l[r], 16);
-      }
+      for (int r = 0; r < NR; ++r) l[r] += __shfl_xor_sync(0xffffffffu, l[r], 16);
 #pragma unroll
       for (int o = NR / 2; o > 0; o >>= 1) {
 #pragma unroll
@@ -395,9 +350,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    // ---- outputs: thread = dim ----
+    // ---- queries, two row tiles ahead; outputs: thread = dim ----
     const int quad = warp & 3, dim = quad * 32 + lane, heads = A.kv_heads * A.G;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
+    Walk ahead = w;
+    bool more = true;
+    auto load_q = [&](int item) {  // rows behind the row tile's last only reach results nobody looks at
+      const int t0 = ahead.rt * A.tp, rows = min(A.tp, ahead.s.n - t0) * A.G;
+      constexpr int CH = D / 8, RW = 128 / CH;  // 16-byte chunks of a row; rows per pass of the 128 threads
+      const int c = dim % CH;
+      const uint32_t qb = sbase + (item & 1) * Sh::kQ;
+      int r = dim / CH, tt = r / A.G, gh = r - tt * A.G;
+#pragma unroll 1
+      for (; r < rows; r += RW) {
+        const uint32_t dst = qb + (c >> 3) * NR * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+        cp_async16(dst, A.q + (int64_t)(ahead.s.lo + t0 + tt) * A.q_row + (int64_t)(ahead.h * A.G + gh) * A.q_head + c * 16);
+        gh += RW;
+        while (gh >= A.G) gh -= A.G, ++tt;
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      tc::fence_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&q_full[item & 1]);
+      more = ahead.next(A);
+    };
+    load_q(0);
+    if (more) load_q(1);
     if (tid == 256) meta[cta].slot = -1, meta[cta].units = N;
     for (int item = 0;; ++item) {
       const int t0 = w.rt * A.tp, rows = min(A.tp, w.s.n - t0) * A.G, row0 = w.s.lo + t0;
@@ -432,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         float o[NR];
-        tmem_load<NR>(o_at(item, blk) + lane_off, o);
+        tc::tmem_ld16(o_at(item, blk) + lane_off, o);
         T* op = reinterpret_cast<T*>(A.out) + ((int64_t)row0 * heads + w.h * A.G) * D + blk * 128 + dim;
         float* pp = part + blk * 128 + dim;
         int n = 0;
@@ -460,6 +438,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&o_free[item & 1]);
+      if (more) {
+        wait_warp(&q_empty[item & 1], (item >> 1) & 1);
+        load_q(item + 2);
+      }
       if (!w.next(A)) break;
     }
   }
@@ -470,11 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // let the copies and MMAs in flight land before shared memory and TMEM go
     if (tid == 0) {
       atomicExch(A.err, 5);
-      for (int st = 0; st < NST; ++st)
-        if (*s_issued > st) {
-          const int last = (*s_issued - 1 - st) / NST;
-          tc::mbar_wait_bounded(&full[st], last & 1, kWait);
-        }
+      drain_ring(full, s_armed, NST);
     }
     if (tid == 32 || tid == 64) {
       tc::mma_commit(drain);
@@ -488,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <typename T, int D, int NR>
+template <typename T, int D>
 Status launch(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& A, int sms, cudaStream_t st) {
   // the attribute belongs to the kernel on the current device: set once on each
   static std::atomic<uint64_t> done{0};
@@ -497,30 +475,27 @@ Status launch(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& A, i
   if (e != cudaSuccess) return cuda_status(e, "spock_paged_attention");
   const uint64_t bit = 1ull << (dev & 63);
   if (!(done.load() & bit)) {
-    e = cudaFuncSetAttribute(paged_few_kernel<T, D, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<D, NR>::kSmem);
+    e = cudaFuncSetAttribute(paged_few_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<D>::kSmem);
     if (e != cudaSuccess) return cuda_status(e, "paged_few_kernel attribute");
     done.fetch_or(bit);
   }
-  e = launch_k(paged_few_kernel<T, D, NR>, dim3(sms), dim3(kThreads), Few<D, NR>::kSmem, st, mk, mv, A);
+  e = launch_k(paged_few_kernel<T, D>, dim3(sms), dim3(kThreads), Few<D>::kSmem, st, mk, mv, A);
   if (e != cudaSuccess) return cuda_status(e, "paged_few_kernel");
   SPOCK_LAUNCH_CHECK("paged_few_kernel");
   return Status::ok();
 }
 
 template <typename T>
-Status by_size(int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& A, int rows, int sms,
-               cudaStream_t st) {
-  if (head_dim == 128)
-    return rows == 16 ? launch<T, 128, 16>(mk, mv, A, sms, st) : launch<T, 128, 32>(mk, mv, A, sms, st);
-  return rows == 16 ? launch<T, 256, 16>(mk, mv, A, sms, st) : launch<T, 256, 32>(mk, mv, A, sms, st);
+Status by_size(int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& A, int sms, cudaStream_t st) {
+  return head_dim == 128 ? launch<T, 128>(mk, mv, A, sms, st) : launch<T, 256>(mk, mv, A, sms, st);
 }
 
 }  // namespace
 
 Status launch_paged_few(int dtype, int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const paged::AttnArgs& A,
-                        int rows, int sms, cudaStream_t st) {
-  if (dtype == SPOCK_F16) return by_size<__half>(head_dim, mk, mv, A, rows, sms, st);
-  return by_size<__nv_bfloat16>(head_dim, mk, mv, A, rows, sms, st);
+                        int sms, cudaStream_t st) {
+  if (dtype == SPOCK_F16) return by_size<__half>(head_dim, mk, mv, A, sms, st);
+  return by_size<__nv_bfloat16>(head_dim, mk, mv, A, sms, st);
 }
 
 }  // namespace spock

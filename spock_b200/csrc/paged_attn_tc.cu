@@ -7,10 +7,10 @@
 // paged_attn_kernel: one CTA per SM walks its share of the batch
 // (paged_sched.cuh): row tiles of up to 128 (token, query head) rows of one
 // sequence and kv head, times KV tiles of 128 positions. Warp roles:
-//   warp 0      K and V tiles by TMA from the pages into a ring of stages
+//   warps 0, 2  K tiles and V tiles by TMA from the pages into a ring of stages
 //   warp 1      issues the MMAs: S = Q K^T (M128 N128 K=D) into one of two TMEM
 //               buffers, O += P V (M128 N=D K128) with P read from TMEM
-//   warps 2-3   the next row tile's queries, into shared memory
+//   warp 3      the next row tile's queries, into shared memory
 //   warps 4-11  softmax, two threads per row (64 of a tile's positions each), and
 //               the output of finished row tiles
 // S(i+1) is issued before O += P(i) V(i), so the tensor pipe has work while the
@@ -36,7 +36,7 @@
 
 namespace spock {
 Status launch_paged_few(int dtype, int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const paged::AttnArgs& A,
-                        int rows, int sms, cudaStream_t st);
+                        int sms, cudaStream_t st);
 
 namespace {
 
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(q_full + 9) + 1;
   int64_t* s_scan = reinterpret_cast<int64_t*>(sm + Sh::kBar + 256);  // [warps + 2]
   int* s_first = reinterpret_cast<int*>(s_scan + kThreads / 32 + 2);  // [4]
-  volatile int* s_issued = s_first + 4;
+  volatile int* s_armed = s_first + 4;  // [NST]
   float* red = reinterpret_cast<float*>(sm + Sh::kRed);  // [2 tiles][2 halves][128] maxima (and sums)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x, ctas = gridDim.x;
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::mbar_init(&full[i], 1);
       tc::mbar_init(&empty[i], 1);
     }
-    tc::mbar_init(q_full, 2);
+    tc::mbar_init(q_full, 1);
     tc::mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&s_full[i], 1);
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc::mbar_init(drain, 1);
     *s_fail = 0;
-    *s_issued = 0;
+    for (int i = 0; i < NST; ++i) s_armed[i] = 0;
     tc::fence_mbar_init();
     tc::prefetch_tmap(&tmk);
     tc::prefetch_tmap(&tmv);
@@ -130,7 +130,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (N == 0) {
     if (tid == 0) meta[cta].slot = -1, meta[cta].units = 0;
   } else if (warp == 0) {
-    load_tiles<D, NST, Sh::kStage>(tmk, tmv, A, w, N, sm + Sh::kQ, full, empty, s_issued, wait);
+    load_tiles<false, D, NST, Sh::kStage>(tmk, A, w, N, sm + Sh::kQ, full, empty, s_armed, wait);
+  } else if (warp == 2) {
+    load_tiles<true, D, NST, Sh::kStage>(tmv, A, w, N, sm + Sh::kQ, full, empty, s_armed, wait);
   } else if (warp == 1) {
     // ---- MMAs ----
     if (lane == 0) {
@@ -196,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp < 4) {
+  } else if (warp == 3) {
     // ---- queries ----
     for (int item = 0;; ++item) {
       bool ok = true;
@@ -208,13 +210,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int t0 = w.rt * A.tp, rows = min(A.tp, w.s.n - t0) * A.G;
       constexpr int CH = D / 8;                   // 16-byte chunks of a row
       constexpr int RW = CH >= 32 ? 1 : 32 / CH;  // rows per warp instruction
-      constexpr int step = 2 * RW;
       const int sub = CH >= 32 ? 0 : lane / CH, c = CH >= 32 ? lane : lane % CH;
-      int r = (warp - 2) * RW + sub, tt = r / A.G, gh = r - tt * A.G;
-      for (; r < rows; r += step) {
+      int r = sub, tt = r / A.G, gh = r - tt * A.G;
+#pragma unroll 4
+      for (; r < rows; r += RW) {
         const uint8_t* src = A.q + (int64_t)(w.s.lo + t0 + tt) * A.q_row + (int64_t)(w.h * A.G + gh) * A.q_head + c * 16;
         cp_async16(sbase + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4), src);
-        gh += step;
+        gh += RW;
         while (gh >= A.G) gh -= A.G, ++tt;
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
@@ -404,11 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // let the copies and MMAs in flight land before shared memory and TMEM go
     if (tid == 0) {
       atomicExch(A.err, 5);
-      for (int st = 0; st < NST; ++st)
-        if (*s_issued > st) {
-          const int last = (*s_issued - 1 - st) / NST;
-          tc::mbar_wait_bounded(&full[st], last & 1, kWait);
-        }
+      drain_ring(full, s_armed, NST);
     }
     if (tid == 32) {
       tc::mma_commit(drain);
@@ -438,8 +436,24 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   const Meta mt = meta[cta];
   if (mt.slot < 0) return;
   const float* parts = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(A.ws) + meta_bytes(ctas));
-  int n = 1;  // parts
-  for (int have = mt.have; have < mt.nt && cta + n < ctas; ++n) have += meta[cta + n].units;
+  // the shares that hold parts: 32 at a time, until their units cover the row tile
+  int n = 1;
+  for (int have = mt.have; have < mt.nt && cta + n < ctas;) {
+    int u = cta + n + lane < ctas ? meta[cta + n + lane].units : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, u, o);
+      if (lane >= o) u += y;
+    }
+    const unsigned enough = __ballot_sync(0xffffffffu, have + u >= mt.nt);
+    if (enough) {
+      n += __ffs(enough);
+      break;
+    }
+    have += __shfl_sync(0xffffffffu, u, 31);
+    n += 32;
+  }
+  n = min(n, ctas - cta);
   auto part = [&](int i) {
     return parts + ((size_t)(cta + i) * 2 + (i == 0 ? mt.slot : 0)) * part_floats<D>();
   };
@@ -461,17 +475,33 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     }
     store_words(A.out + (tok * (A.kv_heads * A.G) + hq) * (D * 2) + lane * V * 2, w);
   };
-  auto add = [&](int i, int r, float m, float (&acc)[V], float& l) {
-    const float* p = part(i);
-    const float mi = p[128 * D + r];
-    const float f = mi == -INFINITY ? 0.f : ex2(mi - m);
-    if (f == 0.f) return;  // a part that saw nothing (or nothing that counts) may hold anything
-    l += f * p[128 * D + 128 + r];
+  // parts i0, i0 + step, .. < n of row r, relative to maximum m; four in flight
+  auto add = [&](int i0, int step, int r, float m, float (&acc)[V], float& l) {
+    constexpr int U = 4;
+    for (int i = i0; i < n; i += U * step) {
+      float f[U], x[U][V];
 #pragma unroll
-    for (int v = 0; v < V; v += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(p + r * D + lane * V + v);
-      acc[v] = fmaf(f, x.x, acc[v]);
-      acc[v + 1] = fmaf(f, x.y, acc[v + 1]);
+      for (int u = 0; u < U; ++u) {
+        const int j = i + u * step;
+        f[u] = 0.f;
+        if (j < n) {
+          const float* p = part(j);
+          const float mi = p[128 * D + r];
+          f[u] = mi == -INFINITY ? 0.f : ex2(mi - m);
+          l += f[u] * p[128 * D + 128 + r];
+#pragma unroll
+          for (int v = 0; v < V; v += 2) {
+            const float2 y = *reinterpret_cast<const float2*>(p + r * D + lane * V + v);
+            x[u][v] = y.x, x[u][v + 1] = y.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (f[u] != 0.f) {  // a part that saw nothing (or nothing that counts) may hold anything
+#pragma unroll
+          for (int v = 0; v < V; ++v) acc[v] = fmaf(f[u], x[u][v], acc[v]);
+        }
     }
   };
   const bool many = n > kMany;
@@ -482,11 +512,11 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float acc[V] = {}, l = 0.f;
     if (!many) {
-      for (int i = 0; i < n; ++i) add(i, r, m, acc, l);
+      add(0, 1, r, m, acc, l);
       finish(r, acc, l);
       continue;
     }
-    for (int i = warp; i < n; i += 8) add(i, r, m, acc, l);
+    add(warp, 8, r, m, acc, l);
     __syncthreads();
 #pragma unroll
     for (int v = 0; v < V; ++v) s_o[warp][lane * V + v] = acc[v];
@@ -541,10 +571,11 @@ CUresult encode_pages(EncodeFn fn, CUtensorMap* map, const spock_paged_kv& kv, v
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 template <typename T, int D>
-Status launch(const spock_paged_kv& kv, AttnArgs& A, int few, int sms, cudaStream_t st) {
+Status launch(const spock_paged_kv& kv, AttnArgs& A, bool few, int sms, cudaStream_t st) {
   EncodeFn fn = encode();
   if (!fn) return Status::err(SPOCK_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  A.tp = (few ? few : 128) / A.G;
+  A.tp = (few ? kFewRows : 128) / A.G;
+  A.whole = !few;
   A.piece_k = gcd(kv.page_size, kTile);
   A.piece_v = gcd(kv.page_size, Shape<D>::VP);
   CUtensorMap mk, mv;
@@ -553,7 +584,7 @@ Status launch(const spock_paged_kv& kv, AttnArgs& A, int few, int sms, cudaStrea
     return Status::err(SPOCK_ERR_CUDA, "spock_paged_attention: tensor map encoding failed");
   cudaError_t e;
   if (few) {
-    const Status s = launch_paged_few(kv.dtype, D, mk, mv, A, few, sms, st);
+    const Status s = launch_paged_few(kv.dtype, D, mk, mv, A, sms, st);
     if (s.code) return s;
   } else {
     // the attribute belongs to the kernel on the current device: set once on each
@@ -611,17 +642,12 @@ Status launch_paged_attention(const spock_paged_kv& kv, int batch, const int32_t
   A.scale_log2 = scale * 1.44269504088896341f;
   A.ws = (float*)ws;
   A.err = err;
-  // Either kernel is right for every batch; the rows a sequence brings on average
-  // decide. A row tile of 32 rows costs half of one of 128 (all of the cache's
-  // side, little of the rows'), so a few long chunks among many decode tokens lose
-  // less than the decode tokens gain.
-  int few = 0;
-  if (kv.head_dim >= 128) {
-    if (total <= batch && A.G <= 16)
-      few = 16;
-    else if (total * A.G <= 32 * (int64_t)batch && A.G <= 32)
-      few = 32;
-  }
+  // Either kernel is right for every batch; the rows that a sequence brings on
+  // average decide. One token each over 256 sequences takes 102 us in the few-row
+  // kernel and 117 in the wide one; five tokens each (64 sequences) 92 in the wide
+  // one, and 113 in a few-row kernel of 32 rows, which is not kept. Head size 64
+  // would leave half of the few-row kernel's output tile empty.
+  const bool few = kv.head_dim >= 128 && total <= batch && A.G <= kFewRows;
   if (kv.dtype == SPOCK_F16) {
     if (kv.head_dim == 64) return launch<__half, 64>(kv, A, few, sms, st);
     if (kv.head_dim == 128) return launch<__half, 128>(kv, A, few, sms, st);

@@ -65,6 +65,7 @@ __host__ __device__ inline int64_t head_units(int n, int len, int tp) {
 // the row tile that unit r of a head falls into (r becomes the unit within it)
 __host__ __device__ inline int find_row_tile(int n, int len, int tp, int64_t& r) {
   int lo = 0, hi = (n + tp - 1) / tp - 1;
+  if (hi == 0) return 0;
   while (lo < hi) {
     const int mid = lo + (hi - lo + 1) / 2;
     if (units_before(n, len, tp, mid) <= r)
@@ -76,7 +77,10 @@ __host__ __device__ inline int find_row_tile(int n, int len, int tp, int64_t& r)
   return lo;
 }
 
-__host__ __device__ inline int64_t share_begin(int64_t units, int c, int shares) { return units * c / shares; }
+__host__ __device__ inline int64_t share_begin(int64_t units, int c, int shares) {
+  if (units < (1 << 20) && shares <= 1024) return (uint32_t)units * (uint32_t)c / (uint32_t)shares;  // fits 32 bits
+  return units * c / shares;
+}
 
 }  // namespace sched
 }  // namespace spock
