@@ -21,7 +21,7 @@ constexpr float kLazy = 8.0f;  // log2 of how far weights may exceed 1
 struct AttnArgs {
   const int32_t *start, *table, *kv_len;
   int64_t table_stride;
-  int batch, total, table_width, num_pages, page_size, kv_heads, G, tp, piece_k, piece_v, whole;
+  int batch, total, table_width, num_pages, page_size, kv_heads, G, tp, piece_k, piece_v, whole, extra;
   int64_t head_blk;  // 64-element blocks from one kv head to the next
   const uint8_t *q, *gate;
   int64_t q_row, q_head, g_row, g_head;  // bytes
@@ -136,71 +136,88 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 
 
 // This CTA's share: the first row tile and KV tile in w; the KV tiles it has. All
-// threads (it synchronises). scan: kThreads / 32 + 2 words, first: 4.
+// threads (it synchronises). scan: 2 kThreads / 32 + 4 words, first: 4.
 //
-// Prefix sums of the sequences' units over the block, then the borders. Where a
-// part is dear (A.whole: 128 rows of it make a round trip through the workspace)
-// a border inside a row tile of at most half a share moves to the row tile's
-// nearer end: shares grow or shrink by a quarter at most, and short row tiles are
-// not cut. Parts of few rows are cheap, and equal shares worth more (256 decode
-// tokens: 18 KV tiles a CTA, 24 at most with moved borders).
+// Prefix sums of the sequences' KV tiles and row tiles over the block, then the
+// borders. Where a part is dear (A.whole: 128 rows of it make a round trip through
+// the workspace) a border inside a row tile of at most half a share moves to the
+// row tile's nearer end: shares grow or shrink by a quarter at most, and short row
+// tiles are not cut. Parts of few rows are cheap, and equal shares worth more (256
+// decode tokens: 18 KV tiles a CTA, 24 at most with moved borders).
+//
+// A share holds a KV tile at least: without `extra` as there are no more shares
+// than units, and with it as a share is 2 (extra + 1) units or more (otherwise it
+// does not count: few tiles are spread as far as they go), half of which the
+// moved borders leave.
 static __device__ __noinline__ int enter_share(const AttnArgs& A, int64_t* scan, int* first, Walk& w) {
+  constexpr int W = kThreads / 32;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x, ctas = gridDim.x;
   const int per = (A.batch + kThreads - 1) / kThreads;
-  int64_t mine = 0;
+  int64_t mine = 0, rts = 0;  // KV tiles, row tiles
   for (int b = tid * per; b < min(A.batch, (tid + 1) * per); ++b) {
     const Seq s = load_seq(A, b, cta == 0);
     mine += sched::head_units(s.n, s.len, A.tp) * A.kv_heads;
+    rts += (int64_t)sched::row_tiles(s.n, A.tp) * A.kv_heads;
   }
-  int64_t incl = mine;
+  int64_t incl = mine, rincl = rts;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
+    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o), z = __shfl_up_sync(0xffffffffu, rincl, o);
+    if (lane >= o) incl += y, rincl += z;
   }
-  if (lane == 31) scan[warp] = incl;
+  if (lane == 31) scan[warp] = incl, scan[W + warp] = rincl;
   __syncthreads();
-  int64_t base = 0, units = 0;
+  int64_t base = 0, units = 0, rbase = 0, rall = 0;
 #pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) {
-    if (i < warp) base += scan[i];
+  for (int i = 0; i < W; ++i) {
+    if (i < warp) base += scan[i], rbase += scan[W + i];
     units += scan[i];
+    rall += scan[W + i];
   }
-  const int64_t from = base + incl - mine;
-  const int shares = units < ctas ? (int)units : ctas;  // none of them empty
+  const int64_t all = units;  // KV tiles
+  int extra = A.extra;
+  if (units + extra * rall < (int64_t)ctas * 2 * (extra + 1)) extra = 0;
+  units += extra * rall;
+  mine += extra * rts;
+  const int64_t rfrom = rbase + rincl - rts, from = base + incl + extra * (rbase + rincl) - mine;
+  const int shares = units < ctas ? (int)units : ctas;
   if (cta >= shares) return 0;
-  int64_t* border = scan + kThreads / 32;
-  if (tid < 2) border[tid] = sched::share_begin(units, cta + tid, shares);
+  int64_t* border = scan + 2 * W;  // [2], then the KV tiles before them [2]
+  if (tid < 2) {
+    border[tid] = sched::share_begin(units, cta + tid, shares);
+    border[2 + tid] = all;  // of a border behind the last unit
+  }
   __syncthreads();
-  // 0, 1: move the borders (where parts are dear); 2: the first row tile
+  // 0, 1: move the borders; 2: the first row tile
 #pragma unroll 1
-  for (int i = A.whole ? 0 : 2; i < 3; ++i) {
-    const int64_t u = border[i < 2 ? i : 0];
+  for (int i = A.whole ? 0 : 1; i < 3; ++i) {
+    const int64_t u = border[i & 1];
     if (A.whole) __syncthreads();  // all have read it before its finder moves it
-    if (from <= u && u < from + mine && (i == 2 || u > 0)) {
-      int64_t r = u - from;
+    if (from <= u && u < from + mine) {
+      int64_t r = u - from, rt_before = rfrom;
       int b = tid * per, h = 0;
       Seq s;
 #pragma unroll 1
       for (;; ++b) {
         s = load_seq(A, b, false);
-        const int64_t hu = sched::head_units(s.n, s.len, A.tp);
+        const int64_t tiles = sched::row_tiles(s.n, A.tp), hu = sched::head_units(s.n, s.len, A.tp) + extra * tiles;
 #pragma unroll 1
-        for (h = 0; h < A.kv_heads && r >= hu; ++h) r -= hu;
+        for (h = 0; h < A.kv_heads && r >= hu; ++h) r -= hu, rt_before += tiles;
         if (h < A.kv_heads) break;
       }
-      const int rt = sched::find_row_tile(s.n, s.len, A.tp, r), k = (int)r;
-      if (i == 2) {
-        first[0] = b, first[1] = h, first[2] = rt, first[3] = k;
-      } else {
-        const int nt = sched::row_tile_units(s.n, s.len, A.tp, rt);
-        if (2 * nt <= units / shares) border[i] = 2 * k <= nt ? u - k : u - k + nt;
-      }
+      const int rt = sched::find_row_tile(s.n, s.len, A.tp, extra, r);
+      const int nt = sched::row_tile_units(s.n, s.len, A.tp, rt), all_of = nt + extra;
+      rt_before += rt;
+      int64_t at = r;  // of the row tile's units
+      if (A.whole && u > 0 && 2 * all_of <= units / shares) at = 2 * r <= all_of ? 0 : all_of;
+      const int k = max((int)at - extra, 0);
+      if (i == 2) first[0] = b, first[1] = h, first[2] = rt, first[3] = k;
+      border[i & 1] = u - r + at;
+      border[2 + (i & 1)] = u - r - extra * rt_before + k;
     }
     __syncthreads();
   }
-  const int64_t u0 = border[0], u1 = border[1];
-  const int n = (int)(u1 - u0);
+  const int n = (int)(border[3] - border[2]);
   w.left = n;
   if (n > 0) {
     w.b = first[0];

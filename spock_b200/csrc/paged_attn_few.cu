@@ -44,7 +44,7 @@ struct Few {
   static constexpr int NST = D == 256 ? 5 : 6;
   static constexpr int kRing = 2 * kQ + 2 * kP;
   static constexpr int kBar = kRing + NST * kStage;
-  static constexpr int kStat = kBar + 512;    // [2 row tiles][4 warps][NR] sums, [2][NR] references
+  static constexpr int kStat = kBar + 576;    // [2 row tiles][4 warps][NR] sums, [2][NR] references
   static constexpr int kMax = kStat + 2 * 5 * NR * 4;  // [4 warps][NR] maxima
   static constexpr int kSmem = kMax + 4 * NR * 4;
   static constexpr int kBlocks = D / 128;     // M blocks of O^T
@@ -75,8 +75,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* drain = q_full + 16;
   volatile int* s_fail = reinterpret_cast<volatile int*>(q_full + 17);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(q_full + 17) + 1;
-  int64_t* s_scan = reinterpret_cast<int64_t*>(sm + Sh::kBar + 264);  // [warps + 2]
-  int* s_first = reinterpret_cast<int*>(s_scan + kThreads / 32 + 2);  // [4]
+  int64_t* s_scan = reinterpret_cast<int64_t*>(sm + Sh::kBar + 264);  // [2 warps + 4]
+  int* s_first = reinterpret_cast<int*>(s_scan + 2 * (kThreads / 32) + 4);  // [4]
   volatile int* s_armed = s_first + 4;  // [NST]
   static_assert((2 * NST + 20) * 8 <= 264 && 264 + (kThreads / 32 + 2) * 8 + (4 + NST) * 4 <= 512, "barrier area");
   float* s_sum = reinterpret_cast<float*>(sm + Sh::kStat);

@@ -53,7 +53,7 @@ struct Shape {
   static constexpr int kQ = 128 * D * 2;
   static constexpr int NST = D == 256 ? 5 : D == 128 ? 6 : 8;
   static constexpr int kBar = kQ + NST * kStage;
-  static constexpr int kRed = kBar + 512;
+  static constexpr int kRed = kBar + 576;
   static constexpr int kSmem = kRed + 4 * 128 * 4;
 };
 static_assert(Shape<256>::kSmem <= 227 * 1024 && Shape<128>::kSmem <= 227 * 1024, "shared memory of one SM");
@@ -78,8 +78,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* drain = q_full + 8;
   volatile int* s_fail = reinterpret_cast<volatile int*>(q_full + 9);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(q_full + 9) + 1;
-  int64_t* s_scan = reinterpret_cast<int64_t*>(sm + Sh::kBar + 256);  // [warps + 2]
-  int* s_first = reinterpret_cast<int*>(s_scan + kThreads / 32 + 2);  // [4]
+  int64_t* s_scan = reinterpret_cast<int64_t*>(sm + Sh::kBar + 256);  // [2 warps + 4]
+  int* s_first = reinterpret_cast<int*>(s_scan + 2 * (kThreads / 32) + 4);  // [4]
   volatile int* s_armed = s_first + 4;  // [NST]
   float* red = reinterpret_cast<float*>(sm + Sh::kRed);  // [2 tiles][2 halves][128] maxima (and sums)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -135,66 +135,62 @@ __global__ void __launch_bounds__(kThreads, 1)
     load_tiles<true, D, NST, Sh::kStage>(tmv, A, w, N, sm + Sh::kQ, full, empty, s_armed, wait);
   } else if (warp == 1) {
     // ---- MMAs ----
-    if (lane == 0) {
+    if (tc::elect_one()) {
       constexpr uint32_t ID_S = tc::idesc_f16(128, kTile, false, false, kBf16);
       constexpr uint32_t ID_O = tc::idesc_f16(128, D, false, true, kBf16);
       constexpr uint32_t kGroup = (D / 64) * 1024;  // bytes from one 8-position group of a V stage to the next
-      int item = 0, k = w.k0;
-      auto issue_s = [&](int g) -> bool {
-        if (k == w.k0 && !wait(q_full, item & 1)) return false;
+      int item = 0, k = w.k0, gs = 0, go = 0;  // the next S and O
+      bool fresh = true;    // S(gs) is its row tile's first
+      uint32_t starts = 0;  // bit g & 1: O(g) starts from zero
+      while (go < N) {
+        // S(g + 1) goes before O(g), unless it waits for the next row tile's queries
+        if (gs < N && (gs == go || (gs == go + 1 && !fresh))) {
+          const int g = gs++;
+          if (fresh && !wait(q_full, item & 1)) break;
+          starts = (starts & ~(1u << (g & 1))) | (uint32_t)fresh << (g & 1);
+          bool ok = true;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const int use = load_of_k(g, KS) + s, st = use % NST;
-          if (!wait(&full[st], (use / NST) & 1)) return false;
-          tc::tc_fence_after();
-          const uint32_t kd = tc::sdesc_lo(sbase + Sh::kQ + st * Sh::kStage, 16);
-          const uint32_t qd = tc::sdesc_lo(sbase + s * (DB / 64) * 16384, 16);
+          for (int s = 0; s < KS; ++s) {
+            const int use = load_of_k(g, KS) + s, st = use % NST;
+            if (!(ok = wait(&full[st], (use / NST) & 1))) break;
+            tc::tc_fence_after();
+            const uint32_t kd = tc::sdesc_lo(sbase + Sh::kQ + st * Sh::kStage, 16);
+            const uint32_t qd = tc::sdesc_lo(sbase + s * (DB / 64) * 16384, 16);
 #pragma unroll
-          for (int ks = 0; ks < DB / 16; ++ks)
-            tc::mma_f16(tb + (g & 1) * kTile, qd + (ks >> 2) * 1024 + (ks & 3) * 2, tc::sdesc_hi(1024),
-                        kd + (ks >> 2) * 64 + (ks & 3) * 2, tc::sdesc_hi((DB / 64) * 1024), ID_S, (s | ks) > 0);
-          tc::mma_commit(&empty[st]);
-        }
-        tc::mma_commit(&s_full[g & 1]);
-        if (k + 1 == w.k1) tc::mma_commit(q_empty);
-        return true;
-      };
-      auto issue_o = [&](int g, bool first) -> bool {  // first: O starts from zero
-        if (!wait(&p_full[g & 1], (g >> 1) & 1)) return false;
-        tc::tc_fence_after();
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const int use = load_of_v(g, N, KS) + s, st = use % NST;
-          if (!wait(&full[st], (use / NST) & 1)) return false;
-          tc::tc_fence_after();
-          const uint32_t vd = tc::sdesc_lo(sbase + Sh::kQ + st * Sh::kStage, 1024);
-#pragma unroll
-          for (int ks = 0; ks < Sh::VP / 16; ++ks)
-            tc::mma_f16_ta(tO, tb + (g & 1) * kTile + (s * (Sh::VP / 16) + ks) * 8, vd + ks * 2 * kGroup / 16,
-                           tc::sdesc_hi(kGroup), ID_O, (s | ks) > 0 || !first);
-          tc::mma_commit(&empty[st]);
-        }
-        tc::mma_commit(&o_done[g & 1]);
-        return true;
-      };
-      bool ok = issue_s(0), first = true;
-      for (int g = 0; g < N && ok; ++g) {
-        bool next_first = false;
-        if (g + 1 < N) {
-          if (++k == w.k1) {  // the next row tile's queries may be on their way: this one's O goes first
-            ok = issue_o(g, first);
+            for (int ks = 0; ks < DB / 16; ++ks)
+              tc::mma_f16(tb + (g & 1) * kTile, qd + (ks >> 2) * 1024 + (ks & 3) * 2, tc::sdesc_hi(1024),
+                          kd + (ks >> 2) * 64 + (ks & 3) * 2, tc::sdesc_hi((DB / 64) * 1024), ID_S, (s | ks) > 0);
+            tc::mma_commit(&empty[st]);
+          }
+          if (!ok) break;
+          tc::mma_commit(&s_full[g & 1]);
+          fresh = ++k == w.k1;
+          if (fresh) {
+            tc::mma_commit(q_empty);
             w.next(A);
             k = w.k0;
             ++item;
-            next_first = true;
-            ok = ok && issue_s(g + 1);
-          } else {
-            ok = issue_s(g + 1) && issue_o(g, first);
           }
         } else {
-          ok = issue_o(g, first);
+          const int g = go++;
+          const bool first = starts >> (g & 1) & 1;
+          if (!wait(&p_full[g & 1], (g >> 1) & 1)) break;
+          bool ok = true;
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            const int use = load_of_v(g, N, KS) + s, st = use % NST;
+            if (!(ok = wait(&full[st], (use / NST) & 1))) break;
+            tc::tc_fence_after();
+            const uint32_t vd = tc::sdesc_lo(sbase + Sh::kQ + st * Sh::kStage, 1024);
+#pragma unroll
+            for (int ks = 0; ks < Sh::VP / 16; ++ks)
+              tc::mma_f16_ta(tO, tb + (g & 1) * kTile + (s * (Sh::VP / 16) + ks) * 8, vd + ks * 2 * kGroup / 16,
+                             tc::sdesc_hi(kGroup), ID_O, (s | ks) > 0 || !first);
+            tc::mma_commit(&empty[st]);
+          }
+          if (!ok) break;
+          tc::mma_commit(&o_done[g & 1]);
         }
-        first = next_first;
       }
     }
     __syncwarp();
@@ -576,6 +572,7 @@ Status launch(const spock_paged_kv& kv, AttnArgs& A, bool few, int sms, cudaStre
   if (!fn) return Status::err(SPOCK_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   A.tp = (few ? kFewRows : 128) / A.G;
   A.whole = !few;
+  A.extra = 3;
   A.piece_k = gcd(kv.page_size, kTile);
   A.piece_v = gcd(kv.page_size, Shape<D>::VP);
   CUtensorMap mk, mv;

@@ -4,10 +4,10 @@
 // kv head (tp = R / G, at most R = 128 rows, or 16 or 32 in the kernel for few
 // rows); its work is the KV tiles of kTile
 // positions that its last token sees, at least one (a row tile that sees
-// nothing still has zeros to write). All row tiles' KV tiles, in the order
-// sequence, kv head, row tile, KV tile, form one line of units; share c of C
-// is units [U c / C, U (c + 1) / C), its borders moved off short row tiles. A row
-// tile cut by a border is computed in parts and joined afterwards, so one long
+// nothing still has zeros to write). Starting and finishing a row tile takes as
+// long as `extra` KV tiles. All row tiles' units (extra, then KV tiles), in the
+// order sequence, kv head, row tile, form one line; share c of C is units
+// [U c / C, U (c + 1) / C), its borders moved off short row tiles. A row tile cut by a border is computed in parts and joined afterwards, so one long
 // sequence, many short ones and any mix all keep every SM busy without the host
 // knowing any length.
 #pragma once
@@ -62,18 +62,20 @@ __host__ __device__ inline int64_t head_units(int n, int len, int tp) {
   if (last == 0) return row_tile_units(n, len, tp, 0);
   return units_before(n, len, tp, last) + row_tile_units(n, len, tp, last);
 }
-// the row tile that unit r of a head falls into (r becomes the unit within it)
-__host__ __device__ inline int find_row_tile(int n, int len, int tp, int64_t& r) {
-  int lo = 0, hi = (n + tp - 1) / tp - 1;
+__host__ __device__ inline int row_tiles(int n, int tp) { return n <= 0 ? 0 : (n + tp - 1) / tp; }
+// the row tile that unit r of a head falls into (r becomes the unit within it),
+// each with `extra` units before its KV tiles
+__host__ __device__ inline int find_row_tile(int n, int len, int tp, int extra, int64_t& r) {
+  int lo = 0, hi = row_tiles(n, tp) - 1;
   if (hi == 0) return 0;
   while (lo < hi) {
     const int mid = lo + (hi - lo + 1) / 2;
-    if (units_before(n, len, tp, mid) <= r)
+    if (units_before(n, len, tp, mid) + (int64_t)extra * mid <= r)
       lo = mid;
     else
       hi = mid - 1;
   }
-  r -= units_before(n, len, tp, lo);
+  r -= units_before(n, len, tp, lo) + (int64_t)extra * lo;
   return lo;
 }
 

@@ -304,5 +304,14 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
       : "memory");
 }
 
+// One lane of a converged warp, always the same. The compiler knows that a branch
+// on this has one lane active, and `if (lane == 0)` not: there each MMA's descriptors
+// go through a loop over the lanes' values.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}" : "=r"(e));
+  return e != 0;
+}
+
 }  // namespace tc
 }  // namespace spock
