@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     load_tiles<false, D, NST, Sh::kStage>(tmk, A, w, N, sm + Sh::kRing, full, empty, s_armed, wait);
   } else if (warp == 1) {
     // ---- S^T = K Q^T ----
-    if (lane == 0) {
+    if (tc::elect_one()) {
       constexpr uint32_t ID_S = tc::idesc_f16(128, NR, false, false, kBf16);
       int item = 0, k = w.k0;
       for (int g = 0; g < N; ++g) {
@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == 2) {
     // ---- O^T += V^T P^T ----
-    if (lane == 0) {
+    if (tc::elect_one()) {
       constexpr uint32_t ID_O = tc::idesc_f16(128, NR, true, false, kBf16);
       constexpr uint32_t kGroup = (D / 64) * 1024;  // bytes from one 8-position group of a stage to the next
       int item = 0, k = w.k0;
