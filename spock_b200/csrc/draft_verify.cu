@@ -29,7 +29,13 @@ namespace {
 
 constexpr int kT = 256, kW = kT / 32;
 constexpr int kCluster = 8;
+// CTAs of verify_pick_kernel on an SM: its arithmetic needs independent chains
+// more than warps (248320 logits x 64 rows: 110 us at 3 with 80 registers and two
+// chunks at a time, 129 at 4 with 64).
+constexpr int kResident = 3;
 constexpr int kSteps = 64;  // step sums kept per warp
+constexpr int U = 2;        // chunks in flight, and of independent 64-bit arithmetic
+constexpr int kBatch = 32 * U;
 // The fp32 Z is off by less than this part of itself: each e by 3 roundings of
 // its exponent (up to 126 * 2^-24 * 3 ln 2 < 2^-15.8 of e) and ex2's 2^-22, the
 // sums by one rounding of 2^-24 per term of a thread (kThreadTerms = 2^11, so
@@ -79,16 +85,30 @@ struct Row {
       }
     }
   }
+  static constexpr uint32_t kNone =  // -inf in each element
+      sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  static __device__ __forceinline__ uint4 none() { return make_uint4(kNone, kNone, kNone, kNone); }
   // any chunk
-  __device__ __forceinline__ void load(int k, float (&v)[C]) const {
-    if (inner(k)) {
-      open(__ldg(base + k), v);
-    } else {
-      const int64_t j0 = (int64_t)k * C - a;
-#pragma unroll
-      for (int i = 0; i < C; ++i) v[i] = j0 + i >= 0 && j0 + i < vocab ? load_as_f32(x, j0 + i) : -INFINITY;
-    }
+  __device__ __forceinline__ uint4 fetch(int k) const {
+    if (inner(k)) return __ldg(base + k);
+    return ragged(x, a, vocab, k);
   }
+  static __device__ __noinline__ uint4 ragged(const T* x, int a, int vocab, int k) {
+    using Bits = typename std::conditional<sizeof(T) == 4, uint32_t, uint16_t>::type;
+    const int64_t j0 = (int64_t)k * C - a;
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const bool there = j0 + i >= 0 && j0 + i < vocab;
+      const uint32_t bits = there ? (uint32_t)reinterpret_cast<const Bits*>(x)[j0 + i] : (uint32_t)(Bits)kNone;
+      const int at = i * (int)sizeof(T);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (u == at >> 2) w[u] |= bits << (at & 3) * 8;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ __forceinline__ void load(int k, float (&v)[C]) const { open(fetch(k), v); }
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -111,19 +131,28 @@ int stat_splits(int64_t total, int64_t vocab) {
 
 template <typename T>
 __global__ void __launch_bounds__(kT) verify_stats_kernel(const VerifyArgs A, int splits) {
-  constexpr int C = kChunk<T>, U = 4;
+  constexpr int C = kChunk<T>;
   __shared__ float s_top[kW], s_z[kW];
   __shared__ int s_best[kW];
   pdl_wait();
   pdl_launch();
   const int row = blockIdx.x / splits, part = blockIdx.x % splits, t = threadIdx.x;
+  const Row<T> x(static_cast<const T*>(A.logits) + row * A.logits_ld, (int)A.vocab);
+  const int k0 = (int)((int64_t)x.chunks * part / splits), k1 = (int)((int64_t)x.chunks * (part + 1) / splits);
+  int k = max(k0, x.f0) + t;
+  const int kf = min(k1, x.f1);
+  // the first loads go out before the row's sequence is known
+  uint4 raw[U];
+  const bool full = k + (U - 1) * kT < kf;
+  if (full) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u] = __ldg(x.base + k + u * kT);
+  }
   const int b = seq_of_row(A.start, A.batch, row, t & 31);
   if (b < 0) return;
   const float temp = A.temperature ? A.temperature[b] : 1.0f;
   const bool greedy = !(temp > 0.f);
   const float c = 1.44269504088896341f / temp;
-  const Row<T> x(static_cast<const T*>(A.logits) + row * A.logits_ld, (int)A.vocab);
-  const int k0 = (int)((int64_t)x.chunks * part / splits), k1 = (int)((int64_t)x.chunks * (part + 1) / splits);
   float top = -INFINITY, z = 0.f;
   int at = -1;  // chunk of the thread's first maximum
   // a thread's chunks are kT apart, U of them in flight at a time
@@ -151,16 +180,18 @@ __global__ void __launch_bounds__(kT) verify_stats_kernel(const VerifyArgs A, in
     }
     top = m;
   };
-  int k = max(k0, x.f0) + t;
-  const int kf = min(k1, x.f1);
   float v[U][C];
-  for (; k + (U - 1) * kT < kf; k += U * kT) {
-    uint4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) raw[u] = __ldg(x.base + k + u * kT);
+  for (bool more = full; more;) {
 #pragma unroll
     for (int u = 0; u < U; ++u) x.open(raw[u], v[u]);
-    take(v, U, k);
+    const int at_k = k;
+    k += U * kT;
+    more = k + (U - 1) * kT < kf;
+    if (more) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) raw[u] = __ldg(x.base + k + u * kT);
+    }
+    take(v, U, at_k);
   }
   for (; k < kf; k += kT) {
     x.open(__ldg(x.base + k), v[0]);
@@ -229,21 +260,6 @@ __global__ void __launch_bounds__(kT) verify_stats_kernel(const VerifyArgs A, in
   }
 }
 
-// 2^(t / 256) for t <= 0: t = n + f with |f| <= 1/2, 2^(n/256) from a table,
-// 2^(f/256) as a cubic of f: with r = f ln 2 / 256 (|r| < 2^-9.5) the next term,
-// r^4 / 24, is below 1.4e-13. Exactly 1 at 0; meaningless below -2^18. Entry i of
-// the table is 2^(i/256) with i * 4096 taken off its high word, so that adding
-// n * 4096 (n = 256 e + i) leaves e in the exponent.
-__device__ __forceinline__ double exp2_neg(double t, const double* tab) {
-  constexpr double h = 0.69314718055994530942 / 256.0, big = 6755399441055744.0;  // 1.5 * 2^52
-  const double k = t + big;  // rounds to a whole number
-  const int n = __double2loint(k);
-  const double f = t - (k - big);
-  const double e = tab[n & 255];
-  const double s = __hiloint2double(__double2hiint(e) + n * 4096, __double2loint(e));
-  return fma(s * f, fma(fma(f, h * h * h / 6.0, h * h / 2.0), f, h), s);
-}
-
 // Combines a row's parts, by one warp.
 __device__ __forceinline__ Part join_parts(const Part* p, int splits, float c, int lane) {
   Part r{-INFINITY, 0x7fffffff, 0.f, 0};
@@ -275,10 +291,28 @@ __device__ __forceinline__ double warp_sum(double x) {
   return x;
 }
 
+// What e is relative to, in 64 bits. With t = x c (c = 256 log2(e) / T) and I = rint(max c):
+//   e = 2^((t - I) / 256), which is `one` (within 2^(1/512) of 1) at the maximum.
+// n = rint(t) - I and f = t - rint(t), |f| <= 1/2, cost three operations as t is
+// never rounded by itself: adding 1.5 * 2^52 - I to the exact product leaves n in
+// the low word. 2^(n/256) comes from a table, 2^(f/256) as a cubic of f: with
+// r = f ln 2 / 256 (|r| < 2^-9.5) the next term, r^4 / 24, is below 1.4e-13. Entry
+// i of the table is 2^(i/256) with i * 4096 taken off its high word, so that
+// adding n * 4096 (n = 256 k + i) leaves k in the exponent.
 struct Top {
-  double d;    // the largest logit
-  float least; // logits up to this one have no weight
-  bool inf;    // the largest is +inf: each +inf weighs 1
+  double c, magic;  // 1.5 * 2^52 - I
+  float least;      // logits up to this one have no weight (e below 2^-1000, -inf, NaN)
+  bool count;       // those above it weigh 1 each: they are +inf, or T is so small
+                    // that only logits equal to the largest have any weight
+  __device__ __forceinline__ double weight(float x, const double* tab) const {
+    constexpr double h = 0.69314718055994530942 / 256.0;
+    const double xd = (double)x, k = fma(xd, c, magic), f = fma(xd, c, magic - k);
+    const int n = __double2loint(k);
+    const double e = tab[n & 255];
+    const double s = __hiloint2double(__double2hiint(e) + n * 4096, __double2loint(e));
+    const double w = fma(s * f, fma(fma(f, h * h * h / 6.0, h * h / 2.0), f, h), s);
+    return x > least ? w : 0.0;
+  }
 };
 
 __device__ __forceinline__ double warp_scan(double x, int lane) {
@@ -315,7 +349,7 @@ __device__ __forceinline__ int first_over(const double (&x)[2], const double (&u
 enum { kAccept = 0, kReject = 1, kUnsure = 2 };
 
 template <typename T>
-__global__ void __launch_bounds__(kT, 4) verify_pick_kernel(const VerifyArgs A, int splits) {
+__global__ void __launch_bounds__(kT, kResident) verify_pick_kernel(const VerifyArgs A, int splits) {
   constexpr int C = kChunk<T>;
   __shared__ double s_tab[256], s_step[kW][kSteps], s_warp[kW];
   __shared__ int s_say[kW];
@@ -341,18 +375,16 @@ __global__ void __launch_bounds__(kT, 4) verify_pick_kernel(const VerifyArgs A, 
   const double c256 = fmin(256.0 * 1.44269504088896340736 / (double)temp, 1e300);
   __syncthreads();
 
-  // e of one logit, exactly 1 at the top; 0 for -inf, for NaN and where e would
-  // be below 2^-1000
-  auto weight = [&](float x, const Top& top) -> double {
-    const double e = exp2_neg(((double)x - top.d) * c256, s_tab);
-    return x > top.least ? e : 0.0;
-  };
   auto top_of = [&](float top) -> Top {
-    // +inf: the logits that are +inf count 1, the others 0
-    if (top == INFINITY) return {0.0, 3.4028235e38f, true};
-    if (top == -INFINITY) return {0.0, INFINITY, false};  // no weights
+    constexpr double big = 6755399441055744.0;  // 1.5 * 2^52
+    if (top == INFINITY) return {0.0, big, 3.4028235e38f, true};
+    if (top == -INFINITY) return {0.0, big, INFINITY, false};  // no weights
+    const float below = nextafterf(top, -INFINITY);
+    const double t = (double)top * c256;
+    // neighbours of the maximum are 2^-24 of it away, and 2^-24 * 2^49 / 256 octaves down
+    if (!(fabs(t) < 562949953421312.0)) return {0.0, big, below, true};
     const double least = (double)top - 256000.0 / c256;
-    return {(double)top, fminf((float)least, nextafterf(top, -INFINITY)), false};
+    return {c256, big - rint(t), fminf((float)least, below), false};
   };
   const int nw = ranks * kW, me = rank * kW + warp;
   // Sums f(chunk, logits) over this warp's chunks of a row, step by step; the
@@ -363,13 +395,18 @@ __global__ void __launch_bounds__(kT, 4) verify_pick_kernel(const VerifyArgs A, 
     k0 = (int)((int64_t)x.chunks * me / nw);
     k1 = (int)((int64_t)x.chunks * (me + 1) / nw);
     const int most = (x.chunks + nw - 1) / nw;  // a warp's most
-    per_step = (most + 32 * kSteps - 1) / (32 * kSteps) * 32;
+    per_step = (most + kBatch * kSteps - 1) / (kBatch * kSteps) * kBatch;
     double all = 0.0;
     int step = 0;
     for (int k = k0; k < k1; k += per_step, ++step) {
       const int end = min(k1, k + per_step);
       double s = 0.0;
-      for (int q = k + lane; q < end; q += 32) s += f(q);
+      for (int q = k + lane; q - lane < end; q += 32 * U) {
+        uint4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = q + u * 32 < end ? x.fetch(q + u * 32) : Row<T>::none();
+        s += f(q, end, raw);
+      }
       s = warp_sum(s);
       if (lane == 0) s_step[warp][step] = s;
       all += s;
@@ -386,19 +423,33 @@ __global__ void __launch_bounds__(kT, 4) verify_pick_kernel(const VerifyArgs A, 
     return __shfl_sync(0xffffffffu, upto[1], 31);
   };
   auto row_of = [&](int r) { return Row<T>(logits + r * A.logits_ld, (int)A.vocab); };
+  // a chunk's weights: e; e without the draft's; max(e / Z - q, 0)
+  auto plain = [&](const Row<T>& x, const Top& top, const uint4& raw, double(&w)[C]) {
+    float v[C];
+    x.open(raw, v);
+    if (top.count) {
+#pragma unroll
+      for (int i = 0; i < C; ++i) w[i] = v[i] > top.least ? 1.0 : 0.0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) w[i] = top.weight(v[i], s_tab);
+    }
+  };
+  auto add_up = [](const double(&w)[C]) {
+    double s[2] = {0.0, 0.0};
+#pragma unroll
+    for (int i = 0; i < C; ++i) s[i & 1] += w[i];
+    return s[0] + s[1];
+  };
   auto sum_e = [&](const Row<T>& x, const Top& top) -> double {
-    return sum_row(x, [&](int k) {
-      float v[C];
-      x.load(k, v);
-      double s[2] = {0.0, 0.0};
-      if (top.inf) {
+    return sum_row(x, [&](int, int, const uint4(&raw)[U]) {
+      double s = 0.0, w[C];
 #pragma unroll
-        for (int i = 0; i < C; ++i) s[0] += v[i] > top.least ? 1.0 : 0.0;
-      } else {
-#pragma unroll
-        for (int i = 0; i < C; ++i) s[i & 1] += weight(v[i], top);
+      for (int u = 0; u < U; ++u) {
+        plain(x, top, raw[u], w);
+        s += add_up(w);
       }
-      return s[0] + s[1];
+      return s;
     });
   };
   auto draft_of = [&](int i) -> int {
@@ -415,7 +466,8 @@ __global__ void __launch_bounds__(kT, 4) verify_pick_kernel(const VerifyArgs A, 
     if (greedy) return (p.best == 0x7fffffff ? 0 : p.best) == d ? kAccept : kReject;
     const Top top = top_of(p.top);
     const float x = load_as_f32(logits + r * A.logits_ld, d);
-    const double e = top.inf ? (double)(x > top.least) : weight(x, top);
+    const double e = top.count ? (double)(x > top.least) : top.weight(x, s_tab);
+    if (sure > 0.0 && !top.count) z *= top.weight(p.top, s_tab);  // Z of 32 bits is relative to e = 1 at the maximum
     const double q = A.probs ? (double)A.probs[r * A.probs_ld + d] : 1.0;
     const double uqz = (double)A.u_accept[r] * q * z;
     if (uqz * (1.0 + sure) < e && uqz * (1.0 - sure) < e) return kAccept;
@@ -462,28 +514,7 @@ __global__ void __launch_bounds__(kT, 4) verify_pick_kernel(const VerifyArgs A, 
     const Top top = top_of(p.top);
     const double inv_z = q ? 1.0 / sum_e(x, top) : 0.0;
     const bool q16 = ((uintptr_t)q & 15) == 0;  // whether they are aligned too
-    // a chunk's weights: e; e without the draft's; max(e / Z - q, 0)
-    auto plain = [&](int k, double(&w)[C]) {
-      float v[C];
-      x.load(k, v);
-      if (top.inf) {
-#pragma unroll
-        for (int i = 0; i < C; ++i) w[i] = v[i] > top.least ? 1.0 : 0.0;
-      } else {
-#pragma unroll
-        for (int i = 0; i < C; ++i) w[i] = weight(v[i], top);
-      }
-    };
-    auto without = [&](int k, double(&w)[C]) {
-      plain(k, w);
-      const int64_t at = (int64_t)drop + x.a - (int64_t)k * C;
-      if (at >= 0 && at < C) {
-#pragma unroll
-        for (int i = 0; i < C; ++i) w[i] = i == at ? 0.0 : w[i];
-      }
-    };
-    auto beyond = [&](int k, double(&w)[C]) {
-      float qv[C];
+    auto fetch_q = [&](int k, float(&qv)[C]) {  // 0 where the chunk has no element
       if (q16 && x.inner(k)) {
 #pragma unroll
         for (int i = 0; i < C; i += 4) {
@@ -497,27 +528,58 @@ __global__ void __launch_bounds__(kT, 4) verify_pick_kernel(const VerifyArgs A, 
           qv[i] = j >= 0 && j < A.vocab ? __ldg(q + (int64_t)k * C + i) : 0.f;
         }
       }
-      plain(k, w);
+    };
+    auto without = [&](int k, double(&w)[C]) {
+      const int64_t at = (int64_t)drop + x.a - (int64_t)k * C;
+      if (at >= 0 && at < C) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) w[i] = i == at ? 0.0 : w[i];
+      }
+    };
+    auto beyond = [&](const float(&qv)[C], double(&w)[C]) {
 #pragma unroll
       for (int i = 0; i < C; ++i) {
         const double y = fma(w[i], inv_z, -(double)qv[i]);
         w[i] = y > 0.0 ? y : 0.0;
       }
     };
-    auto sum_of = [&](auto weights) {
-      return sum_row(x, [&](int k) {
-        double w[C], s[2] = {0.0, 0.0};
-        weights(k, w);
+    auto sum_plain = [&] { return sum_e(x, top); };
+    auto sum_without = [&] {
+      return sum_row(x, [&](int k, int, const uint4(&raw)[U]) {
+        double s = 0.0, w[C];
 #pragma unroll
-        for (int i = 0; i < C; ++i) s[i & 1] += w[i];
-        return s[0] + s[1];
+        for (int u = 0; u < U; ++u) {
+          plain(x, top, raw[u], w);
+          without(k + u * 32, w);
+          s += add_up(w);
+        }
+        return s;
+      });
+    };
+    auto sum_beyond = [&] {
+      return sum_row(x, [&](int k, int end, const uint4(&raw)[U]) {
+        double s = 0.0, w[C];
+        float qv[C];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (k + u * 32 < end) {
+            fetch_q(k + u * 32, qv);
+          } else {
+#pragma unroll
+            for (int i = 0; i < C; ++i) qv[i] = 0.f;
+          }
+          plain(x, top, raw[u], w);
+          beyond(qv, w);
+          s += add_up(w);
+        }
+        return s;
       });
     };
     bool rest = drafted;
-    double W = rest ? (q ? sum_of(beyond) : sum_of(without)) : sum_of(plain);
+    double W = rest ? (q ? sum_beyond() : sum_without()) : sum_plain();
     if (rest && !(W > 0.0)) {
       rest = false;
-      W = sum_of(plain);
+      W = sum_plain();
     }
     // the warp whose sums cross u W, or the last that has any weight
     const double at = (double)A.u_sample[b] * W;
@@ -541,12 +603,14 @@ __global__ void __launch_bounds__(kT, 4) verify_pick_kernel(const VerifyArgs A, 
         for (int e = 0; e < C; ++e) w[e] = 0.0;
         const int j0 = x.first(k + lane);
         if (k + lane < end) {
-          if (!rest)
-            plain(k + lane, w);
-          else if (q)
-            beyond(k + lane, w);
-          else
+          plain(x, top, x.fetch(k + lane), w);
+          if (rest && q) {
+            float qv[C];
+            fetch_q(k + lane, qv);
+            beyond(qv, w);
+          } else if (rest) {
             without(k + lane, w);
+          }
         }
 #pragma unroll
         for (int e = 0; e < C; ++e) s += w[e];
@@ -587,10 +651,9 @@ Status launch(const VerifyArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return cuda_status(e, "verify_stats_kernel");
     SPOCK_LAUNCH_CHECK("verify_stats_kernel");
   }
-  // a CTA per 8192 logits of a row, up to the portable cluster size, while all
-  // are resident at once (4 an SM)
-  int ranks = 1;
-  while (ranks < kCluster && (int64_t)ranks * 8192 < a.vocab && (int64_t)a.batch * ranks * 2 <= 148 * 4) ranks *= 2;
+  // a CTA per 8192 logits of a row, up to the portable cluster size, while all are resident at once
+  const int64_t most = std::min<int64_t>(kCluster, (a.vocab + 8191) / 8192);
+  const int ranks = (int)std::max<int64_t>(1, std::min<int64_t>(most, 148 * kResident / a.batch));
   pdl_scope overlap;  // its launch and table run under the first kernel
   e = launch_k_cluster(verify_pick_kernel<T>, dim3((unsigned)a.batch * ranks), dim3(kT), dim3(ranks), 0, st, a,
                        splits);
