@@ -349,7 +349,9 @@ int spock_paged_attention_prep(spock_ctx* ctx, const spock_paged_kv* kv, int32_t
  * head. One entry for decode tokens, drafts, prompt chunks and any mix.
  *   out[r][h] = sum_p softmax_p(scale * q[r][h] . k_p) v_p, times
  *   sigmoid(gate[r][h]) when gate is not NULL; rounded once
- *   q, gate rows and heads at their own strides (elements, multiples of 8)
+ *   q, gate rows and heads at their own strides (elements, multiples of 8;
+ *           q's positive)
+ *   scale   positive and finite
  *   out     [total][q_heads][head_dim], contiguous
  * Slots behind kv_len are not used, whatever they hold; the positions below
  * it hold finite keys and values.

@@ -522,7 +522,8 @@ def paged_attention(q, start, k_pages, v_pages, page_table, kv_len, scale, gate=
                     stream=None):
     """Causal attention of each sequence's new tokens over its pages (spock_paged_attention).
 
-    q [total, q_heads, head_dim] and gate (or None), any row and head strides; the cache as in paged_attention_prep.
+    q [total, q_heads, head_dim] and gate (or None), any row and head strides (positive ones for q); scale positive
+    and finite; the cache as in paged_attention_prep.
     Token t of n sees positions 0 .. kv_len - n + t. Returns out [total, q_heads, head_dim]: softmax(scale q k) v,
     times sigmoid(gate); rows behind start[batch] are left as they are. `workspace`: a uint8 tensor of
     the caller's instead of one from the caching allocator."""

@@ -1,6 +1,7 @@
 // extern "C" boundary of libspock_b200.so (declared in include/spock_b200.h).
 // Argument validation and error text live here; the kernels' launchers return
 // spock::Status. Nothing here throws across the ABI.
+#include <cfloat>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -372,6 +373,13 @@ __attribute__((visibility("default"))) int spock_paged_attention(
       q_row_stride % 8 || q_head_stride % 8 || (gate && (gate_row_stride % 8 || gate_head_stride % 8)))
     return fail(ctx, SPOCK_ERR_INVALID,
                 std::string(op) + "pointers must be 16-byte aligned and strides multiples of 8");
+  // what a tensor map can hold; a stride that is never used may be anything
+  constexpr int64_t kFar = (int64_t)1 << 38;
+  if ((total > 1 && (q_row_stride <= 0 || q_row_stride > kFar)) ||
+      (q_heads > 1 && (q_head_stride <= 0 || q_head_stride > kFar)))
+    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "q strides must be positive (and at most 2^38)");
+  if (!(scale > 0.f && scale <= FLT_MAX))
+    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "scale must be positive and finite");
   if (workspace_bytes < spock::paged_attention_workspace(q_heads, kv->kv_heads, kv->head_dim, ctx->sms))
     return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "workspace too small");
   DeviceGuard dg(ctx->device);

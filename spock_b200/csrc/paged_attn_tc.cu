@@ -42,6 +42,14 @@ namespace {
 
 using namespace paged;
 
+// A row tile of this CTA, for the roles that do not walk by themselves (a walk's
+// steps cost the softmax warps 1900 cycles each).
+struct Item {
+  int lo, n, len;  // its sequence: first packed row, new tokens, positions
+  int h, rt;       // kv head, row tile
+  int k0, k1, nt;  // KV tiles here, in all
+};
+
 template <int D>
 struct Shape {
   // A stage is 32 KB (16 KB at head size 64): of K 128 positions x DB dims, of V
@@ -54,14 +62,15 @@ struct Shape {
   static constexpr int NST = D == 256 ? 5 : D == 128 ? 6 : 8;
   static constexpr int kBar = kQ + NST * kStage;
   static constexpr int kRed = kBar + 576;
-  static constexpr int kSmem = kRed + 4 * 128 * 4;
+  static constexpr int kItem = kRed + 4 * 128 * 4;
+  static constexpr int kSmem = kItem + 2 * sizeof(Item);
 };
 static_assert(Shape<256>::kSmem <= 227 * 1024 && Shape<128>::kSmem <= 227 * 1024, "shared memory of one SM");
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
-                      const __grid_constant__ AttnArgs A) {
+                      const __grid_constant__ CUtensorMap tmq, const __grid_constant__ AttnArgs A) {
   using Sh = Shape<D>;
   constexpr int DB = Sh::DB, KS = Sh::KS, NST = Sh::NST;
   constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
@@ -76,11 +85,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   // whole phase further on
   uint64_t* o_done = q_full + 6;
   uint64_t* drain = q_full + 8;
-  volatile int* s_fail = reinterpret_cast<volatile int*>(q_full + 9);
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(q_full + 9) + 1;
+  uint64_t* entered = q_full + 9;  // [2], by row tile parity: its Item is there
+  volatile int* s_fail = reinterpret_cast<volatile int*>(q_full + 11);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(q_full + 11) + 1;
   int64_t* s_scan = reinterpret_cast<int64_t*>(sm + Sh::kBar + 256);  // [2 warps + 4]
   int* s_first = reinterpret_cast<int*>(s_scan + 2 * (kThreads / 32) + 4);  // [4]
-  volatile int* s_armed = s_first + 4;  // [NST]
+  volatile int* s_armed = s_first + 4;  // [NST + 1]
+  Item* s_item = reinterpret_cast<Item*>(sm + Sh::kItem);  // [2], by row tile parity
   float* red = reinterpret_cast<float*>(sm + Sh::kRed);  // [2 tiles][2 halves][128] maxima (and sums)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x, ctas = gridDim.x;
@@ -102,13 +113,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::mbar_init(&s_full[i], 1);
       tc::mbar_init(&p_full[i], 8);
       tc::mbar_init(&o_done[i], 1);
+      tc::mbar_init(&entered[i], 1);
     }
     tc::mbar_init(drain, 1);
     *s_fail = 0;
-    for (int i = 0; i < NST; ++i) s_armed[i] = 0;
+    for (int i = 0; i <= NST; ++i) s_armed[i] = 0;
     tc::fence_mbar_init();
     tc::prefetch_tmap(&tmk);
     tc::prefetch_tmap(&tmv);
+    tc::prefetch_tmap(&tmq);
   }
   if (warp == 1) {
     tc::tmem_alloc(s_tmem, 512);
@@ -139,14 +152,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t ID_S = tc::idesc_f16(128, kTile, false, false, kBf16);
       constexpr uint32_t ID_O = tc::idesc_f16(128, D, false, true, kBf16);
       constexpr uint32_t kGroup = (D / 64) * 1024;  // bytes from one 8-position group of a V stage to the next
-      int item = 0, k = w.k0, gs = 0, go = 0;  // the next S and O
+      int item = 0, left = 0, gs = 0, go = 0;  // the next S and O; S tiles left of the row tile
       bool fresh = true;    // S(gs) is its row tile's first
       uint32_t starts = 0;  // bit g & 1: O(g) starts from zero
       while (go < N) {
         // S(g + 1) goes before O(g), unless it waits for the next row tile's queries
         if (gs < N && (gs == go || (gs == go + 1 && !fresh))) {
           const int g = gs++;
-          if (fresh && !wait(q_full, item & 1)) break;
+          if (fresh) {
+            if (!wait(q_full, item & 1)) break;
+            left = s_item[item & 1].k1 - s_item[item & 1].k0;
+            tc::mbar_arrive(&entered[item & 1]);
+          }
           starts = (starts & ~(1u << (g & 1))) | (uint32_t)fresh << (g & 1);
           bool ok = true;
 #pragma unroll
@@ -164,11 +181,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (!ok) break;
           tc::mma_commit(&s_full[g & 1]);
-          fresh = ++k == w.k1;
+          fresh = --left == 0;
           if (fresh) {
             tc::mma_commit(q_empty);
-            w.next(A);
-            k = w.k0;
             ++item;
           }
         } else {
@@ -195,40 +210,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 3) {
-    // ---- queries ----
-    for (int item = 0;; ++item) {
-      bool ok = true;
-      if (item > 0) {
-        if (lane == 0) ok = wait(q_empty, (item - 1) & 1);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+    // ---- queries: a box of tp tokens x G heads for each 64 dims ----
+    if (tc::elect_one()) {
+      const uint32_t bytes = (uint32_t)(A.tp * A.G) * 128;
+      for (int item = 0;; ++item) {
+        if (item > 0 && !wait(q_empty, (item - 1) & 1)) break;
+        s_item[item & 1] = {w.s.lo, w.s.n, w.s.len, w.h, w.rt, w.k0, w.k1, w.nt};
+        s_armed[NST] = item + 1;
+        tc::mbar_arrive_expect_tx(q_full, bytes * (D / 64));
+#pragma unroll
+        for (int blk = 0; blk < D / 64; ++blk)
+          tc::tma_load_3d(sm + blk * 16384, &tmq, q_full, blk * 64, w.h * A.G, w.s.lo + w.rt * A.tp);
+        if (!w.next(A)) break;
       }
-      if (!ok) break;
-      const int t0 = w.rt * A.tp, rows = min(A.tp, w.s.n - t0) * A.G;
-      constexpr int CH = D / 8;                   // 16-byte chunks of a row
-      constexpr int RW = CH >= 32 ? 1 : 32 / CH;  // rows per warp instruction
-      const int sub = CH >= 32 ? 0 : lane / CH, c = CH >= 32 ? lane : lane % CH;
-      int r = sub, tt = r / A.G, gh = r - tt * A.G;
-#pragma unroll 4
-      for (; r < rows; r += RW) {
-        const uint8_t* src = A.q + (int64_t)(w.s.lo + t0 + tt) * A.q_row + (int64_t)(w.h * A.G + gh) * A.q_head + c * 16;
-        cp_async16(sbase + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4), src);
-        gh += RW;
-        while (gh >= A.G) gh -= A.G, ++tt;
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      tc::fence_async_smem();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(q_full);
-      if (!w.next(A)) break;
     }
+    __syncwarp();
   } else {
     // ---- softmax and outputs ----
     const int quad = warp & 3, half = (warp - 4) >> 2, row = quad * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const float c = A.scale_log2;
     // A wait that gives up does not leave the loop: the warps of a pair meet at
-    // named barriers, so all of them walk on (each later wait returns at once)
-    // and the outputs are unspecified.
+    // named barriers, so all of them walk on (each later wait returns at once),
+    // with empty row tiles from the next one on; the outputs are unspecified.
     auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
       if (lane == 0) wait(bar, parity);  // one lane polls: 32 would crowd the pipe that MMAs and loads go through
       __syncwarp();
@@ -237,13 +241,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory"); };
     if (tid == 128) meta[cta].slot = -1, meta[cta].units = N;
     float m = -INFINITY, l = 0.f;
-    int k = w.k0, item = 0;
-    int t0 = 0, rows = 0, lim = 0, lim0 = 0, tt = 0;
-    auto enter = [&] {
-      t0 = w.rt * A.tp;
-      rows = min(A.tp, w.s.n - t0) * A.G;
-      tt = row / A.G;
-      lim = row < rows ? w.s.len - w.s.n + t0 + tt : 0x7fffffff;
+    int k = 0, item = 0;
+    int t0 = 0, rows = 0, lim = 0, lim0 = 0;
+    const int tt = row / A.G;
+    Item it;
+    auto enter = [&] {  // O of the row tile before cannot be issued without this one's warps: never two phases behind
+      bool ok = true;
+      if (lane == 0) ok = wait(&entered[item & 1], (item >> 1) & 1);
+      uint32_t both;  // the pair agrees
+      asm volatile(
+          "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.and.pred q, %2, 64, p;\n selp.u32 %0, 1, 0, q;\n}"
+          : "=r"(both)
+          : "r"((uint32_t)ok), "r"(1 + quad)
+          : "memory");
+      if (both)
+        it = s_item[item & 1];
+      else
+        it = Item{0, 0, 0, 0, 0, 0, 0, 0};
+      k = it.k0;
+      t0 = it.rt * A.tp;
+      rows = min(A.tp, it.n - t0) * A.G;
+      lim = row < rows ? it.len - it.n + t0 + tt : 0x7fffffff;
       lim0 = __shfl_sync(0xffffffffu, lim, 0);
       m = -INFINITY;
       l = 0.f;
@@ -253,8 +271,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int buf = g & 1, p0 = k * kTile;
       const bool live = quad * 32 < rows;
       wait_warp(&s_full[buf], (g >> 1) & 1);
-      if (p0 + kTile > w.s.len) {  // slots behind the sequence: their V rows become zero
-        const int first = max(0, w.s.len - p0);
+      if (p0 + kTile > it.len) {  // slots behind the sequence: their V rows become zero
+        const int first = max(0, it.len - p0);
         // V(g - 1) has been read, so every earlier load of V(g)'s stages is over:
         // their barriers are at most one phase behind and the parities are V(g)'s
         if (g > 0) wait_warp(&o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
@@ -286,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float corr = move ? ex2((m - top) * c) : 1.0f;
           if (move) m = top;
           l *= corr;
-          if (k > w.k0) {
+          if (k > it.k0) {
             wait_warp(&o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
 #pragma unroll 1
             for (int cb = 0; cb < D / 64; ++cb) {
@@ -316,22 +334,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::tc_fence_before();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&p_full[buf]);
-      if (++k < w.k1) continue;
+      if (++k < it.k1) continue;
 
       // ---- the row tile's last KV tile here ----
-      const bool whole = w.k0 == 0 && w.k1 == w.nt;
-      const int64_t tok = w.s.lo + t0 + tt;
-      const int hq = w.h * A.G + row - tt * A.G;
+      const bool whole = it.k0 == 0 && it.k1 == it.nt;
+      const int64_t tok = it.lo + t0 + tt;
+      const int hq = it.h * A.G + row - tt * A.G;
       wait_warp(&o_done[buf], (g >> 1) & 1);
       const int slot = item == 0 ? 0 : 1;
-      if (!whole && w.k0 == 0 && tid == 128) {
+      if (!whole && it.k0 == 0 && tid == 128) {
         Meta& mt = meta[cta];
         mt.slot = slot;
-        mt.row0 = w.s.lo + t0;
+        mt.row0 = it.lo + t0;
         mt.rows = rows;
-        mt.head = w.h;
-        mt.have = w.k1;
-        mt.nt = w.nt;
+        mt.head = it.h;
+        mt.have = it.k1;
+        mt.nt = it.nt;
       }
       if (live) {
         float* rl = red + (buf ^ 1) * 256;  // idle: the maxima of the tile before, read by both halves
@@ -388,11 +406,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (w.next(A)) {
-        k = w.k0;
-        ++item;
-        enter();
-      }
+      ++item;
+      if (g + 1 < N) enter();
     }
   }
   __syncwarp();
@@ -403,6 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) {
       atomicExch(A.err, 5);
       drain_ring(full, s_armed, NST);
+      if (s_armed[NST]) tc::mbar_wait_bounded(q_full, (s_armed[NST] - 1) & 1, kWait);
     }
     if (tid == 32) {
       tc::mma_commit(drain);
@@ -575,7 +591,7 @@ Status launch(const spock_paged_kv& kv, AttnArgs& A, bool few, int sms, cudaStre
   A.extra = 3;
   A.piece_k = gcd(kv.page_size, kTile);
   A.piece_v = gcd(kv.page_size, Shape<D>::VP);
-  CUtensorMap mk, mv;
+  CUtensorMap mk, mv, mq;
   if (encode_pages(fn, &mk, kv, kv.k, A.piece_k, Shape<D>::DB) != CUDA_SUCCESS ||
       encode_pages(fn, &mv, kv, kv.v, A.piece_v, D) != CUDA_SUCCESS)
     return Status::err(SPOCK_ERR_CUDA, "spock_paged_attention: tensor map encoding failed");
@@ -595,7 +611,17 @@ Status launch(const spock_paged_kv& kv, AttnArgs& A, bool few, int sms, cudaStre
       if (e != cudaSuccess) return cuda_status(e, "paged_attn_kernel attribute");
       done.fetch_or(bit);
     }
-    e = launch_k(paged_attn_kernel<T, D>, dim3(sms), dim3(kThreads), Shape<D>::kSmem, st, mk, mv, A);
+    // queries as [token][head][dim]
+    const int heads = A.kv_heads * A.G;
+    cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)A.total};
+    cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? A.q_head : D * 2), (cuuint64_t)(A.total > 1 ? A.q_row : D * 2)};
+    cuuint32_t box[3] = {64, (cuuint32_t)A.G, (cuuint32_t)A.tp}, estr[3] = {1, 1, 1};
+    if (fn(&mq, kv.dtype == SPOCK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+           const_cast<uint8_t*>(A.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return Status::err(SPOCK_ERR_CUDA, "spock_paged_attention: tensor map encoding failed");
+    e = launch_k(paged_attn_kernel<T, D>, dim3(sms), dim3(kThreads), Shape<D>::kSmem, st, mk, mv, mq, A);
     if (e != cudaSuccess) return cuda_status(e, "paged_attn_kernel");
     SPOCK_LAUNCH_CHECK("paged_attn_kernel");
   }

@@ -740,3 +740,159 @@ def test_wrappers_and_binding_agree(cuda_ok):
     a = spock_b200.draft_verify(logits, tokens, s, ua, us, None, q)
     b = spock_b200.draft_verify(logits, tokens, s, ua, us, None, q, stream=cur)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+MORE = [
+    # few rows a sequence: group sizes that do not divide the tile, a length of zero, uneven numbers of tokens
+    (F16, 128, 12, 4, 16, [1] * 70, [1 + 53 * i % 900 for i in range(70)]),
+    (BF16, 256, 16, 1, 16, [1, 1, 0, 1], [3000, 0, 7, 128]),
+    (F16, 128, 20, 1, 16, [1, 1, 1], [77, 0, 1025]),             # 20 heads over one
+    (F16, 128, 8, 2, 16, [0, 0, 1, 0], [5, 0, 40, 3]),
+    (BF16, 256, 8, 2, 32, [9, 0, 0, 2, 0, 0, 0, 0, 0, 0, 0, 0], [300, 9, 0, 130] + [5] * 8),
+    (F16, 128, 8, 2, 64, [1], [40000]),
+    (BF16, 128, 16, 16, 16, [1] * 5, [4000, 1, 129, 128, 127]),
+    # more sequences than a block has threads, many short row tiles
+    (BF16, 128, 8, 4, 32, [1] * 500, [1 + 17 * i % 300 for i in range(500)]),
+    (F16, 64, 4, 2, 16, [1, 0, 2] * 200, [2 + 29 * i % 200 for i in range(600)]),
+    (F16, 128, 16, 4, 16, [37] * 60, [37 + 11 * i for i in range(60)]),
+    (BF16, 256, 8, 2, 16, [70, 1, 5] * 14, [70 + 31 * i for i in range(42)]),
+]
+
+
+@pytest.mark.parametrize("case", range(len(MORE)))
+def test_paged_attention_more_batches(cuda_ok, case):
+    dtype, d, hq, hk, page, new, lens = MORE[case]
+    g = _gen(100 + case)
+    c = Cache(lens, page, hk, d, dtype, g, head_major=case % 2 == 1)
+    starts, total = _starts(new), sum(new)
+    q = torch.randn(total, hq, d, device=DEV, generator=g).to(dtype)
+    gate = torch.randn(total, hq, d, device=DEV, generator=g).to(dtype)
+    got = spock_b200.paged_attention(q, _i32(starts), *c.args(), 1 / math.sqrt(d), gate=gate)
+    spock_b200.Context.get(0).sync()
+    _check_attention(got, *_ref_attention(q, starts, c, 1 / math.sqrt(d), gate))
+
+
+@pytest.mark.parametrize("new", [1, 7])
+def test_pages_behind_the_32_bit_offsets(cuda_ok, new):
+    """Pages whose elements start beyond 2^31, shared by two sequences."""
+    g = _gen(8)
+    pages = 2 ** 31 // (16 * 2 * 256) + 20
+    c = Cache([40, 40], 16, 2, 256, F16, g)
+    big = [torch.empty(pages, 16, 2, 256, dtype=F16, device=DEV) for _ in range(2)]
+    far = _i32([pages - 1, pages - 9, pages - 4])
+    for x, small in zip(big, (c.k, c.v)):
+        x[far.long()] = small[c.table[0].long()]
+    c.k, c.v = big
+    c.table = far[None].repeat(2, 1).contiguous()
+    starts = _starts([new, new])
+    proj = torch.randn(2 * new, (8 + 4) * 256, device=DEV, generator=g).half()
+    qn = torch.zeros(256, dtype=F16, device=DEV)
+    q = spock_b200.paged_attention_prep(proj[:new], _i32([0, new, new]), *c.args(), q_norm=qn, k_norm=qn)
+    got = spock_b200.paged_attention(torch.cat([q, q]), _i32(starts), *c.args(), 0.0625)
+    spock_b200.Context.get(0).sync()
+    ids, slot = c.slots(0, torch.arange(40 - new, 40, device=DEV))
+    assert torch.equal(c.v[ids, slot], proj[:new, 10 * 256:].reshape(new, 2, 256))
+    assert torch.equal(got[:new], got[new:])
+    _check_attention(got, *_ref_attention(torch.cat([q, q]), starts, c, 0.0625, None))
+
+
+def test_calls_on_two_streams_at_once(cuda_ok):
+    g = _gen(9)
+    jobs = []
+    for lens, new in (([3000, 1500, 70], [1, 1, 1]), ([900, 2000], [5, 130])):
+        c = Cache(lens, 16, 2, 256, F16, g)
+        q = torch.randn(sum(new), 8, 256, device=DEV, generator=g).half()
+        jobs.append((c, q, _i32(_starts(new)), torch.cuda.Stream()))
+    rows = _verify_inputs([5, 3], 32003, F16, 5, True)
+    starts = _i32(_starts([5, 3]))
+    alone = [spock_b200.paged_attention(q, s, *c.args(), 0.0625) for c, q, s, _ in jobs]
+    alone_v = spock_b200.draft_verify(*rows[:2], starts, *rows[2:4], draft_probs=rows[4])
+    torch.cuda.synchronize()
+    together = []
+    for _ in range(10):
+        for c, q, s, stream in jobs:
+            with torch.cuda.stream(stream):
+                together.append((spock_b200.paged_attention(q, s, *c.args(), 0.0625),
+                                 spock_b200.draft_verify(*rows[:2], starts, *rows[2:4], draft_probs=rows[4])))
+    torch.cuda.synchronize()
+    for i, (out, verdict) in enumerate(together):
+        assert torch.equal(out, alone[i % 2])
+        assert all(torch.equal(x, y) for x, y in zip(verdict, alone_v))
+
+
+def test_the_four_steps_captured_and_replayed(cuda_ok):
+    """One graph of all four calls, replayed with other inputs, does what the calls do one by one."""
+    g = _gen(12)
+    new, lens, heads, vocab = [3, 1, 5], [40, 1, 300], 4, 1000
+    c = Cache(lens, 16, 2, 256, F16, g)
+    starts = _i32(_starts(new))
+    layer, qkv, conv, state, a, b, z = _span_inputs(new, heads, seed=12)
+    proj = torch.randn(9, 20 * 256, device=DEV, generator=g).half()
+    rope = _table(300, 64)
+    norm = torch.zeros(256, dtype=F16, device=DEV)
+    logits, tokens, ua, us, _ = _verify_inputs(new, vocab, F16, 12, False)
+    conv_out, state_out = torch.empty_like(conv), torch.empty_like(state)
+    gates = proj[:, :16 * 256].reshape(9, 8, 2, 256)[:, :, 1]
+
+    def step():
+        q = spock_b200.paged_attention_prep(proj, starts, *c.args(), rope=rope, q_norm=norm, k_norm=norm, gated=True)
+        att = spock_b200.paged_attention(q, starts, *c.args(), 0.0625, gate=gates)
+        dn = spock_b200.deltanet_decode_span(layer, qkv, conv, state, a, b, z, starts)
+        emitted, out = spock_b200.draft_verify(logits, tokens, starts, ua, us)
+        spock_b200.deltanet_decode_span(layer, qkv, conv, state, a, b, None, starts, counts=emitted,
+                                        conv_out=conv_out, state_out=state_out)
+        return att, dn, emitted, out
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(3):
+        proj.copy_(torch.randn(9, 20 * 256, device=DEV, generator=g))
+        logits.copy_(torch.randn(9, vocab, device=DEV, generator=g) * 3)
+        c.len.copy_(_i32([40 - i, 1 + i, 300 - 7 * i]))
+        pages = c.k.clone(), c.v.clone()
+        graph.replay()
+        got = [t.clone() for t in (*held, conv_out, state_out, c.k, c.v)]
+        c.k.copy_(pages[0])
+        c.v.copy_(pages[1])
+        want = (*step(), conv_out, state_out, c.k, c.v)
+        for x, y in zip(got, want):
+            assert torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8))
+    spock_b200.Context.get(0).sync()
+
+
+@pytest.mark.parametrize("probs", [False, True])
+def test_draft_verify_extreme_temperatures(cuda_ok, probs):
+    """Down to where only the largest logits weigh anything, up to where all weigh the same."""
+    heat = [1e-42, 1e-38, 1e-30, 1e-12, 1e-6, 1e-3, 30.0, 1e6, 1e30, 3e38]
+    rows = [3] * len(heat)
+    logits, tokens, ua, us, q = _verify_inputs(rows, 700, BF16, 21, probs)
+    logits[::3, 5:8] = logits[::3].amax(1, keepdim=True)  # several largest ones
+    temp = torch.tensor(heat, device=DEV, dtype=torch.float64).float()
+    assert _run_verify(logits, tokens, _starts(rows), ua, us, temp, q) == \
+        _ref_verify(logits, tokens, _starts(rows), ua, us, temp, q)
+
+
+def test_draft_verify_many_sequences(cuda_ok):
+    rows = [1 + i % 3 for i in range(700)]
+    logits, tokens, ua, us, q = _verify_inputs(rows, 130, F16, 22, True)
+    assert _run_verify(logits, tokens, _starts(rows), ua, us, None, q) == \
+        _ref_verify(logits, tokens, _starts(rows), ua, us, None, q)
+
+
+def test_paged_attention_refuses_scales_and_strides(cuda_ok):
+    g = _gen(1)
+    c = Cache([20], 16, 2, 64, F16, g)
+    q = torch.randn(2, 8, 64, device=DEV, generator=g).half()
+    call = lambda q, scale: spock_b200.paged_attention(q, _i32([0, q.shape[0]]), *c.args(), scale)
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(spock_b200.SpockError, match="positive and finite"):
+            call(q, scale)
+    for bad in (q[:1].expand(2, -1, -1), q[:, :1].expand(-1, 8, -1)):
+        with pytest.raises(spock_b200.SpockError, match="strides must be positive"):
+            call(bad, 1.0)
+    # a stride that is never used may be anything
+    one = torch.as_strided(q, (1, 8, 64), (0, 64, 1))
+    assert torch.equal(call(one, 1.0), call(q[:1], 1.0))
