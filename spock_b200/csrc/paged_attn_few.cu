@@ -46,7 +46,8 @@ struct Few {
   static constexpr int kBar = kRing + NST * kStage;
   static constexpr int kStat = kBar + 576;    // [2 row tiles][4 warps][NR] sums, [2][NR] references
   static constexpr int kMax = kStat + 2 * 5 * NR * 4;  // [4 warps][NR] maxima
-  static constexpr int kSmem = kMax + 4 * NR * 4;
+  static constexpr int kSums = kMax + 4 * NR * 4;        // [NR][128] each softmax thread's sums
+  static constexpr int kSmem = kSums + NR * 128 * 4;
   static constexpr int kBlocks = D / 128;     // M blocks of O^T
   static constexpr int kO = 2 * NR;           // TMEM: S^T [2][NR], then O^T [2][kBlocks][NR]
 };
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int64_t* s_scan = reinterpret_cast<int64_t*>(sm + Sh::kBar + 264);  // [2 warps + 4]
   int* s_first = reinterpret_cast<int*>(s_scan + 2 * (kThreads / 32) + 4);  // [4]
   volatile int* s_armed = s_first + 4;  // [NST]
-  static_assert((2 * NST + 20) * 8 <= 264 && 264 + (kThreads / 32 + 2) * 8 + (4 + NST) * 4 <= 512, "barrier area");
+  static_assert((2 * NST + 18) * 8 <= 264 && 264 + (2 * (kThreads / 32) + 4) * 8 + (4 + NST) * 4 <= 576, "barrier area");
   float* s_sum = reinterpret_cast<float*>(sm + Sh::kStat);
   float* s_ref = s_sum + 2 * 4 * NR;
   float* s_max = reinterpret_cast<float*>(sm + Sh::kMax);
@@ -223,31 +224,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quad = warp & 3, at = quad * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
     const float c = A.scale_log2;
-    // Rows in blocks of 4, and of those only the ones that the row tile has: with
-    // 4 rows of 16 the rest would be most of the instructions.
-    float ref[NR], l[NR];  // log2 units; a row that has seen nothing yet refers to -1e30
+    // Rows in blocks of 4, of which a row tile has one to four; the loops over them
+    // stay rolled and what they carry (references, sums) in shared memory: unrolled,
+    // the kernel had 116 KB of code and waited for instructions first of all.
+    float* const sum = reinterpret_cast<float*>(sm + Sh::kSums) + at;  // + r * 128
+    float* ref = s_ref;  // log2 units, the row tile's; a row that has seen nothing yet refers to -1e30
     int k = w.k0, item = 0, rows = 0;
-    auto each = [&](auto f) {
-#pragma unroll
-      for (int r0 = 0; r0 < NR; r0 += 4)
-        if (r0 < rows) {
-#pragma unroll
-          for (int r = r0; r < r0 + 4; ++r) f(r);
-        }
-    };
+    auto meet = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
     auto enter = [&] {
       rows = min(A.tp, w.s.n - w.rt * A.tp) * A.G;
-#pragma unroll
-      for (int r = 0; r < NR; ++r) ref[r] = -1e30f, l[r] = 0.f;
+      ref = s_ref + (item & 1) * NR;
+      if (item >= 2) wait_warp(&o_free[item & 1], ((item - 2) >> 1) & 1);
+      if (at < NR) ref[at] = -1e30f;
+#pragma unroll 1
+      for (int r = 0; r < rows; ++r) sum[r * 128] = 0.f;
+      meet();
     };
     enter();
 #pragma unroll 1
     for (int g = 0; g < N; ++g) {
       const int buf = g & 1, p0 = k * kTile;
       const int lim0 = w.s.len - w.s.n + w.rt * A.tp;  // the last position the first row sees
+      const bool masked = p0 + kTile - 1 > lim0;
       wait_warp(&s_full[buf], (g >> 1) & 1);
-      float s[NR];
-      tc::tmem_ld16(tb + buf * NR + lane_off, s);
       if (p0 + kTile > w.s.len) {  // slots behind the sequence: their V rows become zero
         const int first = max(0, w.s.len - p0);
         // O^T of tile g - 1 is done, so every earlier load of V(g)'s stages is over:
@@ -261,16 +260,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc::fence_async_smem();
       }
-      each([&](int r) { s[r] *= c; });
-      if (p0 + kTile - 1 > lim0) {
+      // f(r, scores of rows r .. r + 3)
+      auto each = [&](auto f) {
         int lim = lim0 - (p0 + at), n = 0;  // >= 0: this position is seen by the row
-        each([&](int r) {
-          s[r] = lim >= 0 ? s[r] : -INFINITY;
-          if (++n == A.G) n = 0, ++lim;
-        });
-      }
+#pragma unroll 1
+        for (int r = 0; r < rows; r += 4) {
+          float s[4];
+          tc::tmem_ld4(tb + buf * NR + lane_off + r, s);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[i] *= c;
+            if (masked) {
+              s[i] = lim >= 0 ? s[i] : -INFINITY;
+              if (++n == A.G) n = 0, ++lim;
+            }
+          }
+          f(r, s);
+        }
+      };
       bool over = false;
-      each([&](int r) { over |= s[r] - ref[r] > kLazy; });
+      each([&](int r, const float(&s)[4]) {
+        const float4 m = *reinterpret_cast<const float4*>(ref + r);
+        over |= s[0] - m.x > kLazy || s[1] - m.y > kLazy || s[2] - m.z > kLazy || s[3] - m.w > kLazy;
+      });
       uint32_t any;
       asm volatile(
           "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.or.pred q, 1, 128, p;\n selp.u32 %0, 1, 0, q;\n}"
@@ -278,44 +290,60 @@ __global__ void __launch_bounds__(kThreads, 1)
           : "r"((uint32_t)over)
           : "memory");
       if (any) {  // some row's reference moves: the rows' maxima over the tile
-        each([&](int r) {
-          float m = s[r];
+        each([&](int r, const float(&s)[4]) {
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          if (lane == 0) s_max[quad * NR + r] = m;
-        });
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        float corr[NR];
+          for (int i = 0; i < 4; ++i) {
+            float m = s[i];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) corr[r] = 1.0f;
-        each([&](int r) {
-          const float m = fmaxf(fmaxf(s_max[r], s_max[NR + r]), fmaxf(s_max[2 * NR + r], s_max[3 * NR + r]));
-          const bool move = m - ref[r] > kLazy;
-          corr[r] = move ? ex2(ref[r] - m) : 1.0f;
-          ref[r] = move ? m : ref[r];
-          l[r] *= corr[r];
-        });
-        if (k > w.k0) {
-          wait_warp(&p_free[buf ^ 1], ((g - 1) >> 1) & 1);
-#pragma unroll 1
-          for (int blk = 0; blk < NB; ++blk) {
-            float o[NR];
-            tc::tmem_ld16(o_at(item, blk) + lane_off, o);
-#pragma unroll
-            for (int r = 0; r < NR; ++r) o[r] *= corr[r];
-            tc::tmem_st16(o_at(item, blk) + lane_off, o);
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (lane == 0) s_max[quad * NR + r + i] = m;
           }
-          tc::tmem_st_wait();
+        });
+        meet();
+        auto top_of = [&](int r) {
+          return fmaxf(fmaxf(s_max[r], s_max[NR + r]), fmaxf(s_max[2 * NR + r], s_max[3 * NR + r]));
+        };
+        const bool begun = k > w.k0;
+        if (begun) wait_warp(&p_free[buf ^ 1], ((g - 1) >> 1) & 1);
+#pragma unroll 1
+        for (int r = 0; r < rows; r += 4) {
+          float corr[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float m = top_of(r + i), was = ref[r + i];
+            corr[i] = m - was > kLazy ? ex2(was - m) : 1.0f;
+            sum[(r + i) * 128] *= corr[i];
+          }
+          if (begun) {
+#pragma unroll 1
+            for (int blk = 0; blk < NB; ++blk) {
+              float o[4];
+              tc::tmem_ld4(o_at(item, blk) + lane_off + r, o);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[i] *= corr[i];
+              tc::tmem_st4(o_at(item, blk) + lane_off + r, o);
+            }
+          }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");  // the maxima have been read
+        tc::tmem_st_wait();
+        meet();  // all have read the references
+        if (at < rows) {
+          const float m = top_of(at);
+          if (m - ref[at] > kLazy) ref[at] = m;
+        }
+        meet();
       }
       if (g >= 2) wait_warp(&p_free[buf], ((g - 2) >> 1) & 1);
-      uint8_t* pw = sm + 2 * Sh::kQ + buf * Sh::kP + (at >> 6) * NR * 128 + (at & 7) * 2;
+      uint8_t* const pw = sm + 2 * Sh::kQ + buf * Sh::kP + (at >> 6) * NR * 128 + (at & 7) * 2;
       const int ch = (at & 63) >> 3;
-      each([&](int r) {
-        const float x = ex2(s[r] - ref[r]);
-        l[r] += x;
-        *reinterpret_cast<T*>(pw + r * 128 + ((ch ^ (r & 7)) << 4)) = from_float<T>(x);
+      each([&](int r, const float(&s)[4]) {
+        const float4 m = *reinterpret_cast<const float4*>(ref + r);
+        const float x[4] = {ex2(s[0] - m.x), ex2(s[1] - m.y), ex2(s[2] - m.z), ex2(s[3] - m.w)};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sum[(r + i) * 128] += x[i];
+          *reinterpret_cast<T*>(pw + (r + i) * 128 + ((ch ^ ((r + i) & 7)) << 4)) = from_float<T>(x[i]);
+        }
       });
       tc::fence_async_smem();
       tc::tc_fence_before();
@@ -323,23 +351,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) tc::mbar_arrive(&p_full[buf]);
       if (++k < w.k1) continue;
 
-      // ---- the row tile's last KV tile here: sums over this warp's positions, row r's in lane r (and r + 16) ----
-      if (item >= 2) wait_warp(&o_free[item & 1], ((item - 2) >> 1) & 1);
+      // ---- the row tile's last KV tile here: sums over this warp's positions ----
+#pragma unroll 1
+      for (int r = 0; r < rows; ++r) {
+        float l = sum[r * 128];
 #pragma unroll
-      for (int r = 0; r < NR; ++r) l[r] += __shfl_xor_sync(0xffffffffu, l[r], 16);
-#pragma unroll
-      for (int o = NR / 2; o > 0; o >>= 1) {
-#pragma unroll
-        for (int r = 0; r < o; ++r) {
-          const float keep = lane & o ? l[r + o] : l[r], send = lane & o ? l[r] : l[r + o];
-          l[r] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-        }
-      }
-      if (lane < NR) s_sum[((item & 1) * 4 + quad) * NR + lane] = l[0];
-      if (quad == 0) {
-#pragma unroll
-        for (int r = 0; r < NR; ++r)
-          if (lane == r) s_ref[(item & 1) * NR + r] = ref[r];
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (lane == 0) s_sum[((item & 1) * 4 + quad) * NR + r] = l;
       }
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&stats[item & 1]);
@@ -396,36 +414,35 @@ __global__ void __launch_bounds__(kThreads, 1)
       float* part = parts + ((size_t)cta * 2 + slot) * part_floats<D>();
 #pragma unroll 1
       for (int blk = 0; blk < NB; ++blk) {
-        T gate[NR];
-        if (A.gate && whole) {
-          const uint8_t* gp = A.gate + row0 * A.g_row + (int64_t)w.h * A.G * A.g_head + (blk * 128 + dim) * 2;
-          int n = 0;
+        const uint8_t* gp = A.gate + row0 * A.g_row + (int64_t)w.h * A.G * A.g_head + (blk * 128 + dim) * 2;
+        T* op = reinterpret_cast<T*>(A.out) + ((int64_t)row0 * heads + w.h * A.G) * D + blk * 128 + dim;
+        int ng = 0, no = 0;  // head of the group: of gp, of op
+#pragma unroll 1
+        for (int r = 0; r < rows; r += 4) {
+          T gate[4];
+          if (A.gate && whole) {
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            if (r < rows) {
-              gate[r] = *reinterpret_cast<const T*>(gp);
+            for (int i = 0; i < 4; ++i) {
+              if (r + i < rows) gate[i] = *reinterpret_cast<const T*>(gp);
               gp += A.g_head;
-              if (++n == A.G) n = 0, gp += A.g_row - A.G * A.g_head;
+              if (++ng == A.G) ng = 0, gp += A.g_row - A.G * A.g_head;
             }
           }
-        }
-        float o[NR];
-        tc::tmem_ld16(o_at(item, blk) + lane_off, o);
-        T* op = reinterpret_cast<T*>(A.out) + ((int64_t)row0 * heads + w.h * A.G) * D + blk * 128 + dim;
-        float* pp = part + blk * 128 + dim;
-        int n = 0;
+          float o[4];
+          tc::tmem_ld4(o_at(item, blk) + lane_off + r, o);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          if (r < rows) {
+          for (int i = 0; i < 4; ++i) {
+            if (r + i >= rows) break;
             if (whole) {
-              const float lt = (sums[r] + sums[NR + r]) + (sums[2 * NR + r] + sums[3 * NR + r]);
-              float x = lt == 0.f ? 0.f : __fdividef(o[r], lt);
-              if (A.gate) x = __fdividef(x, 1.0f + __expf(-to_float(gate[r])));
+              const float* l = sums + r + i;
+              const float lt = (l[0] + l[NR]) + (l[2 * NR] + l[3 * NR]);
+              float x = lt == 0.f ? 0.f : __fdividef(o[i], lt);
+              if (A.gate) x = __fdividef(x, 1.0f + __expf(-to_float(gate[i])));
               *op = from_float<T>(x);
               op += D;
-              if (++n == A.G) n = 0, op += (int64_t)(heads - A.G) * D;
+              if (++no == A.G) no = 0, op += (int64_t)(heads - A.G) * D;
             } else {
-              pp[r * D] = o[r];
+              part[(r + i) * D + blk * 128 + dim] = o[i];
             }
           }
         }
