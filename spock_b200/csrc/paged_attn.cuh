@@ -55,6 +55,7 @@ __host__ __device__ constexpr size_t meta_bytes(int ctas) { return ((size_t)ctas
 // Bounded wait for a phase, by one thread; gives up at once when another role has
 // (*fail), and says so to the others when it does itself.
 static __device__ __noinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* fail) {
+#pragma unroll 1
   for (uint32_t i = 0; i < kWait; ++i) {
     uint32_t ok;
     asm volatile(
@@ -80,15 +81,20 @@ __device__ __forceinline__ Seq load_seq(const AttnArgs& A, int b, bool report) {
   const int hi = A.start[b + 1];
   s.n = hi - s.lo;
   s.len = A.kv_len[b];
-  if (s.lo < 0 || hi < s.lo || hi > A.total) {
-    if (report) report_bad_index(A.err);
-    s.n = 0;
-  }
-  if (s.len < 0 || s.len > A.table_width * A.page_size) {
-    if (report) report_bad_index(A.err);
-    s.len = 0;
-  }
+  const bool bad_n = s.lo < 0 || hi < s.lo || hi > A.total, bad_len = s.len < 0 || s.len > A.table_width * A.page_size;
+  if (report && (bad_n || bad_len)) report_bad_index(A.err);
+  if (bad_n) s.n = 0;
+  if (bad_len) s.len = 0;
   return s;
+}
+// inclusive sums of a and b over the warp's lanes
+__device__ __forceinline__ void warp_sums(int64_t& a, int64_t& b) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, a, o), z = __shfl_up_sync(0xffffffffu, b, o);
+    if (lane >= o) a += y, b += z;
+  }
 }
 
 // A role's way through the CTA's units. The sequence after the current one is
@@ -154,26 +160,22 @@ static __device__ __noinline__ int enter_share(const AttnArgs& A, int64_t* scan,
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x, ctas = gridDim.x;
   const int per = (A.batch + kThreads - 1) / kThreads;
   int64_t mine = 0, rts = 0;  // KV tiles, row tiles
+#pragma unroll 1
   for (int b = tid * per; b < min(A.batch, (tid + 1) * per); ++b) {
     const Seq s = load_seq(A, b, cta == 0);
     mine += sched::head_units(s.n, s.len, A.tp) * A.kv_heads;
     rts += (int64_t)sched::row_tiles(s.n, A.tp) * A.kv_heads;
   }
   int64_t incl = mine, rincl = rts;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o), z = __shfl_up_sync(0xffffffffu, rincl, o);
-    if (lane >= o) incl += y, rincl += z;
-  }
+  warp_sums(incl, rincl);
   if (lane == 31) scan[warp] = incl, scan[W + warp] = rincl;
   __syncthreads();
-  int64_t base = 0, units = 0, rbase = 0, rall = 0;
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
-    if (i < warp) base += scan[i], rbase += scan[W + i];
-    units += scan[i];
-    rall += scan[W + i];
-  }
+  // the same over the warps, by each warp
+  int64_t w_incl = lane < W ? scan[lane] : 0, w_rincl = lane < W ? scan[W + lane] : 0;
+  warp_sums(w_incl, w_rincl);
+  int64_t units = __shfl_sync(0xffffffffu, w_incl, 31), base = __shfl_sync(0xffffffffu, w_incl, warp) - scan[warp];
+  const int64_t rall = __shfl_sync(0xffffffffu, w_rincl, 31);
+  const int64_t rbase = __shfl_sync(0xffffffffu, w_rincl, warp) - scan[W + warp];
   const int64_t all = units;  // KV tiles
   int extra = A.extra;
   if (units + extra * rall < (int64_t)ctas * 2 * (extra + 1)) extra = 0;
@@ -182,6 +184,7 @@ static __device__ __noinline__ int enter_share(const AttnArgs& A, int64_t* scan,
   const int64_t rfrom = rbase + rincl - rts, from = base + incl + extra * (rbase + rincl) - mine;
   const int shares = units < ctas ? (int)units : ctas;
   if (cta >= shares) return 0;
+  const int64_t share = sched::share_begin(units, 1, shares);
   int64_t* border = scan + 2 * W;  // [2], then the KV tiles before them [2]
   if (tid < 2) {
     border[tid] = sched::share_begin(units, cta + tid, shares);
@@ -209,7 +212,7 @@ static __device__ __noinline__ int enter_share(const AttnArgs& A, int64_t* scan,
       const int nt = sched::row_tile_units(s.n, s.len, A.tp, rt), all_of = nt + extra;
       rt_before += rt;
       int64_t at = r;  // of the row tile's units
-      if (A.whole && u > 0 && 2 * all_of <= units / shares) at = 2 * r <= all_of ? 0 : all_of;
+      if (A.whole && u > 0 && 2 * all_of <= share) at = 2 * r <= all_of ? 0 : all_of;
       const int k = max((int)at - extra, 0);
       if (i == 2) first[0] = b, first[1] = h, first[2] = rt, first[3] = k;
       border[i & 1] = u - r + at;

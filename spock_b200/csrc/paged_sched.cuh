@@ -18,25 +18,27 @@ namespace sched {
 
 constexpr int kTile = 128;
 
-// sum of floor((b + i a) / m) over i in [0, n): Euclid's steps on (a, m)
-__host__ __device__ __noinline__ inline int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+// sum of floor((b + i a) / m) over i in [0, n): Euclid's steps on (a, m), which
+// are at most 2^12 each, so that no division has 64 bits (those are long in code,
+// and this runs once per launch, when no instruction is cached yet)
+__host__ __device__ __noinline__ inline int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
   int64_t s = 0;
+#pragma unroll 1
   while (n > 0) {
     if (a >= m) {
-      s += n * (n - 1) / 2 * (a / m);
+      s += (int64_t)((uint64_t)n * (n - 1) / 2) * (a / m);
       a %= m;
     }
-    if (b >= m) {
-      s += n * (b / m);
-      b %= m;
-    }
-    const int64_t y = a * n + b;
-    if (y < m) break;
-    n = y / m;
-    b = y % m;
-    const int64_t t = a;
+    s += (int64_t)n * (b / m);
+    b %= m;
+    // y = a n + b = m (a (n / m)) + (a (n % m) + b)
+    const uint32_t low = a * (n % m) + b;
+    n = a * (n / m) + low / m;
+    b = low % m;
+    const uint32_t t = a;
     a = m;
     m = t;
+    if (n == 0) break;  // y < m
   }
   return s;
 }
@@ -44,30 +46,30 @@ __host__ __device__ __noinline__ inline int64_t floor_sum(int64_t n, int64_t m, 
 // KV tiles of row tile j of a sequence with n new tokens out of len positions
 __host__ __device__ inline int row_tile_units(int n, int len, int tp, int j) {
   const int64_t end = (int64_t)(j + 1) * tp;
-  const int64_t seen = (int64_t)len - n + (end < n ? end : n);
-  return seen <= kTile ? 1 : (int)((seen + kTile - 1) / kTile);
+  const int seen = len - n + (end < n ? (int)end : n);
+  return seen <= kTile ? 1 : (int)(((uint32_t)seen + kTile - 1) / kTile);
 }
 // the same summed over row tiles 0 .. j-1, none of them the last
-__host__ __device__ __noinline__ inline int64_t units_before(int n, int len, int tp, int64_t j) {
+__host__ __device__ __noinline__ inline int64_t units_before(int n, int len, int tp, int j) {
   if (j == 0) return 0;
-  const int64_t off = (int64_t)len - n;
-  int64_t j0 = off < 0 ? -off / tp : 0;  // row tiles that see nothing: one unit each
-  if (j0 > j) j0 = j;
-  if (j0 == j) return j0;
-  return j0 + floor_sum(j - j0, kTile, tp, off + (j0 + 1) * tp + kTile - 1);
+  const int off = len - n;
+  int j0 = off < 0 ? -off / tp : 0;  // row tiles that see nothing: one unit each
+  if (j0 >= j) return j;
+  return j0 + floor_sum(j - j0, kTile, tp, (uint32_t)off + (uint32_t)(j0 + 1) * tp + kTile - 1);
 }
+__host__ __device__ inline int row_tiles(int n, int tp) { return n <= 0 ? 0 : (n + tp - 1) / tp; }
 __host__ __device__ inline int64_t head_units(int n, int len, int tp) {
   if (n <= 0) return 0;
-  const int last = (n + tp - 1) / tp - 1;
+  const int last = row_tiles(n, tp) - 1;
   if (last == 0) return row_tile_units(n, len, tp, 0);
   return units_before(n, len, tp, last) + row_tile_units(n, len, tp, last);
 }
-__host__ __device__ inline int row_tiles(int n, int tp) { return n <= 0 ? 0 : (n + tp - 1) / tp; }
 // the row tile that unit r of a head falls into (r becomes the unit within it),
 // each with `extra` units before its KV tiles
 __host__ __device__ inline int find_row_tile(int n, int len, int tp, int extra, int64_t& r) {
   int lo = 0, hi = row_tiles(n, tp) - 1;
   if (hi == 0) return 0;
+#pragma unroll 1
   while (lo < hi) {
     const int mid = lo + (hi - lo + 1) / 2;
     if (units_before(n, len, tp, mid) + (int64_t)extra * mid <= r)
@@ -79,9 +81,12 @@ __host__ __device__ inline int find_row_tile(int n, int len, int tp, int extra, 
   return lo;
 }
 
+// units c / shares, in divisions of 32 bits: units < 2^51, shares <= 2^12
 __host__ __device__ inline int64_t share_begin(int64_t units, int c, int shares) {
-  if (units < (1 << 20) && shares <= 1024) return (uint32_t)units * (uint32_t)c / (uint32_t)shares;  // fits 32 bits
-  return units * c / shares;
+  const uint32_t hi = (uint32_t)(units >> 20), lo = (uint32_t)units & 0xfffffu, m = (uint32_t)shares;
+  const uint32_t low = hi % m << 20 | lo;
+  const int64_t q = (int64_t)(hi / m) << 20 | low / m;
+  return q * c + low % m * (uint32_t)c / m;
 }
 
 }  // namespace sched
