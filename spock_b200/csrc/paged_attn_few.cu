@@ -2,19 +2,22 @@
 // the tensor-core tile turned over.
 //
 // With 128 query rows on the M side (paged_attn_tc.cu) a decode token's 4 rows
-// would leave 124 lanes of every softmax and output instruction idle: it was
-// bound by those (133 us for 256 sequences), not by the cache it reads. Here M is
-// the cache's side, and N the rows, 16:
+// would leave 124 lanes of every softmax and output instruction idle (93 us for
+// 256 sequences of 65 to 1150 positions, and 74 here). Here M is the cache's side,
+// and N the rows, 16:
 //   S^T = K Q^T   M = 128 positions  N = rows  K = head dims
 //   O^T += V^T P^T  M = 128 dims (twice at head size 256)  N = rows  K = positions
 // K and V come straight from their tiles as the A operands (V M-major), the
 // queries and the weights are the small B operands in shared memory. A softmax
-// thread holds one position's scores of all rows; no maximum crosses lanes unless
-// a score exceeds its row's reference by 2^8, which one barrier with a vote finds
-// out for the block. O^T has dims on the lanes, so outputs and gates are read and
-// written in whole rows. Bound by the cache's bytes: an SM streams a tile (128
-// positions, 128 KB at head size 256) in some 5700 cycles of HBM's time, its MMAs
-// take 2300.
+// thread takes one position's scores, four rows at a time; no maximum crosses
+// lanes unless a score exceeds its row's reference by 2^8, which one barrier with
+// a vote finds out for the block. O^T has dims on the lanes, so outputs and gates
+// are read and written in whole rows. Meant to be bound by the cache's bytes: an
+// SM streams a tile (128 positions, 128 KB at head size 256) in some 5700 cycles
+// of HBM's time, its MMAs take 2300. The 256 sequences take 1.5 times those bytes'
+// time: starting, the last tiles and the join are some 15 us, and the ring holds
+// little more than one tile, so every wait on the way shows. Separate rings for K
+// and V (3 + 3 or 4 + 2 stages) were slower (81 and 83 us).
 //
 // One CTA per SM walks its share (paged_attn.cuh). Warp roles:
 //   warps 0, 3  K tiles and V tiles by TMA into a ring

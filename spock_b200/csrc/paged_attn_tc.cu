@@ -22,12 +22,22 @@
 // unnormalised O (fp32), maximum and sum in the workspace, and
 // paged_join_kernel adds the parts in order (no atomics: results repeat).
 //
+// Bound, at head size 256 with long sequences, by the K and V tiles' way from L2
+// and the one and a quarter tiles that the ring holds: 2048 tokens of 8 heads over
+// 16384 positions take 260 us, 0.58 of the measured rate of large matrix products;
+// of a tile's 3900 cycles the MMAs take 2100, the softmax 2000 beside them, and
+// 1700 are waits for tiles. At head size 128 with short prompts (8 of 301 to 1021
+// tokens: 68 us) by starting and finishing row tiles of some three KV tiles each.
+// The MMA thread is the one elected by the warp: the same code under `lane == 0`
+// goes through a loop over the lanes for each descriptor (333 us instead of 285).
+//
 // Slots behind kv_len may hold anything: their scores are masked, and their V
 // rows are zeroed in shared memory, since 0 * NaN would reach every row.
 // Every wait is bounded; one that gives up sets the context's error word, and
 // the CTA lets its copies and MMAs land, frees its TMEM and leaves.
 #include <cuda.h>
 
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 
@@ -441,17 +451,18 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   constexpr int V = D / 32, kMany = 12;
   const int cta = blockIdx.x, ctas = gridDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   __shared__ float s_o[8][D];
-  __shared__ float s_l[8];
+  __shared__ float s_l[8], s_m[8];
   pdl_wait();
   pdl_launch();
   const Meta* meta = reinterpret_cast<const Meta*>(A.ws);
+  const int after = cta + 1 + lane < ctas ? meta[cta + 1 + lane].units : 0;  // on its way with the next
   const Meta mt = meta[cta];
   if (mt.slot < 0) return;
   const float* parts = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(A.ws) + meta_bytes(ctas));
   // the shares that hold parts: 32 at a time, until their units cover the row tile
   int n = 1;
   for (int have = mt.have; have < mt.nt && cta + n < ctas;) {
-    int u = cta + n + lane < ctas ? meta[cta + n + lane].units : 0;
+    int u = n == 1 ? after : cta + n + lane < ctas ? meta[cta + n + lane].units : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, u, o);
@@ -469,12 +480,76 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   auto part = [&](int i) {
     return parts + ((size_t)(cta + i) * 2 + (i == 0 ? mt.slot : 0)) * part_floats<D>();
   };
-  auto finish = [&](int r, float (&acc)[V], float l) {
+  // parts i0, i0 + step, .. < n of row r, four in flight; l and acc relative to the running maximum m
+  auto add = [&](int i0, int step, int r, float& m, float (&acc)[V], float& l) {
+    constexpr int U = 4;
+#pragma unroll 1
+    for (int i = i0; i < n; i += U * step) {
+      float mi[U], li[U], x[U][V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int j = i + u * step;
+        mi[u] = -INFINITY;
+        if (j < n) {
+          const float* p = part(j);
+          mi[u] = p[128 * D + r];
+          li[u] = p[128 * D + 128 + r];
+#pragma unroll
+          for (int v = 0; v < V; v += 2) {
+            const float2 y = *reinterpret_cast<const float2*>(p + r * D + lane * V + v);
+            x[u][v] = y.x, x[u][v + 1] = y.y;
+          }
+        }
+      }
+      const float to = fmaxf(fmaxf(fmaxf(mi[0], mi[1]), fmaxf(mi[2], mi[3])), m);
+      if (to > m) {
+        const float f = ex2(m - to);
+        l *= f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] *= f;
+        m = to;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (mi[u] > -INFINITY) {  // a part that saw nothing may hold anything
+          const float f = ex2(mi[u] - m);
+          l = fmaf(f, li[u], l);
+          if (f != 0.f) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[v] = fmaf(f, x[u][v], acc[v]);
+          }
+        }
+    }
+  };
+  const bool many = n > kMany;
+#pragma unroll 1
+  for (int r = many ? blockIdx.y : blockIdx.y * 8 + warp; r < mt.rows; r += many ? gridDim.y : gridDim.y * 8) {
     const int tt = r / A.G, hq = mt.head * A.G + r - tt * A.G;
     const int64_t tok = mt.row0 + tt;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
     uint32_t w[V / 2], gw[V / 2];
     if (A.gate) load_words(A.gate + tok * A.g_row + hq * A.g_head + lane * V * 2, gw);
+    float m = -INFINITY, acc[V] = {}, l = 0.f;
+    add(many ? warp : 0, many ? 8 : 1, r, m, acc, l);
+    if (many) {
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < V; ++v) s_o[warp][lane * V + v] = acc[v];
+      if (lane == 0) s_m[warp] = m, s_l[warp] = l;
+      __syncthreads();
+      if (warp) continue;
+      float to = s_m[0];
+      for (int k = 1; k < 8; ++k) to = fmaxf(to, s_m[k]);
+      l = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = 0.f;
+      for (int k = 0; k < 8; ++k) {
+        const float f = s_m[k] > -INFINITY ? ex2(s_m[k] - to) : 0.f;
+        l = fmaf(f, s_l[k], l);
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] = fmaf(f, s_o[k][lane * V + v], acc[v]);
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
     for (int e = 0; e < V / 2; ++e) {
       float a = acc[2 * e] * inv, b = acc[2 * e + 1] * inv;
@@ -486,65 +561,6 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
       w[e] = Io<T>::down2(a, b);
     }
     store_words(A.out + (tok * (A.kv_heads * A.G) + hq) * (D * 2) + lane * V * 2, w);
-  };
-  // parts i0, i0 + step, .. < n of row r, relative to maximum m; four in flight
-  auto add = [&](int i0, int step, int r, float m, float (&acc)[V], float& l) {
-    constexpr int U = 4;
-    for (int i = i0; i < n; i += U * step) {
-      float f[U], x[U][V];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int j = i + u * step;
-        f[u] = 0.f;
-        if (j < n) {
-          const float* p = part(j);
-          const float mi = p[128 * D + r];
-          f[u] = mi == -INFINITY ? 0.f : ex2(mi - m);
-          l += f[u] * p[128 * D + 128 + r];
-#pragma unroll
-          for (int v = 0; v < V; v += 2) {
-            const float2 y = *reinterpret_cast<const float2*>(p + r * D + lane * V + v);
-            x[u][v] = y.x, x[u][v + 1] = y.y;
-          }
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (f[u] != 0.f) {  // a part that saw nothing (or nothing that counts) may hold anything
-#pragma unroll
-          for (int v = 0; v < V; ++v) acc[v] = fmaf(f[u], x[u][v], acc[v]);
-        }
-    }
-  };
-  const bool many = n > kMany;
-  for (int r = many ? blockIdx.y : blockIdx.y * 8 + warp; r < mt.rows; r += many ? gridDim.y : gridDim.y * 8) {
-    float m = -INFINITY;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, part(i)[128 * D + r]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float acc[V] = {}, l = 0.f;
-    if (!many) {
-      add(0, 1, r, m, acc, l);
-      finish(r, acc, l);
-      continue;
-    }
-    add(warp, 8, r, m, acc, l);
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < V; ++v) s_o[warp][lane * V + v] = acc[v];
-    if (lane == 0) s_l[warp] = l;
-    __syncthreads();
-    if (warp == 0) {
-      l = 0.f;
-#pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] = 0.f;
-      for (int k = 0; k < 8; ++k) {
-        l += s_l[k];
-#pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] += s_o[k][lane * V + v];
-      }
-      finish(r, acc, l);
-    }
   }
 }
 
@@ -626,7 +642,7 @@ Status launch(const spock_paged_kv& kv, AttnArgs& A, bool few, int sms, cudaStre
     SPOCK_LAUNCH_CHECK("paged_attn_kernel");
   }
   pdl_scope overlap;  // the join's launch runs under the main kernel
-  e = launch_k(paged_join_kernel<T, D>, dim3(sms, 4), dim3(256), 0, st, A);
+  e = launch_k(paged_join_kernel<T, D>, dim3(sms, std::min(4, (A.tp * A.G + 7) / 8)), dim3(256), 0, st, A);
   if (e != cudaSuccess) return cuda_status(e, "paged_join_kernel");
   SPOCK_LAUNCH_CHECK("paged_join_kernel");
   return Status::ok();
@@ -666,9 +682,9 @@ Status launch_paged_attention(const spock_paged_kv& kv, int batch, const int32_t
   A.ws = (float*)ws;
   A.err = err;
   // Either kernel is right for every batch; the rows that a sequence brings on
-  // average decide. One token each over 256 sequences takes 102 us in the few-row
-  // kernel and 117 in the wide one; five tokens each (64 sequences) 92 in the wide
-  // one, and 113 in a few-row kernel of 32 rows, which is not kept. Head size 64
+  // average decide. One token each over 256 sequences takes 75 us in the few-row
+  // kernel and 93 in the wide one; five tokens each (64 sequences) 71 in the wide
+  // one, and 89 in a few-row kernel of 32 rows, which is not kept. Head size 64
   // would leave half of the few-row kernel's output tile empty.
   const bool few = kv.head_dim >= 128 && total <= batch && A.G <= kFewRows;
   if (kv.dtype == SPOCK_F16) {
