@@ -141,6 +141,27 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 }
 
 
+// The row tile that unit r of a head falls into, each with `extra` units before
+// its KV tiles (r becomes the unit within it), by all lanes of a warp: a search
+// in 32 parts, since one step costs up to 3000 cycles (with halves, and one
+// thread, 8 prompts spent 16 us in it).
+__device__ __forceinline__ int find_row_tile(int n, int len, int tp, int extra, int64_t& r) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = sched::row_tiles(n, tp) - 1;
+  int64_t before = 0;  // of row tile lo
+#pragma unroll 1
+  while (lo < hi) {
+    const int step = (hi - lo + 32) / 32, j = lo + lane * step;
+    const int64_t u = j <= hi ? sched::units_before(n, len, tp, j) + (int64_t)extra * j : 0;
+    const int at = __popc(__ballot_sync(0xffffffffu, j <= hi && u <= r)) - 1;  // >= 0: row tile lo is one of them
+    before = __shfl_sync(0xffffffffu, u, at);
+    lo += at * step;
+    hi = min(hi, lo + step - 1);
+  }
+  r -= before;
+  return lo;
+}
+
 // This CTA's share: the first row tile and KV tile in w; the KV tiles it has. All
 // threads (it synchronises). scan: 2 kThreads / 32 + 4 words, first: 4.
 //
@@ -191,15 +212,18 @@ static __device__ __noinline__ int enter_share(const AttnArgs& A, int64_t* scan,
     border[2 + tid] = all;  // of a border behind the last unit
   }
   __syncthreads();
-  // 0, 1: move the borders; 2: the first row tile
+  // Each border by the warp that holds it. The finder moves it (A.whole); both
+  // shares beside it come to the same place.
 #pragma unroll 1
-  for (int i = A.whole ? 0 : 1; i < 3; ++i) {
-    const int64_t u = border[i & 1];
-    if (A.whole) __syncthreads();  // all have read it before its finder moves it
-    if (from <= u && u < from + mine) {
-      int64_t r = u - from, rt_before = rfrom;
-      int b = tid * per, h = 0;
-      Seq s;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t u = border[i];
+    const bool finds = from <= u && u < from + mine;
+    const unsigned finder = __ballot_sync(0xffffffffu, finds);
+    if (!finder) continue;  // of all warps, one has it (none: behind the last unit)
+    int64_t r = u - from, rt_before = rfrom;
+    int b = tid * per, h = 0;
+    Seq s{0, 0, 0};
+    if (finds) {
 #pragma unroll 1
       for (;; ++b) {
         s = load_seq(A, b, false);
@@ -208,18 +232,37 @@ static __device__ __noinline__ int enter_share(const AttnArgs& A, int64_t* scan,
         for (h = 0; h < A.kv_heads && r >= hu; ++h) r -= hu, rt_before += tiles;
         if (h < A.kv_heads) break;
       }
-      const int rt = sched::find_row_tile(s.n, s.len, A.tp, extra, r);
+    }
+    const int who = __ffs(finder) - 1;
+    s.n = __shfl_sync(0xffffffffu, s.n, who);
+    s.len = __shfl_sync(0xffffffffu, s.len, who);
+    r = __shfl_sync(0xffffffffu, r, who);
+    int rt = find_row_tile(s.n, s.len, A.tp, extra, r);
+    if (finds) {
       const int nt = sched::row_tile_units(s.n, s.len, A.tp, rt), all_of = nt + extra;
       rt_before += rt;
       int64_t at = r;  // of the row tile's units
       if (A.whole && u > 0 && 2 * all_of <= share) at = 2 * r <= all_of ? 0 : all_of;
-      const int k = max((int)at - extra, 0);
-      if (i == 2) first[0] = b, first[1] = h, first[2] = rt, first[3] = k;
-      border[i & 1] = u - r + at;
-      border[2 + (i & 1)] = u - r - extra * rt_before + k;
+      int k = max((int)at - extra, 0);
+      border[2 + i] = u - r - extra * rt_before + k;
+      if (i == 0) {
+        if (k == nt) {  // the next row tile's begin
+          k = 0;
+          if (++rt == sched::row_tiles(s.n, A.tp)) {
+            rt = 0;
+            if (++h == A.kv_heads) {
+              h = 0;
+              do ++b;
+              while (b + 1 < A.batch && load_seq(A, b, false).n <= 0);
+              b = min(b, A.batch - 1);
+            }
+          }
+        }
+        first[0] = b, first[1] = h, first[2] = rt, first[3] = k;
+      }
     }
-    __syncthreads();
   }
+  __syncthreads();
   const int n = (int)(border[3] - border[2]);
   w.left = n;
   if (n > 0) {

@@ -18,11 +18,23 @@ namespace sched {
 
 constexpr int kTile = 128;
 
-// sum of floor((b + i a) / m) over i in [0, n): Euclid's steps on (a, m), which
-// are at most 2^12 each, so that no division has 64 bits (those are long in code,
-// and this runs once per launch, when no instruction is cached yet)
-__host__ __device__ __noinline__ inline int64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
-  int64_t s = 0;
+// sum of floor(j / p) over j in [0, x)
+__host__ __device__ inline int64_t steps_sum(uint32_t x, uint32_t p) {
+  const uint32_t k = x / p;
+  return (int64_t)((uint64_t)k * (k > 0 ? k - 1 : 0) / 2) * p + (int64_t)k * (x - k * p);
+}
+// sum of floor((b + i a) / kTile) over i in [0, n), a <= kTile, without divisions
+// of 64 bits. Where a divides kTile (group sizes that are powers of two) the terms
+// rise by one every kTile / a: floor((b + i a) / kTile) = floor((b / a + i) / (kTile / a)).
+// Otherwise Euclid's steps on (a, m), some 3000 cycles.
+__host__ __device__ __noinline__ inline int64_t floor_sum(uint32_t n, uint32_t a, uint32_t b) {
+  int64_t s = (int64_t)n * (b / kTile);
+  b %= kTile;
+  if (kTile % a == 0) {
+    const uint32_t c = b / a, p = kTile / a;
+    return s + steps_sum(c + n, p) - steps_sum(c, p);
+  }
+  uint32_t m = kTile;
 #pragma unroll 1
   while (n > 0) {
     if (a >= m) {
@@ -33,12 +45,11 @@ __host__ __device__ __noinline__ inline int64_t floor_sum(uint32_t n, uint32_t m
     b %= m;
     // y = a n + b = m (a (n / m)) + (a (n % m) + b)
     const uint32_t low = a * (n % m) + b;
-    n = a * (n / m) + low / m;
+    n = a * (n / m) + low / m;  // 0: y < m
     b = low % m;
     const uint32_t t = a;
     a = m;
     m = t;
-    if (n == 0) break;  // y < m
   }
   return s;
 }
@@ -55,7 +66,7 @@ __host__ __device__ __noinline__ inline int64_t units_before(int n, int len, int
   const int off = len - n;
   int j0 = off < 0 ? -off / tp : 0;  // row tiles that see nothing: one unit each
   if (j0 >= j) return j;
-  return j0 + floor_sum(j - j0, kTile, tp, (uint32_t)off + (uint32_t)(j0 + 1) * tp + kTile - 1);
+  return j0 + floor_sum(j - j0, tp, (uint32_t)off + (uint32_t)(j0 + 1) * tp + kTile - 1);
 }
 __host__ __device__ inline int row_tiles(int n, int tp) { return n <= 0 ? 0 : (n + tp - 1) / tp; }
 __host__ __device__ inline int64_t head_units(int n, int len, int tp) {
@@ -64,23 +75,6 @@ __host__ __device__ inline int64_t head_units(int n, int len, int tp) {
   if (last == 0) return row_tile_units(n, len, tp, 0);
   return units_before(n, len, tp, last) + row_tile_units(n, len, tp, last);
 }
-// the row tile that unit r of a head falls into (r becomes the unit within it),
-// each with `extra` units before its KV tiles
-__host__ __device__ inline int find_row_tile(int n, int len, int tp, int extra, int64_t& r) {
-  int lo = 0, hi = row_tiles(n, tp) - 1;
-  if (hi == 0) return 0;
-#pragma unroll 1
-  while (lo < hi) {
-    const int mid = lo + (hi - lo + 1) / 2;
-    if (units_before(n, len, tp, mid) + (int64_t)extra * mid <= r)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  r -= units_before(n, len, tp, lo) + (int64_t)extra * lo;
-  return lo;
-}
-
 // units c / shares, in divisions of 32 bits: units < 2^51, shares <= 2^12
 __host__ __device__ inline int64_t share_begin(int64_t units, int c, int shares) {
   const uint32_t hi = (uint32_t)(units >> 20), lo = (uint32_t)units & 0xfffffu, m = (uint32_t)shares;
