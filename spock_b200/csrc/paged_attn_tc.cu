@@ -77,6 +77,25 @@ struct Shape {
 };
 static_assert(Shape<256>::kSmem <= 227 * 1024 && Shape<128>::kSmem <= 227 * 1024, "shared memory of one SM");
 
+// x[v]: piece v of this lane's row -> piece (lane & 3) of row v of its 4 lanes; and back
+__device__ __forceinline__ void trade(uint32_t (&x)[4][4], int lane) {
+#pragma unroll
+  for (int b = 1; b <= 2; b <<= 1) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      if (v & b) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, lane & b ? x[v][e] : x[v | b][e], b);
+        if (lane & b)
+          x[v][e] = got;
+        else
+          x[v | b][e] = got;
+      }
+    }
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
@@ -369,34 +388,45 @@ __global__ void __launch_bounds__(kThreads, 1)
         pair_sync();  // read before the next tile's maxima go there
         if (whole) {
           const float inv = lt == 0.f ? 0.f : 1.0f / lt;
-          uint8_t* op = A.out + (tok * (A.kv_heads * A.G) + hq) * (D * 2) + half * D;
-          const uint8_t* gp = A.gate + tok * A.g_row + hq * A.g_head + half * D;
+          // 4 lanes trade their rows' 16-byte pieces, so that each store (and load of
+          // gates) has 64 bytes of a row beside each other, 8 rows and not 32 at a time
+          const int64_t op = (tok * (A.kv_heads * A.G) + hq) * (D * 2) + half * D;
+          const int64_t gp = tok * A.g_row + hq * A.g_head + half * D;
+          const int piece = (lane & 3) * 16, first = row & ~3;
+          int64_t ops[4], gps[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            ops[t] = __shfl_sync(0xffffffffu, op, (lane & ~3) + t) + piece;
+            gps[t] = __shfl_sync(0xffffffffu, gp, (lane & ~3) + t) + piece;
+          }
 #pragma unroll 1
           for (int cb = 0; cb < D / 64; ++cb) {
-            uint32_t gw[16];
-            if (A.gate && row < rows) {
+            uint32_t x[4][4];
+            if (A.gate) {
 #pragma unroll
-              for (int v = 0; v < 4; ++v) load_words(gp + cb * 64 + v * 16, reinterpret_cast<uint32_t(&)[4]>(gw[4 * v]));
+              for (int t = 0; t < 4; ++t)
+                if (first + t < rows) load_words(A.gate + gps[t] + cb * 64, x[t]);
+              trade(x, lane);
             }
             float o[32];
             tc::tmem_ld32(tO + lane_off + half * (D / 2) + cb * 32, o);
-            if (row < rows) {
 #pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                uint32_t x[4];
+            for (int v = 0; v < 4; ++v) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  float a = o[v * 8 + 2 * e] * inv, b = o[v * 8 + 2 * e + 1] * inv;
-                  if (A.gate) {
-                    const float2 z = Io<T>::up2(gw[v * 4 + e]);
-                    a = __fdividef(a, 1.0f + __expf(-z.x));
-                    b = __fdividef(b, 1.0f + __expf(-z.y));
-                  }
-                  x[e] = Io<T>::down2(a, b);
+              for (int e = 0; e < 4; ++e) {
+                float a = o[v * 8 + 2 * e] * inv, b = o[v * 8 + 2 * e + 1] * inv;
+                if (A.gate) {
+                  const float2 z = Io<T>::up2(x[v][e]);
+                  a = __fdividef(a, 1.0f + __expf(-z.x));
+                  b = __fdividef(b, 1.0f + __expf(-z.y));
                 }
-                store_words(op + cb * 64 + v * 16, x);
+                x[v][e] = Io<T>::down2(a, b);
               }
             }
+            trade(x, lane);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              if (first + t < rows) store_words(A.out + ops[t] + cb * 64, x[t]);
           }
         } else {
           float* part = parts + ((size_t)cta * 2 + slot) * part_floats<D>();
