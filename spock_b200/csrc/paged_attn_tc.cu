@@ -24,10 +24,10 @@
 //
 // Bound, at head size 256 with long sequences, by the K and V tiles' way from L2
 // and the one and a quarter tiles that the ring holds: 2048 tokens of 8 heads over
-// 16384 positions take 260 us, 0.58 of the measured rate of large matrix products;
+// 16384 positions take 245 us, 0.61 of the measured rate of large matrix products;
 // of a tile's 3900 cycles the MMAs take 2100, the softmax 2000 beside them, and
 // 1700 are waits for tiles. At head size 128 with short prompts (8 of 301 to 1021
-// tokens: 68 us) by starting and finishing row tiles of some three KV tiles each.
+// tokens: 58 us) by starting and finishing row tiles of some three KV tiles each.
 // The MMA thread is the one elected by the warp: the same code under `lane == 0`
 // goes through a loop over the lanes for each descriptor (333 us instead of 285).
 //
@@ -712,8 +712,8 @@ Status launch_paged_attention(const spock_paged_kv& kv, int batch, const int32_t
   A.ws = (float*)ws;
   A.err = err;
   // Either kernel is right for every batch; the rows that a sequence brings on
-  // average decide. One token each over 256 sequences takes 75 us in the few-row
-  // kernel and 93 in the wide one; five tokens each (64 sequences) 71 in the wide
+  // average decide. One token each over 256 sequences takes 74 us in the few-row
+  // kernel and 93 in the wide one; five tokens each (64 sequences) 70 in the wide
   // one, and 89 in a few-row kernel of 32 rows, which is not kept. Head size 64
   // would leave half of the few-row kernel's output tile empty.
   const bool few = kv.head_dim >= 128 && total <= batch && A.G <= kFewRows;
