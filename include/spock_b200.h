@@ -346,7 +346,9 @@ int spock_paged_attention_prep(spock_ctx* ctx, const spock_paged_kv* kv, int32_t
 /* Attention of each sequence's new tokens over its pages: token t of n sees
  * positions 0 .. kv_len - n + t (causal; none if that is negative: the row is
  * then zero), q_heads a multiple of kv_heads, at most 128 query heads per kv
- * head. One entry for decode tokens, drafts, prompt chunks and any mix.
+ * head. One entry for decode tokens, drafts, prompt chunks and any mix; the
+ * kernel is chosen by total against batch, so a prompt chunk runs slower in a
+ * batch that is mostly sequences without new tokens.
  *   out[r][h] = sum_p softmax_p(scale * q[r][h] . k_p) v_p, times
  *   sigmoid(gate[r][h]) when gate is not NULL; rounded once
  *   q, gate rows and heads at their own strides (elements, multiples of 8;
