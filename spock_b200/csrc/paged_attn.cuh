@@ -40,7 +40,7 @@ struct Meta {
   int head;      // kv head
   int have, nt;  // KV tiles done here, in all
   int units;     // of this CTA
-  int pad;
+  int before;    // KV tiles of its first row tile that are in earlier CTAs
 };
 template <int D>
 __host__ __device__ constexpr size_t part_floats() {

@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   if (N == 0) {
-    if (tid == 0) meta[cta].slot = -1, meta[cta].units = 0;
+    if (tid == 0) meta[cta].slot = -1, meta[cta].units = 0, meta[cta].before = 0;
   } else if (warp == 0) {
     load_tiles<false, D, NST, Sh::kStage>(tmk, A, w, N, sm + Sh::kRing, full, empty, s_armed, wait);
   } else if (warp == 1) {
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     load_q(0);
     if (more) load_q(1);
-    if (tid == 256) meta[cta].slot = -1, meta[cta].units = N;
+    if (tid == 256) meta[cta].slot = -1, meta[cta].units = N, meta[cta].before = w.k0;
     for (int item = 0;; ++item) {
       const int t0 = w.rt * A.tp, rows = min(A.tp, w.s.n - t0) * A.G, row0 = w.s.lo + t0;
       const bool whole = w.k0 == 0 && w.k1 == w.nt;

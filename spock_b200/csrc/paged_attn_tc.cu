@@ -37,7 +37,6 @@
 // the CTA lets its copies and MMAs land, frees its TMEM and leaves.
 #include <cuda.h>
 
-#include <algorithm>
 #include <atomic>
 #include <mutex>
 
@@ -170,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_for(tc::smem_u32(bar), parity, s_fail); };
 
   if (N == 0) {
-    if (tid == 0) meta[cta].slot = -1, meta[cta].units = 0;
+    if (tid == 0) meta[cta].slot = -1, meta[cta].units = 0, meta[cta].before = 0;
   } else if (warp == 0) {
     load_tiles<false, D, NST, Sh::kStage>(tmk, A, w, N, sm + Sh::kQ, full, empty, s_armed, wait);
   } else if (warp == 2) {
@@ -268,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::tc_fence_after();
     };
     auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory"); };
-    if (tid == 128) meta[cta].slot = -1, meta[cta].units = N;
+    if (tid == 128) meta[cta].slot = -1, meta[cta].units = N, meta[cta].before = w.k0;
     float m = -INFINITY, l = 0.f;
     int k = 0, item = 0;
     int t0 = 0, rows = 0, lim = 0, lim0 = 0;
@@ -472,10 +471,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the parts of the row tile that begins in share blockIdx.x and ends in a
-// later one, in share order: o = sum 2^{m_i - m} O_i / sum 2^{m_i - m} l_i.
-// Rows are dealt to the blockIdx.y blocks. Few parts: a warp per row; many (a
-// long sequence over the whole GPU): the block's 8 warps share each row's.
+// Joins the parts of each cut row tile, in share order: o = sum 2^{m_i - m} O_i /
+// sum 2^{m_i - m} l_i. The blocks of all its n shares (blockIdx.x) do it, the rows
+// dealt to the n gridDim.y of them: the one that continues in a share, then the
+// one that begins there. (With the first share's blocks alone, a call that ends in
+// 12 row tiles of 13 parts and 128 rows took 80 us, and 46 so.) Few parts: a warp
+// per row; many (a long sequence over the whole GPU): the block's 8 warps share
+// each row's.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ AttnArgs A) {
   constexpr int V = D / 32, kMany = 12;
@@ -485,112 +487,120 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   pdl_wait();
   pdl_launch();
   const Meta* meta = reinterpret_cast<const Meta*>(A.ws);
-  const int after = cta + 1 + lane < ctas ? meta[cta + 1 + lane].units : 0;  // on its way with the next
-  const Meta mt = meta[cta];
-  if (mt.slot < 0) return;
   const float* parts = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(A.ws) + meta_bytes(ctas));
-  // the shares that hold parts: 32 at a time, until their units cover the row tile
-  int n = 1;
-  for (int have = mt.have; have < mt.nt && cta + n < ctas;) {
-    int u = n == 1 ? after : cta + n + lane < ctas ? meta[cta + n + lane].units : 0;
+  // shares from `at` on (by dir), 32 at a time, until their units cover `want`: how many
+  auto cover = [&](int at, int dir, int want) -> int {
+    int n = 0;
+    for (int have = 0; have < want && at >= 0 && at < ctas;) {
+      const int i = at + dir * lane;
+      int u = i >= 0 && i < ctas ? meta[i].units : 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, u, o);
-      if (lane >= o) u += y;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, u, o);
+        if (lane >= o) u += y;
+      }
+      const unsigned enough = __ballot_sync(0xffffffffu, have + u >= want);
+      if (enough) return n + __ffs(enough);
+      have += __shfl_sync(0xffffffffu, u, 31);
+      n += 32;
+      at += dir * 32;
     }
-    const unsigned enough = __ballot_sync(0xffffffffu, have + u >= mt.nt);
-    if (enough) {
-      n += __ffs(enough);
-      break;
-    }
-    have += __shfl_sync(0xffffffffu, u, 31);
-    n += 32;
-  }
-  n = min(n, ctas - cta);
-  auto part = [&](int i) {
-    return parts + ((size_t)(cta + i) * 2 + (i == 0 ? mt.slot : 0)) * part_floats<D>();
+    return n;
   };
-  // parts i0, i0 + step, .. < n of row r, four in flight; l and acc relative to the running maximum m
-  auto add = [&](int i0, int step, int r, float& m, float (&acc)[V], float& l) {
-    constexpr int U = 4;
+  const Meta own = meta[cta];
 #pragma unroll 1
-    for (int i = i0; i < n; i += U * step) {
-      float mi[U], li[U], x[U][V];
+  for (int job = 0; job < 2; ++job) {
+    if (job == 0 ? own.before <= 0 : own.slot < 0) continue;
+    const int c0 = job == 0 ? max(0, cta - cover(cta - 1, -1, own.before)) : cta;
+    const Meta mt = job == 0 ? meta[c0] : own;
+    if (mt.slot < 0) continue;  // only after a wait that gave up
+    const int n = min(1 + cover(c0 + 1, 1, mt.nt - mt.have), ctas - c0);
+    const int rank = (cta - c0) * gridDim.y + blockIdx.y, ranks = n * gridDim.y;
+    auto part = [&](int i) {
+      return parts + ((size_t)(c0 + i) * 2 + (i == 0 ? mt.slot : 0)) * part_floats<D>();
+    };
+    // parts i0, i0 + step, .. < n of row r, four in flight; l and acc relative to the running maximum m
+    auto add = [&](int i0, int step, int r, float& m, float (&acc)[V], float& l) {
+      constexpr int U = 4;
+#pragma unroll 1
+      for (int i = i0; i < n; i += U * step) {
+        float mi[U], li[U], x[U][V];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int j = i + u * step;
-        mi[u] = -INFINITY;
-        if (j < n) {
-          const float* p = part(j);
-          mi[u] = p[128 * D + r];
-          li[u] = p[128 * D + 128 + r];
+        for (int u = 0; u < U; ++u) {
+          const int j = i + u * step;
+          mi[u] = -INFINITY;
+          if (j < n) {
+            const float* p = part(j);
+            mi[u] = p[128 * D + r];
+            li[u] = p[128 * D + 128 + r];
 #pragma unroll
-          for (int v = 0; v < V; v += 2) {
-            const float2 y = *reinterpret_cast<const float2*>(p + r * D + lane * V + v);
-            x[u][v] = y.x, x[u][v + 1] = y.y;
+            for (int v = 0; v < V; v += 2) {
+              const float2 y = *reinterpret_cast<const float2*>(p + r * D + lane * V + v);
+              x[u][v] = y.x, x[u][v + 1] = y.y;
+            }
           }
         }
-      }
-      const float to = fmaxf(fmaxf(fmaxf(mi[0], mi[1]), fmaxf(mi[2], mi[3])), m);
-      if (to > m) {
-        const float f = ex2(m - to);
-        l *= f;
+        const float to = fmaxf(fmaxf(fmaxf(mi[0], mi[1]), fmaxf(mi[2], mi[3])), m);
+        if (to > m) {
+          const float f = ex2(m - to);
+          l *= f;
 #pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] *= f;
-        m = to;
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (mi[u] > -INFINITY) {  // a part that saw nothing may hold anything
-          const float f = ex2(mi[u] - m);
-          l = fmaf(f, li[u], l);
-          if (f != 0.f) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) acc[v] = fmaf(f, x[u][v], acc[v]);
-          }
+          for (int v = 0; v < V; ++v) acc[v] *= f;
+          m = to;
         }
-    }
-  };
-  const bool many = n > kMany;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (mi[u] > -INFINITY) {  // a part that saw nothing may hold anything
+            const float f = ex2(mi[u] - m);
+            l = fmaf(f, li[u], l);
+            if (f != 0.f) {
+#pragma unroll
+              for (int v = 0; v < V; ++v) acc[v] = fmaf(f, x[u][v], acc[v]);
+            }
+          }
+      }
+    };
+    const bool many = n > kMany;
 #pragma unroll 1
-  for (int r = many ? blockIdx.y : blockIdx.y * 8 + warp; r < mt.rows; r += many ? gridDim.y : gridDim.y * 8) {
-    const int tt = r / A.G, hq = mt.head * A.G + r - tt * A.G;
-    const int64_t tok = mt.row0 + tt;
-    uint32_t w[V / 2], gw[V / 2];
-    if (A.gate) load_words(A.gate + tok * A.g_row + hq * A.g_head + lane * V * 2, gw);
-    float m = -INFINITY, acc[V] = {}, l = 0.f;
-    add(many ? warp : 0, many ? 8 : 1, r, m, acc, l);
-    if (many) {
-      __syncthreads();
+    for (int r = many ? rank : rank * 8 + warp; r < mt.rows; r += many ? ranks : ranks * 8) {
+      const int tt = r / A.G, hq = mt.head * A.G + r - tt * A.G;
+      const int64_t tok = mt.row0 + tt;
+      uint32_t w[V / 2], gw[V / 2];
+      if (A.gate) load_words(A.gate + tok * A.g_row + hq * A.g_head + lane * V * 2, gw);
+      float m = -INFINITY, acc[V] = {}, l = 0.f;
+      add(many ? warp : 0, many ? 8 : 1, r, m, acc, l);
+      if (many) {
+        __syncthreads();
 #pragma unroll
-      for (int v = 0; v < V; ++v) s_o[warp][lane * V + v] = acc[v];
-      if (lane == 0) s_m[warp] = m, s_l[warp] = l;
-      __syncthreads();
-      if (warp) continue;
-      float to = s_m[0];
-      for (int k = 1; k < 8; ++k) to = fmaxf(to, s_m[k]);
-      l = 0.f;
+        for (int v = 0; v < V; ++v) s_o[warp][lane * V + v] = acc[v];
+        if (lane == 0) s_m[warp] = m, s_l[warp] = l;
+        __syncthreads();
+        if (warp) continue;
+        float to = s_m[0];
+        for (int k = 1; k < 8; ++k) to = fmaxf(to, s_m[k]);
+        l = 0.f;
 #pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] = 0.f;
-      for (int k = 0; k < 8; ++k) {
-        const float f = s_m[k] > -INFINITY ? ex2(s_m[k] - to) : 0.f;
-        l = fmaf(f, s_l[k], l);
+        for (int v = 0; v < V; ++v) acc[v] = 0.f;
+        for (int k = 0; k < 8; ++k) {
+          const float f = s_m[k] > -INFINITY ? ex2(s_m[k] - to) : 0.f;
+          l = fmaf(f, s_l[k], l);
 #pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] = fmaf(f, s_o[k][lane * V + v], acc[v]);
+          for (int v = 0; v < V; ++v) acc[v] = fmaf(f, s_o[k][lane * V + v], acc[v]);
+        }
       }
-    }
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < V / 2; ++e) {
-      float a = acc[2 * e] * inv, b = acc[2 * e + 1] * inv;
-      if (A.gate) {
-        const float2 z = Io<T>::up2(gw[e]);
-        a = __fdividef(a, 1.0f + __expf(-z.x));
-        b = __fdividef(b, 1.0f + __expf(-z.y));
+      for (int e = 0; e < V / 2; ++e) {
+        float a = acc[2 * e] * inv, b = acc[2 * e + 1] * inv;
+        if (A.gate) {
+          const float2 z = Io<T>::up2(gw[e]);
+          a = __fdividef(a, 1.0f + __expf(-z.x));
+          b = __fdividef(b, 1.0f + __expf(-z.y));
+        }
+        w[e] = Io<T>::down2(a, b);
       }
-      w[e] = Io<T>::down2(a, b);
+      store_words(A.out + (tok * (A.kv_heads * A.G) + hq) * (D * 2) + lane * V * 2, w);
     }
-    store_words(A.out + (tok * (A.kv_heads * A.G) + hq) * (D * 2) + lane * V * 2, w);
   }
 }
 
@@ -673,7 +683,7 @@ Status launch(const spock_paged_kv& kv, AttnArgs& A, bool few, int sms, cudaStre
     SPOCK_LAUNCH_CHECK("paged_attn_kernel");
   }
   pdl_scope overlap;  // the join's launch runs under the main kernel
-  e = launch_k(paged_join_kernel<T, D>, dim3(sms, std::min(4, (A.tp * A.G + 7) / 8)), dim3(256), 0, st, A);
+  e = launch_k(paged_join_kernel<T, D>, dim3(sms, 2), dim3(256), 0, st, A);
   if (e != cudaSuccess) return cuda_status(e, "paged_join_kernel");
   SPOCK_LAUNCH_CHECK("paged_join_kernel");
   return Status::ok();

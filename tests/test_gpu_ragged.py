@@ -896,3 +896,20 @@ def test_paged_attention_refuses_scales_and_strides(cuda_ok):
     # a stride that is never used may be anything
     one = torch.as_strided(q, (1, 8, 64), (0, 64, 1))
     assert torch.equal(call(one, 1.0), call(q[:1], 1.0))
+
+
+@pytest.mark.parametrize("dtype,d,hq,hk,new,lens", [
+    (F16, 256, 8, 2, [60] * 3, [4575] * 3),     # row tiles of full rows in a dozen parts each
+    (BF16, 128, 16, 2, [40], [60000]),          # in some hundred
+    (F16, 256, 16, 1, [1, 1], [30000, 20000]),  # few rows, some seventy parts
+    (BF16, 64, 4, 4, [200], [12000]),
+])
+def test_paged_attention_row_tiles_in_many_parts(cuda_ok, dtype, d, hq, hk, new, lens):
+    g = _gen(31)
+    c = Cache(lens, 64, hk, d, dtype, g)
+    starts = _starts(new)
+    q = torch.randn(sum(new), hq, d, device=DEV, generator=g).to(dtype)
+    gate = torch.randn(sum(new), hq, d, device=DEV, generator=g).to(dtype)
+    got = spock_b200.paged_attention(q, _i32(starts), *c.args(), 1 / math.sqrt(d), gate=gate)
+    spock_b200.Context.get(0).sync()
+    _check_attention(got, *_ref_attention(q, starts, c, 1 / math.sqrt(d), gate))
