@@ -724,7 +724,7 @@ Status launch_paged_attention(const spock_paged_kv& kv, int batch, const int32_t
   A.err = err;
   // Either kernel is right for every batch; the rows that a sequence brings on
   // average decide. One token each over 256 sequences takes 74 us in the few-row
-  // kernel and 93 in the wide one; five tokens each (64 sequences) 70 in the wide
+  // kernel and 93 in the wide one; five tokens each (64 sequences) 67 in the wide
   // one, and 89 in a few-row kernel of 32 rows, which is not kept. Head size 64
   // would leave half of the few-row kernel's output tile empty.
   const bool few = kv.head_dim >= 128 && total <= batch && A.G <= kFewRows;
