@@ -8,7 +8,6 @@
 // with (c, s) the table's row of the token's position. Bound by bandwidth:
 // each projected value is read once and each output written once.
 #include <algorithm>
-#include <mutex>
 
 #include "ragged.cuh"
 #include "ragged.h"
