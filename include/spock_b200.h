@@ -385,7 +385,8 @@ int spock_paged_attention_workspace(spock_ctx* ctx, int32_t q_heads, int32_t kv_
  *           the taken rows (unchanged values when none); may be state and
  *           conv_state themselves
  *   out     [total][num_heads*128] fp16 or NULL; rows not taken keep their values
- * At least one of out and state_out is given. */
+ * At least one of out and state_out is given. The states are 16-byte aligned,
+ * the conv states, conv_weight and out 8-byte, everything else as its type. */
 int spock_deltanet_decode_span(spock_ctx* ctx, const spock_dn_layer* layer, int32_t batch, const int32_t* start,
                                const int32_t* counts, int64_t total, const void* qkv, int64_t qkv_ld, const void* a,
                                const void* b, int64_t ab_ld, const void* z, int64_t z_ld, const void* conv_state,

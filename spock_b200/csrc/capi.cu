@@ -409,9 +409,9 @@ __attribute__((visibility("default"))) int spock_deltanet_decode_span(
     return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "NULL pointer");
   if (!out && !state_out && total) return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "neither out nor state_out");
   if (misaligned(state, 16) || misaligned(state_out, 16) || misaligned(conv_state, 8) ||
-      misaligned(conv_state_out, 8) || misaligned(layer->conv_weight, 8))
+      misaligned(conv_state_out, 8) || misaligned(layer->conv_weight, 8) || misaligned(out, 8))
     return fail(ctx, SPOCK_ERR_INVALID,
-                std::string(op) + "state must be 16-byte aligned, conv_state and conv_weight 8-byte");
+                std::string(op) + "state must be 16-byte aligned, conv_state, conv_weight and out 8-byte");
   if (!total && !state_out) return SPOCK_OK;
   DeviceGuard dg(ctx->device);
   if (!dg.ok) return fail(ctx, SPOCK_ERR_CUDA, std::string(op) + "cannot select device");

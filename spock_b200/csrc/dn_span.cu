@@ -191,7 +191,12 @@ __global__ void __launch_bounds__(kThreads, 2) dn_span_kernel(const __grid_const
   Rows rows = rows_of(blockIdx.x), rows1{0, 0};
   load_in(in, blockIdx.x, rows);
   if (blockIdx.x + step < A.items) rows1 = rows_of(blockIdx.x + step);
-  const float4 norm = reinterpret_cast<const float4*>(A.norm_w)[lane];
+  // by single floats, as spock_deltanet_decode_step: a weight need not start on 16 bytes
+  float4 norm = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (kOut) {
+    const float* w = A.norm_w + lane * 4;
+    norm = make_float4(w[0], w[1], w[2], w[3]);
+  }
   bool ok = true, waited = false;
   int phase = 0;
   __syncthreads();  // the barrier's initialisation
