@@ -41,7 +41,14 @@ struct Meta {
   int have, nt;  // KV tiles done here, in all
   int units;     // of this CTA
   int before;    // KV tiles of its first row tile that are in earlier CTAs
+  int last;      // the last position that the part's first token sees (negative: none)
 };
+// What a part says its weights refer to (log2 units): -inf where it has none, so
+// that the join passes it over; a part whose scores are all NaN has weights (NaN),
+// relative to 0.
+__device__ __forceinline__ float part_reference(float m, float sum) {
+  return m == -INFINITY && sum != 0.f ? 0.f : m;
+}
 template <int D>
 __host__ __device__ constexpr size_t part_floats() {
   return (size_t)128 * D + 256;

@@ -47,8 +47,8 @@ struct Few {
   static constexpr int NST = D == 256 ? 5 : 6;
   static constexpr int kRing = 2 * kQ + 2 * kP;
   static constexpr int kBar = kRing + NST * kStage;
-  static constexpr int kStat = kBar + 576;    // [2 row tiles][4 warps][NR] sums, [2][NR] references
-  static constexpr int kMax = kStat + 2 * 5 * NR * 4;  // [4 warps][NR] maxima
+  static constexpr int kStat = kBar + 576;    // [2 row tiles][4 warps][NR] sums, [2][2][NR] references
+  static constexpr int kMax = kStat + 2 * 6 * NR * 4;  // [4 warps][NR] maxima
   static constexpr int kSums = kMax + 4 * NR * 4;        // [NR][128] each softmax thread's sums
   static constexpr int kSmem = kSums + NR * 128 * 4;
   static constexpr int kBlocks = D / 128;     // M blocks of O^T
@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* s_armed = s_first + 4;  // [NST]
   static_assert((2 * NST + 18) * 8 <= 264 && 264 + (2 * (kThreads / 32) + 4) * 8 + (4 + NST) * 4 <= 576, "barrier area");
   float* s_sum = reinterpret_cast<float*>(sm + Sh::kStat);
+  // [2 row tiles]: of the vote, -inf for a row without scores; then of the weights, 0 for one
   float* s_ref = s_sum + 2 * 4 * NR;
   float* s_max = reinterpret_cast<float*>(sm + Sh::kMax);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -231,14 +232,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     // stay rolled and what they carry (references, sums) in shared memory: unrolled,
     // the kernel had 116 KB of code and waited for instructions first of all.
     float* const sum = reinterpret_cast<float*>(sm + Sh::kSums) + at;  // + r * 128
-    float* ref = s_ref;  // log2 units, the row tile's; a row that has seen nothing yet refers to -1e30
+    float* ref = s_ref;  // log2 units, the row tile's
     int k = w.k0, item = 0, rows = 0;
     auto meet = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
     auto enter = [&] {
       rows = min(A.tp, w.s.n - w.rt * A.tp) * A.G;
       ref = s_ref + (item & 1) * NR;
       if (item >= 2) wait_warp(&o_free[item & 1], ((item - 2) >> 1) & 1);
-      if (at < NR) ref[at] = -1e30f;
+      if (at < NR) ref[at] = -INFINITY, ref[2 * NR + at] = 0.f;
 #pragma unroll 1
       for (int r = 0; r < rows; ++r) sum[r * 128] = 0.f;
       meet();
@@ -332,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         meet();  // all have read the references
         if (at < rows) {
           const float m = top_of(at);
-          if (m - ref[at] > kLazy) ref[at] = m;
+          if (m - ref[at] > kLazy) ref[at] = ref[2 * NR + at] = m;
         }
         meet();
       }
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint8_t* const pw = sm + 2 * Sh::kQ + buf * Sh::kP + (at >> 6) * NR * 128 + (at & 7) * 2;
       const int ch = (at & 63) >> 3;
       each([&](int r, const float(&s)[4]) {
-        const float4 m = *reinterpret_cast<const float4*>(ref + r);
+        const float4 m = *reinterpret_cast<const float4*>(ref + 2 * NR + r);
         const float x[4] = {ex2(s[0] - m.x), ex2(s[1] - m.y), ex2(s[2] - m.z), ex2(s[3] - m.w)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -410,6 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mt.head = w.h;
         mt.have = w.k1;
         mt.nt = w.nt;
+        mt.last = w.s.len - w.s.n + t0;
       }
       wait_warp(&stats[item & 1], (item >> 1) & 1);
       wait_warp(&o_full[item & 1], (item >> 1) & 1);
@@ -420,6 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint8_t* gp = A.gate + row0 * A.g_row + (int64_t)w.h * A.G * A.g_head + (blk * 128 + dim) * 2;
         T* op = reinterpret_cast<T*>(A.out) + ((int64_t)row0 * heads + w.h * A.G) * D + blk * 128 + dim;
         int ng = 0, no = 0;  // head of the group: of gp, of op
+        int last = w.s.len - w.s.n + t0;  // the last position that op's row sees
 #pragma unroll 1
         for (int r = 0; r < rows; r += 4) {
           T gate[4];
@@ -439,11 +442,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (whole) {
               const float* l = sums + r + i;
               const float lt = (l[0] + l[NR]) + (l[2 * NR] + l[3 * NR]);
-              float x = lt == 0.f ? 0.f : __fdividef(o[i], lt);
+              float x = last < 0 ? 0.f : __fdividef(o[i], lt);
               if (A.gate) x = __fdividef(x, 1.0f + __expf(-to_float(gate[i])));
               *op = from_float<T>(x);
               op += D;
-              if (++no == A.G) no = 0, op += (int64_t)(heads - A.G) * D;
+              if (++no == A.G) no = 0, ++last, op += (int64_t)(heads - A.G) * D;
             } else {
               part[(r + i) * D + blk * 128 + dim] = o[i];
             }
@@ -451,9 +454,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!whole && dim < rows) {  // the part's references and sums, a row per thread
-        const float ref = s_ref[(item & 1) * NR + dim];
-        part[128 * D + dim] = ref <= -1e29f ? -INFINITY : ref;
-        part[128 * D + 128 + dim] = (sums[dim] + sums[NR + dim]) + (sums[2 * NR + dim] + sums[3 * NR + dim]);
+        const float l = (sums[dim] + sums[NR + dim]) + (sums[2 * NR + dim] + sums[3 * NR + dim]);
+        part[128 * D + dim] = part_reference(s_ref[(item & 1) * NR + dim], l);
+        part[128 * D + 128 + dim] = l;
       }
       tc::tc_fence_before();
       __syncwarp();

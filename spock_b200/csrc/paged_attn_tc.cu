@@ -378,6 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mt.head = it.h;
         mt.have = it.k1;
         mt.nt = it.nt;
+        mt.last = lim0;
       }
       if (live) {
         float* rl = red + (buf ^ 1) * 256;  // idle: the maxima of the tile before, read by both halves
@@ -386,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float lt = l + rl[(half ^ 1) * 128 + row];
         pair_sync();  // read before the next tile's maxima go there
         if (whole) {
-          const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+          const float inv = lim < 0 ? 0.f : 1.0f / lt;
           // 4 lanes trade their rows' 16-byte pieces, so that each store (and load of
           // gates) has 64 bytes of a row beside each other, 8 rows and not 32 at a time
           const int64_t op = (tok * (A.kv_heads * A.G) + hq) * (D * 2) + half * D;
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           float* part = parts + ((size_t)cta * 2 + slot) * part_floats<D>();
           if (half == 0 && row < rows) {
-            part[128 * D + row] = m == -INFINITY ? -INFINITY : m * c;
+            part[128 * D + row] = part_reference(m == -INFINITY ? m : m * c, lt);
             part[128 * D + 128 + row] = lt;
           }
 #pragma unroll 1
@@ -550,7 +551,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (mi[u] > -INFINITY) {  // a part that saw nothing may hold anything
+          if (mi[u] > -INFINITY) {  // not one without weights
             const float f = ex2(mi[u] - m);
             l = fmaf(f, li[u], l);
             if (f != 0.f) {
@@ -588,7 +589,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
           for (int v = 0; v < V; ++v) acc[v] = fmaf(f, s_o[k][lane * V + v], acc[v]);
         }
       }
-      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      const float inv = mt.last + tt < 0 ? 0.f : 1.0f / l;
 #pragma unroll
       for (int e = 0; e < V / 2; ++e) {
         float a = acc[2 * e] * inv, b = acc[2 * e + 1] * inv;

@@ -1,9 +1,13 @@
-"""Values and calls at the edges of the ragged steps."""
+"""Values and calls at the edges of the ragged steps: scores of any size, NaN and
+infinities in queries, tensors at odd offsets."""
+import math
+
 import pytest
 import torch
 
 import spock_b200
-from tests.test_gpu_ragged import DEV, F16, _i32, _span_inputs
+from tests.test_gpu_ragged import (BF16, DEV, F16, Cache, _check_attention, _gen, _i32, _ref_attention, _span_inputs,
+                                   _starts)
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +42,76 @@ def test_deltanet_decode_span_at_odd_offsets(cuda_ok):
             with pytest.raises(spock_b200.SpockError, match="aligned") as e:
                 span(layer, qkv, args["conv_state"], args["state"], a, b, z, s, stream=stream)
             assert e.value.code == spock_b200.SPOCK_ERR_INVALID
+
+
+# dtype, head_dim, q_heads, kv_heads, new tokens, lengths: both kernels, row tiles of one CTA and of several
+KERNELS = [
+    (F16, 128, 8, 2, [1, 1], [100, 40]),         # few rows, whole
+    (BF16, 256, 8, 2, [1], [40000]),             # few rows, in parts
+    (F16, 128, 6, 2, [1, 1], [30000, 700]),      # the same with pad rows
+    (BF16, 128, 8, 2, [5, 9], [100, 40]),        # wide, whole
+    (F16, 256, 8, 2, [40], [9000]),              # wide, in parts
+    (BF16, 64, 4, 2, [3, 1], [5000, 4]),
+]
+
+
+def _case(case, seed):
+    dtype, d, hq, hk, new, lens = KERNELS[case]
+    g = _gen(seed + case)
+    c = Cache(lens, 16, hk, d, dtype, g)
+    q = torch.randn(sum(new), hq, d, device=DEV, generator=g).to(dtype)
+    return c, q, _starts(new)
+
+
+def _attend(q, starts, c, scale):
+    got = spock_b200.paged_attention(q, _i32(starts), *c.args(), scale)
+    spock_b200.Context.get(0).sync()
+    return got
+
+
+@pytest.mark.parametrize("case", range(len(KERNELS)))
+def test_equal_scores_average_the_values(cuda_ok, case):
+    """All of a row's scores equal, from -2^100 (what the type holds of it) to 2^30: every weight is the same."""
+    c, q, starts = _case(case, 200)
+    big = 2.0 ** 50 if c.k.dtype == BF16 else 2.0 ** 15
+    for a, b in ((0.0, 1.0), (2.0 ** 15, 2.0 ** 15), (big, -big), (-(2.0 ** 13) * 1.25, 1.125 * 2.0 ** 14)):
+        q.zero_()
+        q[..., 5], c.k[..., 5] = a, b
+        for other in (0, 17):  # more than one product to a score
+            c.k[..., other] = 0.0
+        got = _attend(q, starts, c, 1.0)
+        # every term of a score but one is exactly 0, so the scores are exact and equal
+        ref, mag, _ = _ref_attention(q, starts, c, 1.0, None)
+        _check_attention(got, ref, mag, torch.zeros_like(mag))
+
+
+@pytest.mark.parametrize("case", range(len(KERNELS)))
+def test_nan_and_infinite_queries_stay_in_their_rows(cuda_ok, case):
+    """A row whose query holds NaN, or whose scores are all -inf, is NaN, whole or in parts; all others are as ever."""
+    c, q, starts = _case(case, 210)
+    c.k[..., 0] = -c.k[..., 0].abs() - 0.5
+    ref, mag, err = _ref_attention(q, starts, c, 0.125, None)
+    nan = torch.zeros(q.shape[:2], dtype=torch.bool, device=DEV)
+    for i, value in enumerate((math.nan, math.inf)):
+        t, h = i * (q.shape[0] - 1), i * 3
+        q[t, h] = 0.0
+        q[t, h, 0] = value  # +inf times negative keys, and zeros: every score -inf
+        nan[t, h] = True
+    got = _attend(q, starts, c, 0.125)
+    assert bool(torch.isnan(got[nan]).all())
+    _check_attention(got[~nan], ref[~nan], mag[~nan], err[~nan])
+
+
+@pytest.mark.parametrize("dtype,d,n,length", [(F16, 128, 152, 150), (BF16, 256, 300, 290), (F16, 64, 7, 4)])
+def test_nan_queries_that_see_nothing(cuda_ok, dtype, d, n, length):
+    """Tokens before position 0 are zero whatever their queries hold, also beside tokens that see several tiles."""
+    g = _gen(5)
+    c = Cache([length], 16, 2, d, dtype, g)
+    q = torch.randn(n, 8, d, device=DEV, generator=g).to(dtype)
+    q[0, 1], q[1, 2, 3] = math.nan, math.inf
+    got = _attend(q, [0, n], c, 0.125)
+    blind = n - length
+    assert bool((got[:blind] == 0).all())
+    q[:2] = 0
+    ref = _ref_attention(q, [0, n], c, 0.125, None)
+    _check_attention(got[blind:], *(t[blind:] for t in ref))
