@@ -345,17 +345,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        const float mc = m == -INFINITY ? 0.f : m * c;
+        // (s - m) c and not s c - m c: at scores of 2^31 a rounding of m c is 2^7, weights of 2^+-128
+        const float from = m == -INFINITY ? 0.f : m;
         uint32_t p[32];
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        float2 sum[2] = {};
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float a = ex2(fmaf(s[2 * j], c, -mc)), b = ex2(fmaf(s[2 * j + 1], c, -mc));
-          sum[(2 * j) & 3] += a;
-          sum[(2 * j + 1) & 3] += b;
-          p[j] = Io<T>::down2(a, b);
+        for (int j = 0; j < 32; ++j) {  // in pairs, so that this costs no more than the one multiply-add
+          const float2 x = __fmul2_rn(__fadd2_rn(make_float2(s[2 * j], s[2 * j + 1]), make_float2(-from, -from)),
+                                      make_float2(c, c));
+          const float2 w = make_float2(ex2(x.x), ex2(x.y));
+          sum[j & 1] = __fadd2_rn(sum[j & 1], w);
+          p[j] = Io<T>::down2(w.x, w.y);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tc::tmem_st32u(tb + buf * kTile + lane_off + half * 32, p);
         tc::tmem_st_wait();
       }

@@ -115,3 +115,15 @@ def test_nan_queries_that_see_nothing(cuda_ok, dtype, d, n, length):
     q[:2] = 0
     ref = _ref_attention(q, [0, n], c, 0.125, None)
     _check_attention(got[blind:], *(t[blind:] for t in ref))
+
+
+@pytest.mark.parametrize("case", range(len(KERNELS)))
+def test_equal_scores_that_do_not_round_to_powers(cuda_ok, case):
+    """Equal scores of some 2^32, whose product with log2(e) fp32 does not hold: still the average of the values."""
+    c, q, starts = _case(case, 240)
+    for a, b in ((57344.0, 61440.0), (61440.0, 63488.0), (-57344.0, 61440.0)):
+        q.zero_()
+        q[..., 5], c.k[..., 5] = a, b
+        got = _attend(q, starts, c, 1.0)
+        ref, mag, _ = _ref_attention(q, starts, c, 1.0, None)
+        _check_attention(got, ref, mag, torch.zeros_like(mag))
