@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* s_armed = s_first + 4;  // [NST]
   static_assert((2 * NST + 18) * 8 <= 264 && 264 + (2 * (kThreads / 32) + 4) * 8 + (4 + NST) * 4 <= 576, "barrier area");
   float* s_sum = reinterpret_cast<float*>(sm + Sh::kStat);
-  // [2 row tiles]: of the vote, -inf for a row without scores; then of the weights, 0 for one
+  // [2 row tiles]: of the vote, -inf for a row without scores yet; then of the weights, 0 for one
   float* s_ref = s_sum + 2 * 4 * NR;
   float* s_max = reinterpret_cast<float*>(sm + Sh::kMax);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -239,7 +239,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       rows = min(A.tp, w.s.n - w.rt * A.tp) * A.G;
       ref = s_ref + (item & 1) * NR;
       if (item >= 2) wait_warp(&o_free[item & 1], ((item - 2) >> 1) & 1);
-      if (at < NR) ref[at] = -INFINITY, ref[2 * NR + at] = 0.f;
+      // rows behind the last, in its block of 4, have whatever scores: none is above their reference, all weights are 0
+      if (at < NR) ref[at] = at < rows ? -INFINITY : INFINITY, ref[2 * NR + at] = at < rows ? 0.f : INFINITY;
 #pragma unroll 1
       for (int r = 0; r < rows; ++r) sum[r * 128] = 0.f;
       meet();
