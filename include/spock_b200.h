@@ -350,7 +350,10 @@ int spock_paged_attention_prep(spock_ctx* ctx, const spock_paged_kv* kv, int32_t
  * kernel is chosen by total against batch, so a prompt chunk runs slower in a
  * batch that is mostly sequences without new tokens.
  *   out[r][h] = sum_p softmax_p(scale * q[r][h] . k_p) v_p, times
- *   sigmoid(gate[r][h]) when gate is not NULL; rounded once
+ *   sigmoid(gate[r][h]) when gate is not NULL; scores, sums and outputs in
+ *   fp32, the weights exp(score - about the row's largest) rounded to the
+ *   cache's dtype before they meet v (fp16: ones below 2^-32 of the largest
+ *   are lost), the result rounded once
  *   q, gate rows and heads at their own strides (elements, multiples of 8;
  *           q's positive)
  *   scale   positive and finite

@@ -17,6 +17,13 @@ constexpr uint32_t kSleep = 20000;      // ns that one poll may sleep
 constexpr int kThreads = 384;
 constexpr int kFewRows = 16;  // rows of a row tile of the few-row kernel
 constexpr float kLazy = 8.0f;  // log2 of how far weights may exceed 1
+// Weights (and so their sums and O) are 2^kUp times as large where they are rounded
+// to fp16: the largest stay below 2^15, and those far below a row's largest keep
+// their bits down to 2^-21 of it and are lost below 2^-32. Without, a position
+// e^16 below the largest had 2 of its 11 bits, and one e^18 below none, although
+// thousands of them may weigh more than the largest.
+template <typename T>
+constexpr float kUp = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 
 struct AttnArgs {
   const int32_t *start, *table, *kv_len;

@@ -343,7 +343,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int ch = (at & 63) >> 3;
       each([&](int r, const float(&s)[4]) {
         const float4 m = *reinterpret_cast<const float4*>(ref + 2 * NR + r);
-        const float x[4] = {ex2(s[0] - m.x), ex2(s[1] - m.y), ex2(s[2] - m.z), ex2(s[3] - m.w)};
+        const float x[4] = {ex2(s[0] - m.x + kUp<T>), ex2(s[1] - m.y + kUp<T>), ex2(s[2] - m.z + kUp<T>),
+                            ex2(s[3] - m.w + kUp<T>)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           sum[(r + i) * 128] += x[i];

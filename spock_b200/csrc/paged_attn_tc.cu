@@ -17,7 +17,7 @@
 // softmax of a tile runs; the ring and the walk run on across row tiles. P
 // overwrites its S in TMEM, in the operand type. The running maximum a row's
 // weights refer to moves only when a tile's exceeds it by 2^8 (weights stay
-// below 256, exact sums in fp32), so O is rarely rescaled.
+// below 2^8, times kUp; sums in fp32), so O is rarely rescaled.
 // A row tile that is one CTA's alone is finished there; a cut one leaves its
 // unnormalised O (fp32), maximum and sum in the workspace, and
 // paged_join_kernel adds the parts in order (no atomics: results repeat).
@@ -351,8 +351,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         float2 sum[2] = {};
 #pragma unroll
         for (int j = 0; j < 32; ++j) {  // in pairs, so that this costs no more than the one multiply-add
-          const float2 x = __fmul2_rn(__fadd2_rn(make_float2(s[2 * j], s[2 * j + 1]), make_float2(-from, -from)),
-                                      make_float2(c, c));
+          const float2 x = __ffma2_rn(__fadd2_rn(make_float2(s[2 * j], s[2 * j + 1]), make_float2(-from, -from)),
+                                      make_float2(c, c), make_float2(kUp<T>, kUp<T>));
           const float2 w = make_float2(ex2(x.x), ex2(x.y));
           sum[j & 1] = __fadd2_rn(sum[j & 1], w);
           p[j] = Io<T>::down2(w.x, w.y);

@@ -1,13 +1,14 @@
 """Values and calls at the edges of the ragged steps: scores of any size, NaN and
-infinities in queries, tensors at odd offsets."""
+infinities in queries, weights far below a row's largest, group sizes that leave
+pad rows, tensors at odd offsets."""
 import math
 
 import pytest
 import torch
 
 import spock_b200
-from tests.test_gpu_ragged import (BF16, DEV, F16, Cache, _check_attention, _gen, _i32, _ref_attention, _span_inputs,
-                                   _starts)
+from tests.test_gpu_ragged import (BF16, DEV, F16, Cache, _check_attention, _gen, _half_step, _i32, _ref_attention,
+                                   _span_inputs, _starts)
 
 pytestmark = pytest.mark.gpu
 
@@ -156,3 +157,29 @@ def test_pad_rows_cost_nothing(cuda_ok, group):
     """Decode reads the cache whatever the group size: one that leaves pad rows is no slower than the next one of 4."""
     full = _decode_us((group + 3) // 4 * 4)
     assert _decode_us(group) <= 1.1 * full, (group, _decode_us(group), full)
+
+
+@pytest.mark.parametrize("case", range(len(KERNELS)))
+def test_weights_far_below_the_largest(cuda_ok, case):
+    """One position in 64 weighs e^16 times as much as the others, whose values are all that is seen."""
+    c, q, starts = _case(case, 220)
+    for b, n in enumerate(c.lens):
+        p = torch.arange(n, device=DEV)
+        ids, slot = c.slots(b, p)
+        c.k[ids, slot] = 0.0
+        c.v[ids, slot] = 1000.0
+        few = p % 64 == 0
+        c.k[ids[few], slot[few], :, 3] = 16.0
+        c.v[ids[few], slot[few]] = 0.0
+    q.zero_()
+    q[..., 3] = 1.0
+    got = _attend(q, starts, c, 1.0).double()
+    ref, mag, _ = _ref_attention(q, starts, c, 1.0, None)
+    # as in _check_attention, with exact scores; and fp16 weights, kept with 7 more octaves below the row's
+    # largest than fp16's own 2^-24: off by 2^-32 of it each, 63 of 64 positions 1000 times that
+    e = _half_step(q.dtype)
+    tol = e * ref.abs() + (2 * e + 2.0 ** -15) * mag
+    if q.dtype == F16:
+        tol = tol + 6e-8 + 64 * 1000 * 2.0 ** -32
+    off = (got - ref).abs()
+    assert bool((off <= tol).all()), float((off / tol).max())
