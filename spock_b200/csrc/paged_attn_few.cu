@@ -347,8 +347,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                             ex2(s[3] - m.w + kUp<T>)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          sum[(r + i) * 128] += x[i];
-          *reinterpret_cast<T*>(pw + (r + i) * 128 + ((ch ^ ((r + i) & 7)) << 4)) = from_float<T>(x[i]);
+          const T p = from_float<T>(x[i]);
+          sum[(r + i) * 128] += to_float(p);  // of the weights that V gets: they add up to 1
+          *reinterpret_cast<T*>(pw + (r + i) * 128 + ((ch ^ ((r + i) & 7)) << 4)) = p;
         }
       });
       tc::fence_async_smem();

@@ -354,8 +354,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float2 x = __ffma2_rn(__fadd2_rn(make_float2(s[2 * j], s[2 * j + 1]), make_float2(-from, -from)),
                                       make_float2(c, c), make_float2(kUp<T>, kUp<T>));
           const float2 w = make_float2(ex2(x.x), ex2(x.y));
-          sum[j & 1] = __fadd2_rn(sum[j & 1], w);
           p[j] = Io<T>::down2(w.x, w.y);
+          sum[j & 1] = __fadd2_rn(sum[j & 1], Io<T>::up2(p[j]));  // of the weights that V gets: they add up to 1
         }
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tc::tmem_st32u(tb + buf * kTile + lane_off + half * 32, p);

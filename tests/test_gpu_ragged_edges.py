@@ -183,3 +183,20 @@ def test_weights_far_below_the_largest(cuda_ok, case):
         tol = tol + 6e-8 + 64 * 1000 * 2.0 ** -32
     off = (got - ref).abs()
     assert bool((off <= tol).all()), float((off / tol).max())
+
+
+@pytest.mark.parametrize("case", range(len(KERNELS)))
+def test_weights_sum_to_one(cuda_ok, case):
+    """Values that are all the same come out as they are (times the gate), whatever the weights' roundings."""
+    c, q, starts = _case(case, 230)
+    c.k *= 4  # some weights carry most of a row, in tiles behind the first
+    c.v[:] = torch.where(torch.isnan(c.v), math.nan, 1.0)
+    gate = torch.randn(q.shape, device=DEV, generator=_gen(case)).to(q.dtype)
+    got = spock_b200.paged_attention(q, _i32(starts), *c.args(), 0.125, gate=gate)
+    spock_b200.Context.get(0).sync()
+    ref = torch.sigmoid(gate.double())
+    # the output's rounding; both sums of weights in fp32, in chains of at most 2^9 steps of 2^-23 (the matrix
+    # instructions may cut off what they add); 2^-15 for the division and the gate. No rounding of weights.
+    tol = (_half_step(q.dtype) + 2 * 2.0 ** -14 + 2.0 ** -15) * ref
+    off = (got.double() - ref).abs()
+    assert bool((off <= tol).all()), float((off / tol).max())
