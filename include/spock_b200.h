@@ -294,6 +294,8 @@ int spock_attention_prefill(spock_ctx* ctx, int32_t exact, const void* proj, con
  * that is out of range is never used as an address, the outputs of that
  * sequence are unspecified, and the next spock_sync (spock_model_sync for a
  * model on the same context) returns SPOCK_ERR_INVALID.
+ * Outputs overlap no input and no other output of the call, unless its comment
+ * says that they may.
  * The calls keep no scratch in the context: workspaces are the caller's, so
  * calls on several streams, or captured in several CUDA graphs, need only
  * workspaces of their own. A workspace's contents need no initialisation and
@@ -417,6 +419,7 @@ int spock_deltanet_decode_span(spock_ctx* ctx, const spock_dn_layer* layer, int3
  *              to commit (spock_deltanet_decode_span's counts); 0 for no rows
  *   out_tokens int32 [total]: accepted drafts, the next token, then -1 to the
  *              sequence's end
+ * Neither overlaps tokens, start or the other.
  * workspace: at least spock_draft_verify_workspace() bytes, 16-byte aligned. */
 int spock_draft_verify(spock_ctx* ctx, int32_t dtype, const void* logits, int64_t logits_ld, int64_t total,
                        int64_t vocab, int32_t batch, const int32_t* start, const int32_t* tokens,

@@ -94,6 +94,9 @@ struct DeviceGuard {
 };
 
 bool misaligned(const void* p, uintptr_t bytes) { return (uintptr_t)p % bytes != 0; }
+bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  return a && b && (uintptr_t)a < (uintptr_t)b + b_bytes && (uintptr_t)b < (uintptr_t)a + a_bytes;
+}
 
 // What the two paged-attention calls check of the cache and the packed rows.
 int check_paged(spock_ctx* ctx, const char* op, const spock_paged_kv* kv, int32_t batch, const int32_t* start,
@@ -444,6 +447,12 @@ __attribute__((visibility("default"))) int spock_draft_verify(
     return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "bad arguments");
   if (misaligned(logits, dtype == SPOCK_F32 ? 4 : 2) || misaligned(workspace, 16))
     return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "misaligned pointer");
+  const size_t rows = (size_t)total * 4, seqs = (size_t)batch * 4;
+  if (overlap(out_tokens, rows, tokens, rows) || overlap(emitted, seqs, tokens, rows) ||
+      overlap(out_tokens, rows, start, seqs + 4) || overlap(emitted, seqs, start, seqs + 4) ||
+      overlap(out_tokens, rows, emitted, seqs))
+    return fail(ctx, SPOCK_ERR_INVALID,
+                std::string(op) + "emitted and out_tokens must not overlap tokens, start or each other");
   if (batch > (1 << 27)) return fail(ctx, SPOCK_ERR_UNSUPPORTED, std::string(op) + "at most 2^27 sequences");
   if (workspace_bytes < spock::draft_verify_workspace(total, vocab, batch))
     return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "workspace too small");

@@ -1,6 +1,6 @@
 """Values and calls at the edges of the ragged steps: scores of any size, NaN and
 infinities in queries, weights far below a row's largest, group sizes that leave
-pad rows, tensors at odd offsets."""
+pad rows, tensors at odd offsets, outputs over inputs."""
 import math
 
 import pytest
@@ -8,7 +8,7 @@ import torch
 
 import spock_b200
 from tests.test_gpu_ragged import (BF16, DEV, F16, Cache, _check_attention, _gen, _half_step, _i32, _ref_attention,
-                                   _span_inputs, _starts)
+                                   _span_inputs, _starts, _verify_inputs)
 
 pytestmark = pytest.mark.gpu
 
@@ -200,3 +200,22 @@ def test_weights_sum_to_one(cuda_ok, case):
     tol = (_half_step(q.dtype) + 2 * 2.0 ** -14 + 2.0 ** -15) * ref
     off = (got.double() - ref).abs()
     assert bool((off <= tol).all()), float((off / tol).max())
+
+
+def test_draft_verify_refuses_outputs_over_its_inputs(cuda_ok):
+    """Threads that write out_tokens would race with those that still read tokens: refused on the host."""
+    logits, tokens, ua, us, _ = _verify_inputs([3, 2], 50, F16, 3, False)
+    buf = torch.zeros(16, dtype=torch.int32, device=DEV)
+    buf[:3], buf[3:8] = _i32([0, 3, 5]), tokens
+    start, toks = buf[:3], buf[3:8]
+    want = spock_b200.draft_verify(logits, tokens, _i32([0, 3, 5]), ua, us)
+    for stream in (None, torch.cuda.current_stream()):
+        call = lambda **k: spock_b200.draft_verify(logits, toks, start, ua, us, stream=stream, **k)
+        for bad in (dict(out_tokens=toks), dict(out_tokens=buf[7:12]), dict(out_tokens=buf[2:7]),
+                    dict(emitted=buf[7:9]), dict(emitted=buf[1:3]), dict(out_tokens=buf[8:13], emitted=buf[12:14])):
+            with pytest.raises(spock_b200.SpockError, match="must not overlap") as e:
+                call(**bad)
+            assert e.value.code == spock_b200.SPOCK_ERR_INVALID
+        got = call(out_tokens=buf[8:13], emitted=buf[13:15])  # side by side is apart
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert torch.equal(toks, tokens)
