@@ -415,6 +415,12 @@ __attribute__((visibility("default"))) int spock_deltanet_decode_span(
       misaligned(conv_state_out, 8) || misaligned(layer->conv_weight, 8) || misaligned(out, 8))
     return fail(ctx, SPOCK_ERR_INVALID,
                 std::string(op) + "state must be 16-byte aligned, conv_state, conv_weight and out 8-byte");
+  const size_t items = (size_t)batch * layer->num_heads, state_bytes = items * 128 * 128 * 4;
+  const size_t conv_bytes = items * 3 * 128 * 4 * 2;
+  if ((state_out != state && overlap(state_out, state_bytes, state, state_bytes)) ||
+      (conv_state_out != conv_state && overlap(conv_state_out, conv_bytes, conv_state, conv_bytes)))
+    return fail(ctx, SPOCK_ERR_INVALID,
+                std::string(op) + "state_out and conv_state_out are state and conv_state, or apart from them");
   if (!total && !state_out) return SPOCK_OK;
   DeviceGuard dg(ctx->device);
   if (!dg.ok) return fail(ctx, SPOCK_ERR_CUDA, std::string(op) + "cannot select device");

@@ -219,3 +219,22 @@ def test_draft_verify_refuses_outputs_over_its_inputs(cuda_ok):
         got = call(out_tokens=buf[8:13], emitted=buf[13:15])  # side by side is apart
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         assert torch.equal(toks, tokens)
+
+
+def test_deltanet_decode_span_refuses_shifted_states(cuda_ok):
+    """New states over another sequence's old ones would race with their reads; in place and apart are fine."""
+    layer, qkv, conv, state, a, b, z = _span_inputs([2, 1], 4, seed=1)
+    s = _i32([0, 2, 3])
+    pool, pool_c = torch.zeros(5, *state.shape[1:], device=DEV), torch.zeros(5, *conv.shape[1:], dtype=F16, device=DEV)
+    pool[1:3], pool_c[1:3] = state, conv
+    run = lambda st, cv, **k: spock_b200.deltanet_decode_span(layer, qkv, pool_c[1:3], pool[1:3], a, b, None, s,
+                                                              state_out=st, conv_out=cv, **k)
+    for stream in (None, torch.cuda.current_stream()):
+        for i, j in ((0, 1), (2, 1), (1, 2), (1, 0), (0, 3), (3, 2)):
+            with pytest.raises(spock_b200.SpockError, match="apart from them") as e:
+                run(pool[i:i + 2], pool_c[j:j + 2], stream=stream)
+            assert e.value.code == spock_b200.SPOCK_ERR_INVALID
+    run(pool[3:5], pool_c[3:5])
+    run(pool[1:3], pool_c[1:3])
+    spock_b200.Context.get(0).sync()
+    assert torch.equal(pool[1:3], pool[3:5]) and torch.equal(pool_c[1:3], pool_c[3:5])
