@@ -410,9 +410,13 @@ def _stream_of(d, stream):
 
 def _new(shape, dtype, like, stream):
     """An uninitialised tensor for work on `stream` (None: the current one)."""
-    t = like.new_empty(shape, dtype=dtype)
-    if stream is not None:  # allocated on the current stream: not to be reused before `stream` is done with it
-        t.record_stream(stream)
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    import torch
+    # From the allocator's blocks of `stream`: one of the current stream's may still be in use by work queued there.
+    with torch.cuda.stream(stream):
+        t = like.new_empty(shape, dtype=dtype)
+    t.record_stream(torch.cuda.current_stream(like.device))  # where the caller may read it
     return t
 
 

@@ -1,6 +1,6 @@
 """Values and calls at the edges of the ragged steps: scores of any size, NaN and
 infinities in queries, weights far below a row's largest, group sizes that leave
-pad rows, tensors at odd offsets, outputs over inputs."""
+pad rows, tensors at odd offsets, outputs over inputs, named streams."""
 import math
 
 import pytest
@@ -238,3 +238,35 @@ def test_deltanet_decode_span_refuses_shifted_states(cuda_ok):
     run(pool[1:3], pool_c[1:3])
     spock_b200.Context.get(0).sync()
     assert torch.equal(pool[1:3], pool[3:5]) and torch.equal(pool_c[1:3], pool_c[3:5])
+
+
+def test_named_streams_do_not_take_memory_in_use(cuda_ok):
+    """Memory that the current stream has freed, with work on it still queued, is not what a call on another stream
+    gets for its outputs and workspaces."""
+    g = _gen(6)
+    c, starts = Cache([900, 130], 16, 2, 256, F16, g), _i32([0, 200, 300])
+    q = torch.randn(300, 8, 256, device=DEV, generator=g).half()
+    proj = torch.randn(300, 20 * 256, device=DEV, generator=g).half()
+    layer, qkv, conv, state, a, b, z = _span_inputs([200, 100], 4, seed=1)
+    logits, tokens, ua, us, _ = _verify_inputs([200, 100], 5000, F16, 3, False)
+    side = torch.cuda.Stream()
+    calls = [lambda **k: (spock_b200.paged_attention(q, starts, *c.args(), 0.0625, **k),),
+             lambda **k: (spock_b200.paged_attention_prep(proj, starts, *c.args(), **k),),
+             lambda **k: (spock_b200.deltanet_decode_span(layer, qkv, conv, state, a, b, z, starts, **k),),
+             lambda **k: spock_b200.draft_verify(logits, tokens, starts, ua, us, **k)]
+    for call in calls:
+        want = [t.clone() for t in call()]
+        torch.cuda.synchronize()
+        sizes = [t.numel() * t.element_size() for t in want] + [1 << 25, 1 << 23, 1 << 21, 1 << 12]
+        held = [torch.empty(n, dtype=torch.uint8, device=DEV) for n in sizes for _ in range(2)]
+        was = {t.data_ptr() for t in held}
+        torch.cuda._sleep(40_000_000)  # some 20 ms
+        for t in held:
+            t.fill_(255)
+        del held, t
+        got = call(stream=side)
+        assert not was & {t.data_ptr() for t in got}
+        side.synchronize()
+        torch.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
