@@ -70,16 +70,30 @@ def build_apps(force=False, verbose=False):
             raise RuntimeError("nvcc failed on " + src)
 
 
-BINDING = os.path.join(HERE, "_binding.so")
+def binding_path():
+    """Where this interpreter's and this torch's binding lives: another one's would load and then misread its tensors."""
+    import sysconfig
+
+    import torch
+    return os.path.join(HERE, "_binding.%s.torch%s.so" % (sysconfig.get_config_var("SOABI"), torch.__version__))
 
 
 def build_binding(force=False, verbose=False):
     """The Python wrappers' short way into the library (csrc/binding.cpp): a
-    CPython extension over torch's tensors, linked against libspock_b200.so."""
-    src = os.path.join(CSRC, "binding.cpp")
+    CPython extension over torch's tensors, linked against libspock_b200.so.
+    One process at a time, and into place in one step: others that make their
+    first call meanwhile find a whole file or none. Raises RuntimeError or
+    OSError where it cannot be built."""
+    import fcntl
+
+    path, src = binding_path(), os.path.join(CSRC, "binding.cpp")
     deps = [src, os.path.join(HERE, "..", "include", "spock_b200.h")]
-    if not force and os.path.exists(BINDING) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in deps):
-        return BINDING
+
+    def fresh():
+        return os.path.exists(path) and all(os.path.getmtime(d) <= os.path.getmtime(path) for d in deps)
+
+    if not force and fresh():
+        return path
     import sysconfig
 
     import torch
@@ -87,17 +101,27 @@ def build_binding(force=False, verbose=False):
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
     libdir = os.path.join(root, "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
-    cmd += ["-isystem" + i for i in inc]
-    cmd += [src, "-o", BINDING, "-L" + HERE, "-l:libspock_b200.so", "-Wl,-rpath,$ORIGIN", "-L" + libdir, "-lc10",
-            "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath," + libdir]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or r.returncode:
-        sys.stderr.write(r.stdout + r.stderr)
-    if r.returncode:
-        raise RuntimeError("g++ failed on binding.cpp")
-    return BINDING
+    with open(src) as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        if not force and fresh():  # another process was first
+            return path
+        part = "%s.%d.part" % (path, os.getpid())
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+               "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+        cmd += ["-isystem" + i for i in inc]
+        cmd += [src, "-o", part, "-L" + HERE, "-l:libspock_b200.so", "-Wl,-rpath,$ORIGIN", "-L" + libdir, "-lc10",
+                "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath," + libdir]
+        try:
+            r = subprocess.run(cmd, capture_output=True, text=True)
+            if verbose or r.returncode:
+                sys.stderr.write(r.stdout + r.stderr)
+            if r.returncode:
+                raise RuntimeError("g++ failed on binding.cpp")
+            os.replace(part, path)
+        finally:
+            if os.path.exists(part):
+                os.remove(part)
+    return path
 
 
 if __name__ == "__main__":
