@@ -18,6 +18,7 @@ Reference interfaces mirrored here:
 import ctypes
 import os
 import struct
+import warnings
 from dataclasses import dataclass, field
 from typing import List, Optional
 
@@ -80,7 +81,10 @@ def build(force=False):
     from . import builder as _b
     lib_path = _b.build(force=force)
     _b.build_apps(force=force)
-    _b.build_binding(force=force)
+    try:
+        _b.build_binding(force=force)
+    except (ImportError, OSError, RuntimeError) as e:  # the library and the wrappers do without
+        _no_binding(e)
     return lib_path
 
 
@@ -331,11 +335,16 @@ def deltanet_recurrent(q, k, v, g, beta, state, num_heads=16, key_dim=128, value
     return out
 
 
-_BINDING = None
+_BINDING = None  # the module; False where it cannot be had
+
+
+def _no_binding(why):
+    warnings.warn("spock_b200: %s; calls of the ragged steps take some 10 us longer on the host" % why)
 
 
 def _binding():
-    """The ragged steps' short way into the library (csrc/binding.cpp), built in-tree when absent."""
+    """The ragged steps' short way into the library (csrc/binding.cpp), built in-tree when absent; None where it cannot
+    be built or loaded: the wrappers then make their checks themselves."""
     global _BINDING
     if _BINDING is None:
         lib()
@@ -343,12 +352,17 @@ def _binding():
         import importlib.util
         import torch  # noqa: F401  (its libraries are loaded first)
         from . import builder
-        path = builder.build_binding()
-        loader = importlib.machinery.ExtensionFileLoader("spock_b200._binding", path)
-        spec = importlib.util.spec_from_file_location("spock_b200._binding", path, loader=loader)
-        _BINDING = importlib.util.module_from_spec(spec)
-        loader.exec_module(_BINDING)
-    return _BINDING
+        try:
+            path = builder.build_binding()
+            loader = importlib.machinery.ExtensionFileLoader("spock_b200._binding", path)
+            spec = importlib.util.spec_from_file_location("spock_b200._binding", path, loader=loader)
+            module = importlib.util.module_from_spec(spec)
+            loader.exec_module(module)
+            _BINDING = module
+        except (ImportError, OSError, RuntimeError) as e:
+            _no_binding(e)
+            _BINDING = False
+    return _BINDING or None
 
 
 # ---- ragged steps: several new tokens per sequence, packed rows ----------------
@@ -471,9 +485,10 @@ def paged_attention_prep(proj, start, k_pages, v_pages, page_table, kv_len, rope
     q_norm, k_norm [head_dim] ((1 + w) RMSNorm) or None. Returns q [total, q_heads, head_dim]."""
     import torch
     d = proj.get_device()
-    if d >= 0 and stream is None:
-        r = _binding().paged_attention_prep(Context.get(d).h.value, proj, start, k_pages, v_pages, page_table, kv_len,
-                                            rope, q_norm, k_norm, gated, eps, q_out)
+    short = _binding() if d >= 0 and stream is None else None
+    if short is not None:
+        r = short.paged_attention_prep(Context.get(d).h.value, proj, start, k_pages, v_pages, page_table, kv_len,
+                                       rope, q_norm, k_norm, gated, eps, q_out)
         if r is not None:
             return _checked(d, r)
     i32, f32, dt = torch.int32, torch.float32, k_pages.dtype
@@ -533,9 +548,10 @@ def paged_attention(q, start, k_pages, v_pages, page_table, kv_len, scale, gate=
     the caller's instead of one from the caching allocator."""
     import torch
     d = q.get_device()
-    if d >= 0 and stream is None:
-        r = _binding().paged_attention(Context.get(d).h.value, q, start, k_pages, v_pages, page_table, kv_len, scale,
-                                       gate, out, workspace)
+    short = _binding() if d >= 0 and stream is None else None
+    if short is not None:
+        r = short.paged_attention(Context.get(d).h.value, q, start, k_pages, v_pages, page_table, kv_len, scale,
+                                  gate, out, workspace)
         if r is not None:
             return _checked(d, r)
     i32, dt = torch.int32, k_pages.dtype
@@ -582,11 +598,12 @@ def deltanet_decode_span(layer, qkv, conv_state, state, a, b, z, start, counts=N
     (which may be state and conv_state) the state after each sequence's first counts[b] rows (None: all)."""
     import torch
     d = qkv.get_device()
-    if d >= 0 and stream is None:
-        r = _binding().deltanet_decode_span(Context.get(d).h.value, layer.num_heads, layer.key_dim, layer.value_dim,
-                                            layer.conv_kernel, layer.eps, layer.conv_weight, layer.a_log_bias,
-                                            layer.norm_weight, qkv, conv_state, state, a, b, z, start, counts,
-                                            state_out, conv_out, out)
+    short = _binding() if d >= 0 and stream is None else None
+    if short is not None:
+        r = short.deltanet_decode_span(Context.get(d).h.value, layer.num_heads, layer.key_dim, layer.value_dim,
+                                       layer.conv_kernel, layer.eps, layer.conv_weight, layer.a_log_bias,
+                                       layer.norm_weight, qkv, conv_state, state, a, b, z, start, counts,
+                                       state_out, conv_out, out)
         if r is not None:
             return _checked(d, r)
     f16, f32, i32 = torch.float16, torch.float32, torch.int32
@@ -640,9 +657,10 @@ def draft_verify(logits, tokens, start, u_accept, u_sample, temperature=None, dr
     drafts, the next token, then -1."""
     import torch
     d = logits.get_device()
-    if d >= 0 and stream is None:
-        r = _binding().draft_verify(Context.get(d).h.value, logits, tokens, start, u_accept, u_sample, temperature,
-                                    draft_probs, emitted, out_tokens, workspace)
+    short = _binding() if d >= 0 and stream is None else None
+    if short is not None:
+        r = short.draft_verify(Context.get(d).h.value, logits, tokens, start, u_accept, u_sample, temperature,
+                               draft_probs, emitted, out_tokens, workspace)
         if r is not None:
             return _checked(d, r)
     f32, i32, dt = torch.float32, torch.int32, logits.dtype

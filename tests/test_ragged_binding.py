@@ -70,3 +70,46 @@ def test_another_torch_has_a_binding_of_its_own(tree, monkeypatch):
     monkeypatch.setattr(torch, "__version__", "9.9.9")
     second = builder.build_binding()
     assert first != second and tree.runs == 2 and os.path.exists(first)
+
+
+def _unbuildable(*_, **__):
+    raise RuntimeError("no compiler here")
+
+
+def test_library_builds_without_the_binding(monkeypatch):
+    monkeypatch.setattr(builder, "build", lambda force=False: "the library")
+    monkeypatch.setattr(builder, "build_apps", lambda force=False: None)
+    monkeypatch.setattr(builder, "build_binding", _unbuildable)
+    with pytest.warns(UserWarning, match="no compiler here"):
+        assert spock_b200.build() == "the library"
+
+
+def test_wrappers_do_without_the_binding(monkeypatch):
+    """A binding that cannot be had is said once and not tried again; None sends the wrappers their own way."""
+    tried = []
+    monkeypatch.setattr(spock_b200, "_BINDING", None)
+    monkeypatch.setattr(builder, "build_binding", lambda *a, **k: tried.append(1) or _unbuildable())
+    with pytest.warns(UserWarning, match="no compiler here"):
+        assert spock_b200._binding() is None
+    assert spock_b200._binding() is None and len(tried) == 1
+
+
+def test_a_file_that_does_not_load_is_done_without(monkeypatch, tmp_path):
+    broken = tmp_path / "_binding.so"
+    broken.write_bytes(b"\x7fELF and no more")
+    monkeypatch.setattr(spock_b200, "_BINDING", None)
+    monkeypatch.setattr(builder, "build_binding", lambda *a, **k: str(broken))
+    with pytest.warns(UserWarning):
+        assert spock_b200._binding() is None
+
+
+@pytest.mark.gpu
+def test_calls_without_the_binding(cuda_ok, monkeypatch):
+    from tests.test_gpu_ragged import DEV, F16, Cache, _gen, _i32
+    g = _gen(2)
+    c, s = Cache([70, 9], 16, 2, 64, F16, g), _i32([0, 3, 4])
+    q = torch.randn(4, 8, 64, device=DEV, generator=g).half()
+    with_it = spock_b200.paged_attention(q, s, *c.args(), 0.125)
+    assert spock_b200._binding() is not None
+    monkeypatch.setattr(spock_b200, "_BINDING", False)
+    assert torch.equal(spock_b200.paged_attention(q, s, *c.args(), 0.125), with_it)
