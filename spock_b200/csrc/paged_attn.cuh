@@ -39,7 +39,7 @@ struct AttnArgs {
 };
 
 // Workspace: per CTA a Meta and two parts (its first and its last row tile).
-// A part: O [128][D] fp32, then the reference maxima (log2 units) and sums [128].
+// A part: O [128][D] fp32, then the references (part_reference) and sums [128].
 struct Meta {
   int slot;      // part of the row tile that begins in this CTA and ends in a later one, or -1
   int row0;      // its first packed row
@@ -50,7 +50,7 @@ struct Meta {
   int before;    // KV tiles of its first row tile that are in earlier CTAs
   int last;      // the last position that the part's first token sees (negative: none)
 };
-// What a part says its weights refer to (log2 units): -inf where it has none, so
+// What a part says its weights refer to (a score before its scale): -inf where it has none, so
 // that the join passes it over; a part whose scores are all NaN has weights (NaN),
 // relative to 0.
 __device__ __forceinline__ float part_reference(float m, float sum) {

@@ -227,12 +227,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- softmax: thread = position of the tile ----
     const int quad = warp & 3, at = quad * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
-    const float c = A.scale_log2;
+    const float c = A.scale_log2, lazy = kLazy / c;  // an infinite one (c < 2^-125): weights refer to 0 throughout
     // Rows in blocks of 4, of which a row tile has one to four; the loops over them
     // stay rolled and what they carry (references, sums) in shared memory: unrolled,
     // the kernel had 116 KB of code and waited for instructions first of all.
     float* const sum = reinterpret_cast<float*>(sm + Sh::kSums) + at;  // + r * 128
-    float* ref = s_ref;  // log2 units, the row tile's
+    float* ref = s_ref;  // in scores, before their scale (which could overflow); the row tile's
     int k = w.k0, item = 0, rows = 0;
     auto meet = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
     auto enter = [&] {
@@ -274,7 +274,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::tmem_ld4(tb + buf * NR + lane_off + r, s);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s[i] *= c;
             if (masked) {
               s[i] = lim >= 0 ? s[i] : -INFINITY;
               if (++n == A.G) n = 0, ++lim;
@@ -286,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool over = false;
       each([&](int r, const float(&s)[4]) {
         const float4 m = *reinterpret_cast<const float4*>(ref + r);
-        over |= s[0] - m.x > kLazy || s[1] - m.y > kLazy || s[2] - m.z > kLazy || s[3] - m.w > kLazy;
+        over |= s[0] - m.x > lazy || s[1] - m.y > lazy || s[2] - m.z > lazy || s[3] - m.w > lazy;
       });
       uint32_t any;
       asm volatile(
@@ -316,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float m = top_of(r + i), was = ref[r + i];
-            corr[i] = m - was > kLazy ? ex2(was - m) : 1.0f;
+            corr[i] = m - was > lazy ? ex2((was - m) * c) : 1.0f;
             sum[(r + i) * 128] *= corr[i];
           }
           if (begun) {
@@ -334,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         meet();  // all have read the references
         if (at < rows) {
           const float m = top_of(at);
-          if (m - ref[at] > kLazy) ref[at] = ref[2 * NR + at] = m;
+          if (m - ref[at] > lazy) ref[at] = ref[2 * NR + at] = m;
         }
         meet();
       }
@@ -343,8 +342,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int ch = (at & 63) >> 3;
       each([&](int r, const float(&s)[4]) {
         const float4 m = *reinterpret_cast<const float4*>(ref + 2 * NR + r);
-        const float x[4] = {ex2(s[0] - m.x + kUp<T>), ex2(s[1] - m.y + kUp<T>), ex2(s[2] - m.z + kUp<T>),
-                            ex2(s[3] - m.w + kUp<T>)};
+        const float x[4] = {ex2(fmaf(s[0] - m.x, c, kUp<T>)), ex2(fmaf(s[1] - m.y, c, kUp<T>)),
+                            ex2(fmaf(s[2] - m.z, c, kUp<T>)), ex2(fmaf(s[3] - m.w, c, kUp<T>))};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const T p = from_float<T>(x[i]);

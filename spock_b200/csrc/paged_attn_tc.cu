@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           float* part = parts + ((size_t)cta * 2 + slot) * part_floats<D>();
           if (half == 0 && row < rows) {
-            part[128 * D + row] = part_reference(m == -INFINITY ? m : m * c, lt);
+            part[128 * D + row] = part_reference(m, lt);
             part[128 * D + 128 + row] = lt;
           }
 #pragma unroll 1
@@ -474,8 +474,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the parts of each cut row tile, in share order: o = sum 2^{m_i - m} O_i /
-// sum 2^{m_i - m} l_i. The blocks of all its n shares (blockIdx.x) do it, the rows
+// Joins the parts of each cut row tile, in share order: o = sum e_i O_i /
+// sum e_i l_i, e_i = exp(scale (m_i - m)). The blocks of all its n shares (blockIdx.x) do it, the rows
 // dealt to the n gridDim.y of them: the one that continues in a share, then the
 // one that begins there. (With the first share's blocks alone, a call that ends in
 // 12 row tiles of 13 parts and 128 rows took 80 us, and 46 so.) Few parts: a warp
@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
         }
         const float to = fmaxf(fmaxf(fmaxf(mi[0], mi[1]), fmaxf(mi[2], mi[3])), m);
         if (to > m) {
-          const float f = ex2(m - to);
+          const float f = ex2((m - to) * A.scale_log2);
           l *= f;
 #pragma unroll
           for (int v = 0; v < V; ++v) acc[v] *= f;
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (mi[u] > -INFINITY) {  // not one without weights
-            const float f = ex2(mi[u] - m);
+            const float f = ex2((mi[u] - m) * A.scale_log2);
             l = fmaf(f, li[u], l);
             if (f != 0.f) {
 #pragma unroll
@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
 #pragma unroll
         for (int v = 0; v < V; ++v) acc[v] = 0.f;
         for (int k = 0; k < 8; ++k) {
-          const float f = s_m[k] > -INFINITY ? ex2(s_m[k] - to) : 0.f;
+          const float f = s_m[k] > -INFINITY ? ex2((s_m[k] - to) * A.scale_log2) : 0.f;
           l = fmaf(f, s_l[k], l);
 #pragma unroll
           for (int v = 0; v < V; ++v) acc[v] = fmaf(f, s_o[k][lane * V + v], acc[v]);

@@ -270,3 +270,24 @@ def test_named_streams_do_not_take_memory_in_use(cuda_ok):
         torch.cuda.synchronize()
         for x, y in zip(got, want):
             assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.parametrize("case", range(len(KERNELS)))
+def test_scales_that_take_scores_out_of_range(cuda_ok, case):
+    """Scaled scores that fp32 does not hold: a row is its largest score's value (or the average of equal ones)."""
+    c, q, starts = _case(case, 250)
+    c.k.copy_(torch.where(torch.isnan(c.k), math.nan, torch.round(c.k * 2)))
+    q.copy_(torch.round(q))  # whole numbers: scores are exact, the largest ones are equal or at least 1 apart
+    q[..., 16:] = 0
+    got = _attend(q, starts, c, 2.0 ** 125)
+    ref, mag, _ = _ref_attention(q, starts, c, 2.0 ** 125, None)
+    _check_attention(got, ref, mag, torch.zeros_like(mag))
+
+
+@pytest.mark.parametrize("case", range(len(KERNELS)))
+def test_scales_next_to_zero(cuda_ok, case):
+    """The smallest normal scale and subnormal ones: all positions weigh the same."""
+    c, q, starts = _case(case, 260)
+    for scale in (2.0 ** -126, 2.0 ** -140, 2.0 ** -149):
+        got = _attend(q, starts, c, scale)
+        _check_attention(got, *_ref_attention(q, starts, c, scale, None))
