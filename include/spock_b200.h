@@ -358,7 +358,7 @@ int spock_paged_attention_prep(spock_ctx* ctx, const spock_paged_kv* kv, int32_t
  *   are lost), the result rounded once
  *   q, gate rows and heads at their own strides (elements, multiples of 8;
  *           q's positive)
- *   scale   positive and finite
+ *   scale   positive and finite, also times log2(e)
  *   out     [total][q_heads][head_dim], contiguous
  * Slots behind kv_len are not used, whatever they hold; the positions below
  * it hold finite keys and values.

@@ -381,8 +381,8 @@ __attribute__((visibility("default"))) int spock_paged_attention(
   if ((total > 1 && (q_row_stride <= 0 || q_row_stride > kFar)) ||
       (q_heads > 1 && (q_head_stride <= 0 || q_head_stride > kFar)))
     return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "q strides must be positive (and at most 2^38)");
-  if (!(scale > 0.f && scale <= FLT_MAX))
-    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "scale must be positive and finite");
+  if (!(scale > 0.f && scale * spock::kLog2e <= FLT_MAX))
+    return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "scale must be positive and finite, also times log2(e)");
   if (workspace_bytes < spock::paged_attention_workspace(q_heads, kv->kv_heads, kv->head_dim, ctx->sms))
     return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "workspace too small");
   DeviceGuard dg(ctx->device);

@@ -722,7 +722,7 @@ Status launch_paged_attention(const spock_paged_kv& kv, int batch, const int32_t
   A.g_row = g_row * 2;
   A.g_head = g_head * 2;
   A.out = (uint8_t*)out;
-  A.scale_log2 = scale * 1.44269504088896341f;
+  A.scale_log2 = scale * kLog2e;
   A.ws = (float*)ws;
   A.err = err;
   // Either kernel is right for every batch; the rows that a sequence brings on

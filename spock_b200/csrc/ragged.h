@@ -5,6 +5,8 @@
 
 namespace spock {
 
+constexpr float kLog2e = 1.44269504088896341f;
+
 Status launch_paged_prep(const spock_paged_kv& kv, int batch, const int32_t* start, int64_t total, const void* proj,
                          int64_t proj_ld, int q_heads, bool gated, const void* q_norm, const void* k_norm, float eps,
                          const float* rope, int64_t rope_len, int rotary, void* q_out, int* err, cudaStream_t st);

@@ -291,3 +291,14 @@ def test_scales_next_to_zero(cuda_ok, case):
     for scale in (2.0 ** -126, 2.0 ** -140, 2.0 ** -149):
         got = _attend(q, starts, c, scale)
         _check_attention(got, *_ref_attention(q, starts, c, scale, None))
+
+
+def test_scales_that_overflow_with_log2e_are_refused(cuda_ok):
+    """The kernels work with scale * log2(e): one that makes that infinite would turn every row into NaN."""
+    c, q, starts = _case(0, 270)
+    top = torch.finfo(torch.float32).max
+    for scale in (top, top / 1.44, 2.4e38):
+        with pytest.raises(spock_b200.SpockError, match="positive and finite") as e:
+            _attend(q, starts, c, scale)
+        assert e.value.code == spock_b200.SPOCK_ERR_INVALID
+    assert not bool(torch.isnan(_attend(q, starts, c, top / 1.4427)).any())
