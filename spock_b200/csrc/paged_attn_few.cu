@@ -93,7 +93,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* parts = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(A.ws) + meta_bytes(ctas));
 
   if (tc::smem_u32(sm) & 1023) {  // never on this toolchain; the operand layouts need it
-    if (tid == 0) atomicExch(A.err, 6);
+    if (tid == 0) {
+      atomicExch(A.err, 6);
+      pdl_wait();
+      meta[cta].slot = -1, meta[cta].units = 0, meta[cta].before = 0;  // for the join: nothing here
+    }
     return;
   }
   if (tid == 0) {
