@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       atomicExch(A.err, 5);
       drain_ring(full, s_armed, NST);
     }
-    if (tid == 32 || tid == 64) {
+    if ((warp == 1 || warp == 2) && tc::elect_one()) {  // the threads that issued the MMAs: a commit is for its own
       tc::mma_commit(drain);
       tc::mbar_wait_bounded(drain, 0, kWait);
     }

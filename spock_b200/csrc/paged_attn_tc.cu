@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       drain_ring(full, s_armed, NST);
       if (s_armed[NST]) tc::mbar_wait_bounded(q_full, (s_armed[NST] - 1) & 1, kWait);
     }
-    if (tid == 32) {
+    if (warp == 1 && tc::elect_one()) {  // the thread that issued the MMAs: a commit is for its own
       tc::mma_commit(drain);
       tc::mbar_wait_bounded(drain, 0, kWait);
     }
