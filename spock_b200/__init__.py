@@ -524,19 +524,6 @@ def paged_attention_prep(proj, start, k_pages, v_pages, page_table, kv_len, rope
     return q_out
 
 
-def _workspace(ctx, query, key, like, stream):
-    """A workspace tensor from the caching allocator (so a captured graph keeps its own)."""
-    import torch
-    n = ctx.ws_bytes.get(key)
-    if n is None:
-        size = ctypes.c_size_t()
-        ctx.check(query(ctx.h, *key[1:], ctypes.byref(size)))
-        n = size.value
-        if len(ctx.ws_bytes) < 1024:  # sizes only, by shape
-            ctx.ws_bytes[key] = n
-    return _new((n,), torch.uint8, like, stream), n
-
-
 def paged_attention(q, start, k_pages, v_pages, page_table, kv_len, scale, gate=None, out=None, workspace=None,
                     stream=None):
     """Causal attention of each sequence's new tokens over its pages (spock_paged_attention).
