@@ -26,6 +26,7 @@
 
 #include "common.cuh"
 #include "tc.cuh"
+#include "tmap.h"
 
 namespace spock {
 namespace {
@@ -297,29 +298,13 @@ __global__ void __launch_bounds__(256, 1)
   if (warp == 0) tc::tmem_dealloc(tb, 512);
 }
 
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                             const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encode() {
-  static EncodeFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult qr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess &&
-        qr == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeFn>(p);
-  });
-  return fn;
-}
-
 }  // namespace
 
 // kv: the cache of this layer for every sequence, [batch][max_seq][K|V][2][256]
 // fp16 with sequence stride kv_seq_stride elements (kv points at this layer).
 Status launch_attn_prefill_tc(const void* q, const void* gate, const void* kv, int64_t kv_seq_stride, int max_seq,
                               const int* pos, float scale, void* out, int batch, int T, int* err, cudaStream_t st) {
-  EncodeFn fn = encode();
+  EncodeFn fn = tensor_map_encoder();
   if (!fn) return Status::err(SPOCK_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   if (((uintptr_t)kv & 15) || (kv_seq_stride * 2) % 16)
     return Status::err(SPOCK_ERR_INVALID, "attention prefill: KV cache must be 16-byte aligned");

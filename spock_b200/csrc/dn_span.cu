@@ -34,12 +34,12 @@
 
 #include <algorithm>
 #include <atomic>
-#include <mutex>
 
 #include "chunk_common.cuh"
 #include "ragged.cuh"
 #include "ragged.h"
 #include "tc.cuh"
+#include "tmap.h"
 
 namespace spock {
 namespace {
@@ -449,24 +449,9 @@ __global__ void __launch_bounds__(kThreads, 2) dn_span_kernel(const __grid_const
   }
 }
 
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                             const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encode() {
-  static EncodeFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult qr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess &&
-        qr == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeFn>(p);
-  });
-  return fn;
-}
 // All heads' states as [items * 128 rows][128], in boxes of 128 rows x 32 columns.
 bool encode_states(CUtensorMap* map, const float* state, int items) {
-  EncodeFn fn = encode();
+  EncodeFn fn = tensor_map_encoder();
   if (!fn) return false;
   cuuint64_t dims[2] = {kDim, (cuuint64_t)items * kDim}, strides[1] = {kDim * 4};
   cuuint32_t box[2] = {32, kDim}, estr[2] = {1, 1};

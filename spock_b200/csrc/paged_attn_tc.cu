@@ -38,10 +38,10 @@
 #include <cuda.h>
 
 #include <atomic>
-#include <mutex>
 
 #include "paged_attn.cuh"
 #include "ragged.h"
+#include "tmap.h"
 
 namespace spock {
 Status launch_paged_few(int dtype, int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const paged::AttnArgs& A,
@@ -611,22 +611,6 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   }
 }
 
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                             const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encode() {
-  static EncodeFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult qr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qr) == cudaSuccess &&
-        qr == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeFn>(p);
-  });
-  return fn;
-}
-
 // Pages as [page][8-position group][64-dim block][position in group][64]: one
 // box of a piece's groups lands as [group][block][8][128 B], which both the
 // K-major and the MN-major operand layouts read with constant strides whatever
@@ -647,7 +631,7 @@ int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 template <typename T, int D>
 Status launch(const spock_paged_kv& kv, AttnArgs& A, bool few, int sms, cudaStream_t st) {
-  EncodeFn fn = encode();
+  EncodeFn fn = tensor_map_encoder();
   if (!fn) return Status::err(SPOCK_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   A.tp = (few ? kFewRows : 128) / A.G;
   // a part of 128 rows is dear, one of 20 (five drafts of 4 heads) not: equal shares 65.6 us, moved borders 70.5
