@@ -22,7 +22,6 @@
 // the CTA lets its copies and MMAs land, releases TMEM and leaves.
 #include <cuda.h>
 
-#include <mutex>
 
 #include "common.cuh"
 #include "tc.cuh"

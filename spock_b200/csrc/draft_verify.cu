@@ -464,6 +464,7 @@ __global__ void __launch_bounds__(kT, kResident) verify_pick_kernel(const Verify
       return kReject;
     }
     if (greedy) return (p.best == 0x7fffffff ? 0 : p.best) == d ? kAccept : kReject;
+    if (sure > 0.0 && !(c < INFINITY)) return kUnsure;  // T below 2^-127: the Z of 32 bits counts equal logits only
     const Top top = top_of(p.top);
     const float x = load_as_f32(logits + r * A.logits_ld, d);
     const double e = top.count ? (double)(x > top.least) : top.weight(x, s_tab);

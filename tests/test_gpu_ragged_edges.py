@@ -8,7 +8,7 @@ import torch
 
 import spock_b200
 from tests.test_gpu_ragged import (BF16, DEV, F16, Cache, _check_attention, _gen, _half_step, _i32, _ref_attention,
-                                   _span_inputs, _starts, _verify_inputs)
+                                   _ref_verify, _run_verify, _span_inputs, _starts, _verify_inputs)
 
 pytestmark = pytest.mark.gpu
 
@@ -302,3 +302,16 @@ def test_scales_that_overflow_with_log2e_are_refused(cuda_ok):
             _attend(q, starts, c, scale)
         assert e.value.code == spock_b200.SPOCK_ERR_INVALID
     assert not bool(torch.isnan(_attend(q, starts, c, top / 1.4427)).any())
+
+
+def test_draft_verify_at_subnormal_temperatures(cuda_ok):
+    """Logits and temperatures so small that log2(e) / T is not an fp32 number: 64 bits still tell the logits apart."""
+    rows, vocab = [2] * 8, 1000
+    logits = -torch.arange(vocab, device=DEV).repeat(16, 1).float() * 2.0 ** -149
+    tokens = torch.tensor([0, 5] * 8, dtype=torch.int32, device=DEV)
+    ua = torch.linspace(0.0, 0.01, 16, device=DEV)
+    us = torch.linspace(0.0, 0.99, 8, device=DEV)
+    temp = torch.tensor([2.0 ** -140, 2.0 ** -149] * 4, device=DEV)
+    starts = _starts(rows)
+    got = _run_verify(logits, tokens, starts, ua, us, temp, None)
+    assert got == _ref_verify(logits, tokens, starts, ua, us, temp, None)
