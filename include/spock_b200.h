@@ -376,10 +376,11 @@ int spock_paged_attention_workspace(spock_ctx* ctx, int32_t q_heads, int32_t kv_
  * only where asked, so drafted tokens can be verified (outputs, no state) and
  * the accepted ones committed afterwards (state, no outputs). Per token: the
  * conv window, SiLU, L2 of q and k, g and beta, S <- e^g S + k d^T with
- * d = beta (v - (e^g S)^T k), o = S^T q / sqrt(key_dim), gated RMSNorm. All of
- * it in fp32, rounded to fp16 once (the single-token step also rounds the conv
- * output, q, k and w*norm, as the shaders store them). key_dim = value_dim =
- * 128, conv width 4.
+ * d = beta (v - (e^g S)^T k), o = S^T q / sqrt(key_dim), gated RMSNorm. Sums,
+ * norms, gates and states in fp32; operands of the products with keys, queries
+ * and the state as two tf32 parts (some 21 of fp32's 24 bits); outputs rounded
+ * to fp16 once (the single-token step also rounds the conv output, q, k and
+ * w*norm, as the shaders store them). key_dim = value_dim = 128, conv width 4.
  *   qkv     [total] rows of conv_dim fp16, qkv_ld elements apart; not changed
  *   a, b    [total] rows of num_heads fp16, ab_ld apart; z [total] rows of
  *           num_heads*128 fp16, z_ld apart (NULL when out is NULL)
@@ -407,9 +408,12 @@ int spock_deltanet_decode_span(spock_ctx* ctx, const spock_dn_layer* layer, int3
  * that is zero everywhere), or from p at the last row when all were accepted:
  * the lowest j with weight > 0 whose inclusive running sum exceeds
  * u_sample[b] * (sum of the weights), the last j with weight > 0 if none does.
- * temperature[b] <= 0: greedy, a draft is accepted iff it is the arg max
- * (lowest index among equals), which is also the next token. Decided in 64
- * bits. NaN logits count as -inf.
+ * temperature[b] <= 0 (or NaN): greedy, a draft is accepted iff it is the arg
+ * max (lowest index among equals), which is also the next token. Sums and
+ * comparisons in 64 bits, of weights good to 1.5e-13 of their value; one below
+ * 2^-1000 of its row's largest counts as 0. NaN logits count as -inf. A draft
+ * behind the first one that is not accepted is not looked at, nor is its token
+ * id checked.
  *   logits [total] rows of vocab, logits_ld apart (fp32, fp16, bf16)
  *   tokens int32 [total]; draft_probs fp32 [total] rows, probs_ld apart (a
  *   sequence's last row is not read) or NULL

@@ -1,6 +1,6 @@
 // Several tokens per sequence through a Gated DeltaNet layer's mixer core
 // (spock_deltanet_decode_span). Per token t of a head, with S the 128 x 128
-// state (key x value), in fp32 throughout:
+// state (key x value), sums, norms and states in fp32:
 //   y = silu(conv4(x)), q = y_q / |y_q| / sqrt(128), k = y_k / |y_k|, v = y_v
 //   S <- e^{g_t} S;  d_t = beta_t (v_t - S^T k_t);  S <- S + k_t d_t^T;  o_t = S^T q_t
 //   out = rmsnorm(o) * w * silu(z)

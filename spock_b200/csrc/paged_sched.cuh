@@ -1,15 +1,15 @@
 // How spock_paged_attention cuts a ragged batch into equal shares.
 //
 // A row tile is `tp` whole tokens of one sequence times the G query heads of one
-// kv head (tp = R / G, at most R = 128 rows, or 16 or 32 in the kernel for few
-// rows); its work is the KV tiles of kTile
-// positions that its last token sees, at least one (a row tile that sees
-// nothing still has zeros to write). Starting and finishing a row tile takes as
-// long as `extra` KV tiles. All row tiles' units (extra, then KV tiles), in the
+// kv head (tp = R / G; R = 128, or 16 in the kernel for few rows); its work is
+// the KV tiles of kTile positions that its last token sees, at least one (a row
+// tile that sees nothing still has zeros to write). Starting and finishing a row
+// tile takes as long as `extra` KV tiles. All row tiles' units (extra, then KV tiles), in the
 // order sequence, kv head, row tile, form one line; share c of C is units
-// [U c / C, U (c + 1) / C), its borders moved off short row tiles. A row tile cut by a border is computed in parts and joined afterwards, so one long
-// sequence, many short ones and any mix all keep every SM busy without the host
-// knowing any length.
+// [U c / C, U (c + 1) / C); where parts are dear its borders are moved off short
+// row tiles (enter_share). A row tile cut by a border is computed in parts and
+// joined afterwards, so one long sequence, many short ones and any mix all keep
+// every SM busy without the host knowing any length.
 #pragma once
 #include <stdint.h>
 
