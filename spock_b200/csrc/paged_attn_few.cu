@@ -1,21 +1,22 @@
-// spock_paged_attention for few query rows a sequence (decode tokens, drafts):
-// the tensor-core tile turned over.
+// spock_paged_attention for batches of decode tokens with small groups at head
+// size 256: the tensor-core tile turned over.
 //
 // With 128 query rows on the M side (paged_attn_tc.cu) a decode token's 4 rows
-// would leave 124 lanes of every softmax and output instruction idle (93 us for
-// 256 sequences of 65 to 1150 positions, and 74 here). Here M is the cache's side,
+// leave 124 lanes of every softmax and output instruction idle, which shows where
+// row tiles are short (launch_paged_attention has both kernels' times, and the
+// rule between them). Here M is the cache's side,
 // and N the rows, 16:
 //   S^T = K Q^T   M = 128 positions  N = rows  K = head dims
-//   O^T += V^T P^T  M = 128 dims (twice at head size 256)  N = rows  K = positions
+//   O^T += V^T P^T  M = 128 dims, twice  N = rows  K = positions
 // K and V come straight from their tiles as the A operands (V M-major), the
 // queries and the weights are the small B operands in shared memory. A softmax
 // thread takes one position's scores, four rows at a time; no maximum crosses
 // lanes unless a score exceeds its row's reference by 2^8, which one barrier with
 // a vote finds out for the block. O^T has dims on the lanes, so outputs and gates
 // are read and written in whole rows. Meant to be bound by the cache's bytes: an
-// SM streams a tile (128 positions, 128 KB at head size 256) in some 5700 cycles
-// of HBM's time, its MMAs take 2300. The 256 sequences take 1.5 times those bytes'
-// time: starting, the last tiles and the join are some 15 us, and the ring holds
+// SM streams a tile (128 positions, 128 KB) in some 5700 cycles
+// of HBM's time, its MMAs take 2300. 256 sequences of 65 to 1150 positions take 1.5
+// times those bytes' time: starting, the last tiles and the join are some 15 us, and the ring holds
 // little more than one tile, so every wait on the way shows. Separate rings for K
 // and V (3 + 3 or 4 + 2 stages) were slower (81 and 83 us).
 //
@@ -40,11 +41,12 @@ constexpr int NR = kFewRows;
 
 template <int D>
 struct Few {
+  static_assert(D == 256, "head size");
   static constexpr int DB = 128, KS = D / DB, VP = kTile / KS;
   static constexpr int kStage = kTile * DB * 2;
   static constexpr int kQ = NR * D * 2;       // one of two query buffers: [64-dim block][row][128 B]
   static constexpr int kP = NR * kTile * 2;   // one of two weight buffers: [64-position block][row][128 B]
-  static constexpr int NST = D == 256 ? 5 : 6;
+  static constexpr int NST = 5;
   static constexpr int kRing = 2 * kQ + 2 * kP;
   static constexpr int kBar = kRing + NST * kStage;
   static constexpr int kStat = kBar + 576;    // [2 row tiles][4 warps][NR] sums, [2][2][NR] references
@@ -514,17 +516,12 @@ Status launch(const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& A, i
   return Status::ok();
 }
 
-template <typename T>
-Status by_size(int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const AttnArgs& A, int sms, cudaStream_t st) {
-  return head_dim == 128 ? launch<T, 128>(mk, mv, A, sms, st) : launch<T, 256>(mk, mv, A, sms, st);
-}
-
 }  // namespace
 
-Status launch_paged_few(int dtype, int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const paged::AttnArgs& A,
-                        int sms, cudaStream_t st) {
-  if (dtype == SPOCK_F16) return by_size<__half>(head_dim, mk, mv, A, sms, st);
-  return by_size<__nv_bfloat16>(head_dim, mk, mv, A, sms, st);
+Status launch_paged_few(int dtype, const CUtensorMap& mk, const CUtensorMap& mv, const paged::AttnArgs& A, int sms,
+                        cudaStream_t st) {
+  if (dtype == SPOCK_F16) return launch<__half, 256>(mk, mv, A, sms, st);
+  return launch<__nv_bfloat16, 256>(mk, mv, A, sms, st);
 }
 
 }  // namespace spock

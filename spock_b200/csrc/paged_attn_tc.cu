@@ -44,8 +44,8 @@
 #include "tmap.h"
 
 namespace spock {
-Status launch_paged_few(int dtype, int head_dim, const CUtensorMap& mk, const CUtensorMap& mv, const paged::AttnArgs& A,
-                        int sms, cudaStream_t st);
+Status launch_paged_few(int dtype, const CUtensorMap& mk, const CUtensorMap& mv, const paged::AttnArgs& A, int sms,
+                        cudaStream_t st);
 
 namespace {
 
@@ -634,7 +634,11 @@ Status launch(const spock_paged_kv& kv, AttnArgs& A, bool few, int sms, cudaStre
   EncodeFn fn = tensor_map_encoder();
   if (!fn) return Status::err(SPOCK_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   A.tp = (few ? kFewRows : 128) / A.G;
-  // a part of 128 rows is dear, one of 20 (five drafts of 4 heads) not: equal shares 65.6 us, moved borders 70.5
+  // A part of 128 rows is dear, one of 20 (five drafts of 4 heads) not. us with moved borders / equal shares by the
+  // rows of a sequence, back to back, 256 sequences of 65 to 1150 positions: head size 256, groups of 4: 20 rows
+  // 86.2 / 80.6, 48 89.0 / 86.9, 64 90.4 / 90.5, 96 91.8 / 96.7, 128 93.4 / 104, 512 262 / 280; head size 128: 32
+  // 94.4 / 92.4, 48 96.5 / 99.0, 64 96.2 / 97.6, 128 100 / 109. Of longer ones (64 of 130 to 4000) equal shares are
+  // ahead up to 200 rows (head size 256: 64 71.6 / 71.4, 200 127 / 115; 128: 64 81.5 / 71.8, 200 149 / 127).
   A.whole = !few && A.total * (int64_t)A.G > 64 * (int64_t)A.batch;
   A.extra = 3;
   A.piece_k = gcd(kv.page_size, kTile);
@@ -644,8 +648,8 @@ Status launch(const spock_paged_kv& kv, AttnArgs& A, bool few, int sms, cudaStre
       encode_pages(fn, &mv, kv, kv.v, A.piece_v, D) != CUDA_SUCCESS)
     return Status::err(SPOCK_ERR_CUDA, "spock_paged_attention: tensor map encoding failed");
   cudaError_t e;
-  if (few) {
-    const Status s = launch_paged_few(kv.dtype, D, mk, mv, A, sms, st);
+  if (D == 256 && few) {
+    const Status s = launch_paged_few(kv.dtype, mk, mv, A, sms, st);
     if (s.code) return s;
   } else {
     // the attribute belongs to the kernel on the current device: set once on each
@@ -713,12 +717,21 @@ Status launch_paged_attention(const spock_paged_kv& kv, int batch, const int32_t
   A.scale_log2 = scale * kLog2e;
   A.ws = (float*)ws;
   A.err = err;
-  // Either kernel is right for every batch; the rows that a sequence brings on
-  // average decide. One token each over 256 sequences takes 74 us in the few-row
-  // kernel and 93 in the wide one; five tokens each (64 sequences) 67 in the wide
-  // one, and 89 in a few-row kernel of 32 rows, which is not kept. Head size 64
-  // would leave half of the few-row kernel's output tile empty.
-  const bool few = kv.head_dim >= 128 && total <= batch && A.G <= kFewRows;
+  // Either kernel is right for every batch. us of the few-row / the wide one, back to
+  // back over caches beyond L2, 2 kv heads, "short" 65 to 1150 positions, "long" 130
+  // to 4000:
+  //   head size 256, one token each, 4 query heads a group
+  //     sequences          64          128          192          256          512
+  //     short       33.2 / 37.0  47.0 / 47.1  59.9 / 61.8  74.4 / 76.1  130.9 / 132.8
+  //     long        62.4 / 61.5   101 / 101    142 / 143    184 / 187    350 / 365
+  //     1 sequence of 577 18.6 / 17.6; 8 of 8000 43.1 / 43.1; 1000 of up to 300 129 / 137
+  //   other groups, 256 short: 1 73.9 / 76.3, 3 73.8 / 76.4, 6 78.3 / 77.4, 8 79.9 / 77.7,
+  //     16 99.0 / 79.3
+  //   more tokens each, 256 short, group of 4: 2 79.6 / 77.2, 3 89.4 / 77.6, 4 98.4 / 78.6
+  //   head size 128, group of 4: 64 short 32.9 / 32.8, long 44.8 / 42.0; 256 short
+  //     57.2 / 56.1, long 114 / 106; group of 8, 256 short 67.5 / 56.4
+  // At head size 64 half of the few-row kernel's output tile would be empty.
+  const bool few = kv.head_dim == 256 && total <= batch && batch >= 64 && A.G <= 4;
   if (kv.dtype == SPOCK_F16) {
     if (kv.head_dim == 64) return launch<__half, 64>(kv, A, few, sms, st);
     if (kv.head_dim == 128) return launch<__half, 128>(kv, A, few, sms, st);

@@ -47,12 +47,17 @@ def test_deltanet_decode_span_at_odd_offsets(cuda_ok):
 
 # dtype, head_dim, q_heads, kv_heads, new tokens, lengths: both kernels, row tiles of one CTA and of several
 KERNELS = [
-    (F16, 128, 8, 2, [1, 1], [100, 40]),         # few rows, whole
-    (BF16, 256, 8, 2, [1], [40000]),             # few rows, in parts
-    (F16, 128, 6, 2, [1, 1], [30000, 700]),      # the same with pad rows
-    (BF16, 128, 8, 2, [5, 9], [100, 40]),        # wide, whole
-    (F16, 256, 8, 2, [40], [9000]),              # wide, in parts
+    (F16, 128, 8, 2, [1, 1], [100, 40]),
+    (BF16, 256, 8, 2, [1], [40000]),
+    (F16, 128, 6, 2, [1, 1], [30000, 700]),
+    (BF16, 128, 8, 2, [5, 9], [100, 40]),
+    (F16, 256, 8, 2, [40], [9000]),
     (BF16, 64, 4, 2, [3, 1], [5000, 4]),
+    # the kernel for few rows: 64 sequences and more, no more tokens than those, head size 256, groups up to 4
+    (F16, 256, 8, 2, [1] * 70, [100 - i for i in range(70)]),
+    (BF16, 256, 8, 2, [1, 1] + [0] * 70, [40000, 77] + [0] * 70),
+    (F16, 256, 6, 2, [1, 0, 1] + [0] * 70, [30000, 5, 700] + [0] * 70),
+    (BF16, 256, 4, 4, [3, 1, 40] + [0] * 70, [5000, 4, 1700] + [0] * 70),
 ]
 
 
@@ -315,3 +320,38 @@ def test_draft_verify_at_subnormal_temperatures(cuda_ok):
     starts = _starts(rows)
     got = _run_verify(logits, tokens, starts, ua, us, temp, None)
     assert got == _ref_verify(logits, tokens, starts, ua, us, temp, None)
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 4])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_batches_of_few_rows(cuda_ok, group, dtype):
+    """The kernel for decode batches: lengths of zero and one, ends on and beside a tile's border, sequences with
+    nothing and with several tokens among them, pages either way round, gates; the same bits every time."""
+    g = _gen(300 + group)
+    new = [1] * 90 + [0, 5, 0, 0, 17, 0, 0, 0, 2, 0, 0, 0] + [0] * 30
+    lens = ([0, 1, 2, 127, 128, 129, 130, 255, 256, 257, 4000] * 9)[:90] + [7, 3, 0, 200, 300, 1, 1, 128, 2, 0, 5, 9] + [3] * 30
+    c = Cache(lens, 16 if group % 2 else 24, 2, 256, dtype, g, head_major=group > 2)
+    starts, total = _starts(new), sum(new)
+    rows = torch.randn(total + 2, 2 * group, 2, 256, device=DEV, generator=g).to(dtype)
+    q, gate = rows[:, :, 0], rows[:, :, 1]
+    out = torch.full((total + 2, 2 * group, 256), 7.0, dtype=dtype, device=DEV)
+    assert total + 2 <= len(new)
+    spock_b200.paged_attention(q, _i32(starts), *c.args(), 0.0625, gate=gate, out=out)
+    spock_b200.Context.get(0).sync()
+    assert bool((out[total:] == 7.0).all())
+    ref = _ref_attention(q, starts, c, 0.0625, gate)
+    _check_attention(out[:total], *(t[:total] for t in ref))
+    for _ in range(3):
+        assert torch.equal(spock_b200.paged_attention(q, _i32(starts), *c.args(), 0.0625, gate=gate)[:total], out[:total])
+
+
+def test_nan_queries_of_few_rows_that_see_nothing(cuda_ok):
+    g = _gen(5)
+    c = Cache([7] + [1] * 70, 16, 2, 256, F16, g)
+    q = torch.randn(10, 8, 256, device=DEV, generator=g).half()
+    q[0, 1], q[1, 2, 3] = math.nan, math.inf
+    got = _attend(q, _starts([10] + [0] * 70), c, 0.0625)
+    assert bool((got[:3] == 0).all())
+    q[:2] = 0
+    ref = _ref_attention(q, _starts([10] + [0] * 70), c, 0.0625, None)
+    _check_attention(got[3:], *(t[3:] for t in ref))
