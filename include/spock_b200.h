@@ -348,9 +348,10 @@ int spock_paged_attention_prep(spock_ctx* ctx, const spock_paged_kv* kv, int32_t
 /* Attention of each sequence's new tokens over its pages: token t of n sees
  * positions 0 .. kv_len - n + t (causal; none if that is negative: the row is
  * then zero), q_heads a multiple of kv_heads, at most 128 query heads per kv
- * head. One entry for decode tokens, drafts, prompt chunks and any mix; the
- * kernel is chosen by total against batch, so a prompt chunk runs slower in a
- * batch that is mostly sequences without new tokens.
+ * head. One entry for decode tokens, drafts, prompt chunks and any mix. At head
+ * size 256 a batch of 64 sequences and more with no more tokens than those goes
+ * to a kernel for decode tokens, where a prompt chunk among sequences without
+ * new tokens runs slower.
  *   out[r][h] = sum_p softmax_p(scale * q[r][h] . k_p) v_p, times
  *   sigmoid(gate[r][h]) when gate is not NULL; scores, sums and outputs in
  *   fp32, the weights exp(score - about the row's largest) rounded to the

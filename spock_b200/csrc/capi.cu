@@ -345,7 +345,7 @@ __attribute__((visibility("default"))) int spock_paged_attention_prep(
   DeviceGuard dg(ctx->device);
   if (!dg.ok) return fail(ctx, SPOCK_ERR_CUDA, std::string(op) + "cannot select device");
   return finish(ctx, spock::launch_paged_prep(*kv, batch, start, total, proj, proj_ld, q_heads, gated != 0, q_norm,
-                                              k_norm, eps, rope, rope_len, rotary, q_out, ctx->d_err_flag,
+                                              k_norm, eps, rope, rope_len, rotary, q_out, ctx->sms, ctx->d_err_flag,
                                               (cudaStream_t)stream));
 }
 
@@ -434,7 +434,7 @@ __attribute__((visibility("default"))) int spock_draft_verify_workspace(spock_ct
   if (!ctx) return fail(nullptr, SPOCK_ERR_INVALID, "spock_draft_verify_workspace: ctx is NULL");
   if (!bytes || total < 0 || vocab <= 0 || batch <= 0)
     return fail(ctx, SPOCK_ERR_INVALID, "spock_draft_verify_workspace: bad arguments");
-  *bytes = spock::draft_verify_workspace(total, vocab, batch);
+  *bytes = spock::draft_verify_workspace(total, vocab, ctx->sms);
   return SPOCK_OK;
 }
 
@@ -460,12 +460,12 @@ __attribute__((visibility("default"))) int spock_draft_verify(
     return fail(ctx, SPOCK_ERR_INVALID,
                 std::string(op) + "emitted and out_tokens must not overlap tokens, start or each other");
   if (batch > (1 << 27)) return fail(ctx, SPOCK_ERR_UNSUPPORTED, std::string(op) + "at most 2^27 sequences");
-  if (workspace_bytes < spock::draft_verify_workspace(total, vocab, batch))
+  if (workspace_bytes < spock::draft_verify_workspace(total, vocab, ctx->sms))
     return fail(ctx, SPOCK_ERR_INVALID, std::string(op) + "workspace too small");
   DeviceGuard dg(ctx->device);
   if (!dg.ok) return fail(ctx, SPOCK_ERR_CUDA, std::string(op) + "cannot select device");
   spock::VerifyArgs v{logits, logits_ld, total, vocab, batch, start, tokens, draft_probs, probs_ld, temperature,
-                      u_accept, u_sample, emitted, out_tokens, workspace, ctx->d_err_flag};
+                      u_accept, u_sample, emitted, out_tokens, workspace, ctx->sms, ctx->d_err_flag};
   return finish(ctx, spock::launch_draft_verify(dtype, v, (cudaStream_t)stream));
 }
 

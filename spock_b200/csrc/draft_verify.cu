@@ -122,10 +122,10 @@ __device__ __forceinline__ float rebase(float z, float m, float to, float c) {
   return m == to ? z : z * ex2((m - to) * c);
 }
 
-int stat_splits(int64_t total, int64_t vocab) {
+int stat_splits(int64_t total, int64_t vocab, int sms) {
   // a wave of 8 CTAs an SM (more cost more than they hide), at least 8192 logits each; and no
   // thread sums more than kThreadTerms terms
-  const int64_t want = total > 0 ? (148 * 8 + total - 1) / total : 1, most = (vocab + 8191) / 8192;
+  const int64_t want = total > 0 ? (sms * 8 + total - 1) / total : 1, most = (vocab + 8191) / 8192;
   const int64_t least = (vocab + kThreadTerms * kT / 2 - 1) / (kThreadTerms * kT / 2);
   return (int)std::max(least, std::min(want, most));
 }
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kT, kResident) verify_pick_kernel(const Verify
 
 template <typename T>
 Status launch(const VerifyArgs& a, cudaStream_t st) {
-  const int splits = stat_splits(a.total, a.vocab);
+  const int splits = stat_splits(a.total, a.vocab, a.sms);
   cudaError_t e = cudaSuccess;
   if (a.total > 0) {
     e = launch_k(verify_stats_kernel<T>, dim3((unsigned)(a.total * splits)), dim3(kT), 0, st, a, splits);
@@ -655,7 +655,7 @@ Status launch(const VerifyArgs& a, cudaStream_t st) {
   }
   // a CTA per 8192 logits of a row, up to the portable cluster size, while all are resident at once
   const int64_t most = std::min<int64_t>(kCluster, (a.vocab + 8191) / 8192);
-  const int ranks = (int)std::max<int64_t>(1, std::min<int64_t>(most, 148 * kResident / a.batch));
+  const int ranks = (int)std::max<int64_t>(1, std::min<int64_t>(most, a.sms * kResident / a.batch));
   pdl_scope overlap;  // its launch and table run under the first kernel
   e = launch_k_cluster(verify_pick_kernel<T>, dim3((unsigned)a.batch * ranks), dim3(kT), dim3(ranks), 0, st, a,
                        splits);
@@ -666,8 +666,8 @@ Status launch(const VerifyArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-size_t draft_verify_workspace(int64_t total, int64_t vocab, int) {
-  return (size_t)total * stat_splits(total, vocab) * sizeof(Part) + 16;
+size_t draft_verify_workspace(int64_t total, int64_t vocab, int sms) {
+  return (size_t)total * stat_splits(total, vocab, sms) * sizeof(Part) + 16;
 }
 
 Status launch_draft_verify(int dtype, const VerifyArgs& a, cudaStream_t st) {

@@ -167,12 +167,13 @@ Status by_type(int dtype, int head_dim, F f) {
 
 Status launch_paged_prep(const spock_paged_kv& kv, int batch, const int32_t* start, int64_t total, const void* proj,
                          int64_t proj_ld, int q_heads, bool gated, const void* q_norm, const void* k_norm, float eps,
-                         const float* rope, int64_t rope_len, int rotary, void* q_out, int* err, cudaStream_t st) {
+                         const float* rope, int64_t rope_len, int rotary, void* q_out, int sms, int* err,
+                         cudaStream_t st) {
   return by_type(kv.dtype, kv.head_dim, [&](auto t, auto d) -> Status {
     using T = decltype(t);
     // two waves of 6 CTAs an SM; a head each while there are few tokens
     const int64_t heads = q_heads + kv.kv_heads, ctas = (total + 7) / 8;
-    const int64_t split = std::max<int64_t>(1, std::min<int64_t>(heads, 2 * 148 * 6 / ctas));
+    const int64_t split = std::max<int64_t>(1, std::min<int64_t>(heads, 2 * sms * 6 / ctas));
     const cudaError_t e =
         launch_k(paged_prep_kernel<T, decltype(d)::value>, dim3((unsigned)ctas, (unsigned)split), dim3(256), 0, st,
                  cache_of(kv), batch, start, (int)total, (const T*)proj, proj_ld, q_heads, (int)gated,

@@ -9,7 +9,8 @@ constexpr float kLog2e = 1.44269504088896341f;
 
 Status launch_paged_prep(const spock_paged_kv& kv, int batch, const int32_t* start, int64_t total, const void* proj,
                          int64_t proj_ld, int q_heads, bool gated, const void* q_norm, const void* k_norm, float eps,
-                         const float* rope, int64_t rope_len, int rotary, void* q_out, int* err, cudaStream_t st);
+                         const float* rope, int64_t rope_len, int rotary, void* q_out, int sms, int* err,
+                         cudaStream_t st);
 
 size_t paged_attention_workspace(int q_heads, int kv_heads, int head_dim, int sms);
 Status launch_paged_attention(const spock_paged_kv& kv, int batch, const int32_t* start, int64_t total, int q_heads,
@@ -31,9 +32,10 @@ struct VerifyArgs {
   const float *temperature, *u_accept, *u_sample;
   int32_t *emitted, *out_tokens;
   void* ws;
+  int sms;
   int* err;
 };
-size_t draft_verify_workspace(int64_t total, int64_t vocab, int batch);
+size_t draft_verify_workspace(int64_t total, int64_t vocab, int sms);
 Status launch_draft_verify(int dtype, const VerifyArgs& a, cudaStream_t st);
 
 }  // namespace spock
