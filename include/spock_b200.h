@@ -316,7 +316,8 @@ typedef struct {
   int64_t table_stride;
   const int32_t* kv_len;     /* device [batch]: positions held, this call's new
                                 tokens included                                      */
-  int32_t table_width;       /* entries per row (<= table_stride)                    */
+  int32_t table_width;       /* entries per row (<= table_stride); times page_size:
+                                at most 2^31 - 256                                   */
   int32_t num_pages;
   int32_t page_size;         /* a multiple of 8                                      */
   int32_t kv_heads;

@@ -112,8 +112,8 @@ int check_paged(spock_ctx* ctx, const char* op, const spock_paged_kv* kv, int32_
   if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256)
     return fail(ctx, SPOCK_ERR_UNSUPPORTED, o + "head_dim is 64, 128 or 256");
   if (kv->page_size % 8) return fail(ctx, SPOCK_ERR_UNSUPPORTED, o + "page_size must be a multiple of 8");
-  if ((int64_t)kv->table_width * kv->page_size > INT32_MAX)
-    return fail(ctx, SPOCK_ERR_UNSUPPORTED, o + "at most 2^31 - 1 positions per sequence");
+  if ((int64_t)kv->table_width * kv->page_size > INT32_MAX - 255)  // a tile's end is still an int
+    return fail(ctx, SPOCK_ERR_UNSUPPORTED, o + "at most 2^31 - 256 positions per sequence");
   if (misaligned(kv->k, 16) || misaligned(kv->v, 16) || kv->page_stride <= 0 || kv->pos_stride <= 0 ||
       kv->head_stride <= 0 || kv->page_stride % 8 || kv->pos_stride % 8 || kv->head_stride % 64)
     return fail(ctx, SPOCK_ERR_INVALID,

@@ -355,3 +355,17 @@ def test_nan_queries_of_few_rows_that_see_nothing(cuda_ok):
     q[:2] = 0
     ref = _ref_attention(q, _starts([10] + [0] * 70), c, 0.0625, None)
     _check_attention(got[3:], *(t[3:] for t in ref))
+
+
+def test_tables_whose_last_tile_passes_31_bits_are_refused(cuda_ok):
+    pages = torch.zeros(1, 114808, 1, 64, dtype=F16, device=DEV)
+    table = torch.zeros(1, 18705, dtype=torch.int32, device=DEV)  # 2^31 - 8 positions
+    q, proj = torch.zeros(1, 4, 64, dtype=F16, device=DEV), torch.zeros(1, 6 * 64, dtype=F16, device=DEV)
+    one, s = _i32([1]), _i32([0, 1])
+    for call in (lambda t: spock_b200.paged_attention(q, s, pages, pages, t, one, 1.0),
+                 lambda t: spock_b200.paged_attention_prep(proj, s, pages, pages.clone(), t, one, gated=False)):
+        with pytest.raises(spock_b200.SpockError, match="positions per sequence") as e:
+            call(table)
+        assert e.value.code == spock_b200.SPOCK_ERR_UNSUPPORTED
+        call(table[:, :18704])
+        spock_b200.Context.get(0).sync()
