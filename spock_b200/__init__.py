@@ -417,6 +417,8 @@ def _whole(t, dtype, ndim, d):
 def _stream_of(d, stream):
     """The stream's handle; None: device d's current stream."""
     if stream is not None:
+        if stream.device.index != d:
+            _bad(f"stream: expected one of cuda:{d}, got one of {stream.device}")
         return stream.cuda_stream
     import torch
     return torch._C._cuda_getCurrentRawStream(d)

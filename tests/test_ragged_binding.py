@@ -1,5 +1,4 @@
-"""How the ragged steps' native binding is built and found, with the compiler played by the test."""
-import os
+"""How the ragged steps' native binding is built and found, with the compiler played by the test; the wrappers' streams."""
 import subprocess
 import threading
 import time
@@ -113,3 +112,11 @@ def test_calls_without_the_binding(cuda_ok, monkeypatch):
     assert spock_b200._binding() is not None
     monkeypatch.setattr(spock_b200, "_BINDING", False)
     assert torch.equal(spock_b200.paged_attention(q, s, *c.args(), 0.125), with_it)
+
+
+def test_streams_of_another_device_are_refused():
+    stream = types.SimpleNamespace(device=torch.device("cuda", 1), cuda_stream=77)
+    assert spock_b200._stream_of(1, stream) == 77
+    with pytest.raises(spock_b200.SpockError, match="stream: expected one of cuda:0") as e:
+        spock_b200._stream_of(0, stream)
+    assert e.value.code == spock_b200.SPOCK_ERR_INVALID
