@@ -1,4 +1,6 @@
-"""How the ragged steps' native binding is built and found, with the compiler played by the test; the wrappers' streams."""
+"""How the ragged steps' native binding is built and found, with the compiler
+played by the test; and which streams the wrappers take."""
+import os
 import subprocess
 import threading
 import time
