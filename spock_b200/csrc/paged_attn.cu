@@ -58,7 +58,8 @@ __device__ __forceinline__ void check_ragged(const Cache& c, int batch, const in
 // lane and a pair's two halves sit (r/2)/V lanes apart. The token's sequence,
 // position and table row are found once for all heads of a warp. Bound by issued
 // instructions, then by latency: 4112 tokens of 8 + 2 heads take 15.4 us with 3
-// or 4 heads a warp, 18.0 with one and 17.4 with all of them.
+// or 4 heads a warp, 18.0 with one and 17.4 with all of them (the same call again and
+// again; 17.5 us where inputs change from call to call).
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 6)
     paged_prep_kernel(Cache c, int batch, const int32_t* __restrict__ start, int total, const T* __restrict__ proj,

@@ -18,7 +18,7 @@
 // of HBM's time, its MMAs take 2300. 256 sequences of 65 to 1150 positions take 1.5
 // times those bytes' time: starting, the last tiles and the join are some 15 us, and the ring holds
 // little more than one tile, so every wait on the way shows. Separate rings for K
-// and V (3 + 3 or 4 + 2 stages) were slower (81 and 83 us).
+// and V (3 + 3 or 4 + 2 stages) were slower (81 and 83 us against 75).
 //
 // One CTA per SM walks its share (paged_attn.cuh). Warp roles:
 //   warps 0, 3  K tiles and V tiles by TMA into a ring

@@ -24,10 +24,11 @@
 //
 // Bound, at head size 256 with long sequences, by the K and V tiles' way from L2
 // and the one and a quarter tiles that the ring holds: 2048 tokens of 8 heads over
-// 16384 positions take 245 us, 0.61 of the measured rate of large matrix products;
+// 16384 positions take 286 us where inputs change from call to call, 0.52 of the
+// measured rate of large matrix products (247 us, 0.61, the same call again and again);
 // of a tile's 3900 cycles the MMAs take 2100, the softmax 2000 beside them, and
 // 1700 are waits for tiles. At head size 128 with short prompts (8 of 301 to 1021
-// tokens: 58 us) by starting and finishing row tiles of some three KV tiles each.
+// tokens: 59 us) by starting and finishing row tiles of some three KV tiles each.
 // The MMA thread is the one elected by the warp: the same code under `lane == 0`
 // goes through a loop over the lanes for each descriptor (333 us instead of 285).
 //
